@@ -1,0 +1,587 @@
+// Products of 8-bit codes with a power-of-two scale per 128 values of the contraction.
+//
+//   out[q, p] = sum_k  a[q, k] sa[q / ga, k / 128]  b[p, k] sb[p / gb, k / 128]   (+ add[q, p])      ga, gb: 1 or 128
+//
+// a holds Q rows (tokens; for a weight gradient the output channels), b holds P rows.  Either operand lies with k innermost
+// or with its rows innermost, so that a weight serves the forward product and the input gradient from one set of codes, and
+// a weight gradient reads activations and gradients as they lie.
+//
+// The tensor cores apply the scales (tcgen05.mma kind::mxf8f6f4): one byte per row and 32 values of k, taken from TMEM.  Four
+// instructions of 32 values go over a block of 128 with the same byte, so a 32-bit word of TMEM holds a row's scales of 512
+// values, and the word is what lies in memory: four warps load words and store them to TMEM, each to its quarter of the
+// lanes.
+//
+// The result is computed transposed: b's rows are the lanes of TMEM and a's the columns.  A thread then has one p and walks
+// over q, and the 32 lanes of a warp store 32 neighbours of a row of the output, whatever its alignment and pitch.
+//
+//  fp8_gemm_pair   two CTAs (cta_group::2) per tile of 256 p x 256 q, persistent
+//  fp8_gemm_split  one CTA per tile of 128 p x 16..128 q and part of k, for outputs too small to fill the GPU with pairs: the
+//                  CTAs of a cluster hold the parts of k and add them up in the order of k through distributed shared memory
+//
+// All sums are in fp32 and in a fixed order: the same bits in every run.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "fp8_common.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "smem_limit.h"
+#include "tmap.cuh"
+
+namespace dcpk {
+
+static constexpr int kGemmThreads = 512;   // TMA producer, UMMA issuer, 2 idle warps; 4 scale warps; 8 epilogue warps
+static constexpr int kGemmStages = 7;
+static constexpr int kTileBytes = 128 * 128;  // 128 rows x 128 values, or 128 values x 128 rows
+static constexpr int kScaleBufs = 4;          // of 512 values of k each
+static constexpr int kGemmPairs = 148 / 2;
+
+struct GemmOperand {
+  const uint8_t* scales;
+  long row_stride, k_stride;   // of the scales, in bytes
+  int shift;                   // 7: 128 rows share a scale
+  int rows;
+  int words;                   // four scales along k can be read as a 32-bit word
+};
+struct GemmArgs {
+  GemmOperand p, q;
+  int n_kb;                    // blocks of 128 values of k
+  void* out;
+  const void* add;             // null, or what the product is added to, of the output's type
+  long out_pitch, add_pitch;   // in elements
+  int out_type;
+  int tiles_p, tiles_q;
+  uint32_t idesc;
+  int* status;
+};
+
+// Instruction descriptor of kind::mxf8f6f4: [4,6) byte of B's scale word; [7,10) / [10,13) type of A / B (0 e4m3, 1 e5m2);
+// [15] / [16] A / B with rows innermost; [17,23) N >> 3; [23] scales are e8m0; [24,29) M >> 4; [29,31) byte of A's word.
+__host__ __device__ constexpr uint32_t make_idesc_mx(int M, int N, int a_type, int b_type, int a_mn, int b_mn) {
+  return (uint32_t(a_type) << 7) | (uint32_t(b_type) << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) |
+         (uint32_t(N >> 3) << 17) | (1u << 23) | (uint32_t(M >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t with_scale_byte(uint32_t idesc, uint32_t byte) { return idesc | (byte << 4) | (byte << 29); }
+
+__device__ __forceinline__ void umma_mx_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m, uint32_t cluster_bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(cluster_bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+
+// scales of a row (the last one's where it is past the end: those results are not stored) of blocks kb .. kb + 3
+__device__ __forceinline__ uint32_t scale_word(const GemmOperand& o, int row, int kb, int n_kb) {
+  const uint8_t* p = o.scales + long(min(row, o.rows - 1) >> o.shift) * o.row_stride + long(kb) * o.k_stride;
+  if (o.words && kb + 4 <= n_kb) return __ldg(reinterpret_cast<const uint32_t*>(p));
+  uint32_t v = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (kb + i < n_kb) v |= uint32_t(p[i * o.k_stride]) << (8 * i);
+  return v;
+}
+
+// one result (and what it is added to) in the output's type
+__device__ __forceinline__ void store_result(const GemmArgs& a, int q, int p, float v) {
+  const size_t at = size_t(q) * a.out_pitch + p, from = size_t(q) * a.add_pitch + p;
+  if (a.out_type == kTypeBf16) {
+    if (a.add) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.add)[from]);
+    static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+  } else if (a.out_type == kTypeF16) {
+    if (a.add) v += __half2float(static_cast<const __half*>(a.add)[from]);
+    static_cast<__half*>(a.out)[at] = __float2half_rn(v);
+  } else {
+    if (a.add) v += static_cast<const float*>(a.add)[from];
+    static_cast<float*>(a.out)[at] = v;
+  }
+}
+
+struct __align__(1024) GemmSmem {
+  uint8_t p[kGemmStages][kTileBytes];
+  uint8_t q[kGemmStages][kTileBytes];
+  // of the even CTA (bytes and arrivals of both): full, scale_full, acc_empty; the others are signalled in both
+  uint64_t full[kGemmStages], empty[kGemmStages], scale_full[kScaleBufs], scale_empty[kScaleBufs], acc_full, acc_empty;
+  uint32_t tmem_base;
+  int abort_word;
+};
+
+// Neighbouring tiles in time share operands in L2: eight tiles of q by as many of p as are under way.
+__device__ __forceinline__ void tile_at(int i, int tiles_p, int tiles_q, int& tp, int& tq) {
+  constexpr int kBand = 8;
+  const int band = i / (kBand * tiles_p), first = band * kBand, height = min(kBand, tiles_q - first), r = i - first * tiles_p;
+  tq = first + r % height;
+  tp = r / height;
+}
+
+template <bool kPMn, bool kQMn>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constant__ CUtensorMap tm_q,
+                     const __grid_constant__ GemmArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  GemmSmem& sm = *reinterpret_cast<GemmSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int X = blockIdx.x & 1;   // rank in the cluster
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_p);
+    tma_prefetch_desc(&tm_q);
+    for (int i = 0; i < kGemmStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
+    for (int i = 0; i < kScaleBufs; ++i) { mbar_init(&sm.scale_full[i], 8); mbar_init(&sm.scale_empty[i], 1); }
+    mbar_init(&sm.acc_full, 1);
+    mbar_init(&sm.acc_empty, 16);
+    sm.abort_word = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc_pair(&sm.tmem_base, 512);
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  grid_let_next();
+  grid_wait();
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* abort_word = &sm.abort_word;
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, n_tiles = args.tiles_p * args.tiles_q, n_kb = args.n_kb;
+  constexpr int kScaleCol = 256;   // TMEM: results [0, 256), scales of the buffers behind them, 4 columns of p, 8 of q each
+  // a CTA that gives up tells the other, which waits for it
+  auto wait = [&](uint64_t* bar, int parity) -> bool {
+    if (mbar_wait(bar, parity, abort_word)) return true;
+    st_cluster_u32(smem_u32(&sm.abort_word), X ^ 1, 1u);
+    return false;
+  };
+
+  if (warp >= 8) {
+    // ------------------------------------------------------------ epilogue: lane = p, 128 of the tile's q
+    // registers: 256 x 184 + 256 x 64 = 63488 of the 65536 the block is launched with
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const int quad = warp & 3, half = (warp - 8) >> 2;
+    const uint32_t addr = tmem + (uint32_t(quad * 32) << 16) + half * 128;
+    const uint32_t empty_bar = cluster_addr(smem_u32(&sm.acc_empty), 0);
+    int ph = 0;
+    for (int i = pair; i < n_tiles; i += n_pairs, ph ^= 1) {
+      int tp, tq;
+      tile_at(i, args.tiles_p, args.tiles_q, tp, tq);
+      if (!__all_sync(0xffffffffu, wait(&sm.acc_full, ph))) break;
+      tc_fence_after();
+      uint32_t acc[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(addr + c * 32, acc + c * 32);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(empty_bar);   // the results are in registers: the next tile's products may come
+      const int p = (tp * 2 + X) * 128 + quad * 32 + lane, q0 = tq * 256 + half * 128;
+      if (p < args.p.rows) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (q0 + c < args.q.rows) store_result(args, q0 + c, p, __uint_as_float(acc[c]));
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ scales: every warp to its quarter of the lanes
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int quad = warp & 3;
+    const uint32_t full_bar = cluster_addr(smem_u32(&sm.scale_full[0]), 0);
+    int buf = 0, ph = 1, used = 0;
+    bool ok = true;
+    for (int i = pair; i < n_tiles && ok; i += n_pairs) {
+      int tp, tq;
+      tile_at(i, args.tiles_p, args.tiles_q, tp, tq);
+      const int p0 = (tp * 2 + X) * 128 + lane, q0 = tq * 256 + lane;
+      for (int kb = 0; kb < n_kb; kb += 4) {
+        uint32_t wp[4], wq[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wp[j] = scale_word(args.p, p0 + 32 * j, kb, n_kb);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) wq[j] = scale_word(args.q, q0 + 32 * j, kb, n_kb);
+        ok = __all_sync(0xffffffffu, wait(&sm.scale_empty[buf], ph));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t to = tmem + (uint32_t(quad * 32) << 16) + kScaleCol + buf * 16;
+        tmem_st4(to, wp);
+        tmem_st8(to + 4, wq);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(full_bar + 8 * buf);
+        used |= 1 << buf;
+        if (++buf == kScaleBufs) { buf = 0; ph ^= 1; }
+      }
+    }
+    // what the even CTA's issuer signals has all come in before this CTA may retire
+    for (int i = 0; i < kScaleBufs && ok; ++i) {
+      if ((used >> buf) & 1) ok = wait(&sm.scale_empty[buf], ph);
+      if (++buf == kScaleBufs) { buf = 0; ph ^= 1; }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 0 && lane == 0) {
+      // ------------------------------------------------------------ TMA producer
+      const uint32_t full_bar = cluster_addr(smem_u32(&sm.full[0]), 0);
+      int stage = 0, ph = 1, used = 0;
+      bool ok = true;
+      for (int i = pair; i < n_tiles && ok; i += n_pairs) {
+        int tp, tq;
+        tile_at(i, args.tiles_p, args.tiles_q, tp, tq);
+        const int p0 = (tp * 2 + X) * 128, q0 = tq * 256 + X * 128;
+        for (int kb = 0; kb < n_kb; ++kb) {
+          ok = wait(&sm.empty[stage], ph);
+          if (!ok) break;
+          if (X == 0) mbar_expect_tx(&sm.full[stage], 4 * kTileBytes);
+          tma_load_2d_pair(sm.p[stage], &tm_p, full_bar + 8 * stage, kPMn ? p0 : kb * 128, kPMn ? kb * 128 : p0);
+          tma_load_2d_pair(sm.q[stage], &tm_q, full_bar + 8 * stage, kQMn ? q0 : kb * 128, kQMn ? kb * 128 : q0);
+          used |= 1 << stage;
+          if (++stage == kGemmStages) { stage = 0; ph ^= 1; }
+        }
+      }
+      for (int i = 0; i < kGemmStages && ok; ++i) {
+        if ((used >> stage) & 1) ok = wait(&sm.empty[stage], ph);
+        if (++stage == kGemmStages) { stage = 0; ph ^= 1; }
+      }
+      // copies already in flight get a millisecond to land before the CTAs retire
+      if (!ok)
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    } else if (warp == 1 && X == 0 && elect_one()) {
+      // ------------------------------------------------------------ UMMA issuer, for both CTAs
+      const uint64_t some = make_sdesc_sw128(0, 16, 1024);
+      const uint32_t hi = uint32_t(some >> 32);
+      const uint32_t p_lo = uint32_t(some) + sdesc_addr(sm.p[0]), q_lo = uint32_t(some) + sdesc_addr(sm.q[0]);
+      auto desc = [&](uint32_t lo) { return (uint64_t(hi) << 32) | lo; };
+      constexpr uint32_t kStep = kTileBytes >> 4;             // in a descriptor's 16-byte units
+      constexpr uint32_t kPK = kPMn ? 256 : 2, kQK = kQMn ? 256 : 2;   // 32 values of k
+      int stage = 0, ph = 0, buf = 0, sph = 0, aph = 1, done = 0;
+      bool ok = true;
+      for (int i = pair; i < n_tiles && ok; i += n_pairs) {
+        ok = wait(&sm.acc_empty, aph);   // the last tile's results are in registers
+        aph ^= 1;
+        for (int kb = 0; kb < n_kb && ok; ++kb) {
+          if ((kb & 3) == 0) ok = wait(&sm.scale_full[buf], sph);
+          ok = ok && wait(&sm.full[stage], ph);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t idesc = with_scale_byte(args.idesc, kb & 3), scales = tmem + kScaleCol + buf * 16;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_mx_pair(tmem, desc(p_lo + stage * kStep + k * kPK), desc(q_lo + stage * kStep + k * kQK), idesc, scales, scales + 4,
+                         (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit_pair(&sm.empty[stage]);
+          if ((kb & 3) == 3 || kb + 1 == n_kb) {
+            umma_commit_pair(&sm.scale_empty[buf]);
+            if (++buf == kScaleBufs) { buf = 0; sph ^= 1; }
+          }
+          if (++stage == kGemmStages) { stage = 0; ph ^= 1; }
+        }
+        umma_commit_pair(&sm.acc_full);
+        ++done;
+      }
+      // TMEM and operands stay until all has retired
+      for (int spin = 0; spin < 200000 && done > 0 && !mbar_try_wait(&sm.acc_full, (done - 1) & 1); ++spin) {}
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+  if (threadIdx.x == 0 && sm.abort_word) atomicExch(args.status, kStatusBarrierTimeout);
+}
+
+// ------------------------------------------------------------------ small outputs
+static constexpr int kSplitThreads = 256;   // TMA producer, UMMA issuer, 2 idle warps; 4 warps for scales, then results
+static constexpr int kSplitMax = 8;
+
+template <int kN> constexpr int split_stages() { return kN <= 32 ? 8 : 6; }
+
+template <int kN>
+struct __align__(1024) SplitSmem {
+  union {
+    struct {
+      uint8_t p[split_stages<kN>()][kTileBytes];
+      uint8_t q[split_stages<kN>()][kN * 128];
+    };
+    float part[kN][128];   // this CTA's sums, when all products are through
+  };
+  uint64_t full[split_stages<kN>()], empty[split_stages<kN>()], scale_full[kScaleBufs], scale_empty[kScaleBufs], acc_full;
+  uint32_t tmem_base;
+  int abort_word;
+};
+
+template <int kN, bool kPMn, bool kQMn>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constant__ CUtensorMap tm_q,
+                      const __grid_constant__ GemmArgs args, int splits) {
+  static_assert(!kQMn || kN == 128, "rows innermost: a tile is 128 of them wide");
+  constexpr int kStages = split_stages<kN>();
+  extern __shared__ uint8_t smem_raw[];
+  SplitSmem<kN>& sm = *reinterpret_cast<SplitSmem<kN>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_p);
+    tma_prefetch_desc(&tm_q);
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
+    for (int i = 0; i < kScaleBufs; ++i) { mbar_init(&sm.scale_full[i], 4); mbar_init(&sm.scale_empty[i], 1); }
+    mbar_init(&sm.acc_full, 1);
+    sm.abort_word = 0;
+    mbar_fence_init();
+  }
+  constexpr int kColumns = 256;   // results up to 128, scales behind them
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, kColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_let_next();
+  grid_wait();
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* abort_word = &sm.abort_word;
+  constexpr int kScaleCol = 128;
+  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
+  const int tp = tile % args.tiles_p, tq = tile / args.tiles_p;
+  // parts of k in whole groups of four blocks, so that a scale word belongs to one CTA
+  const int groups = (args.n_kb + 3) / 4, kb0 = 4 * (groups * rank / splits), kb1 = min(4 * (groups * (rank + 1) / splits), args.n_kb);
+  const int p0 = tp * 128, q0 = tq * kN;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, ph = 1;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait(&sm.empty[stage], ph, abort_word);
+        if (!ok) break;
+        mbar_expect_tx(&sm.full[stage], kTileBytes + kN * 128);
+        tma_load_2d(sm.p[stage], &tm_p, &sm.full[stage], kPMn ? p0 : kb * 128, kPMn ? kb * 128 : p0);
+        tma_load_2d(sm.q[stage], &tm_q, &sm.full[stage], kQMn ? q0 : kb * 128, kQMn ? kb * 128 : q0);
+        if (++stage == kStages) { stage = 0; ph ^= 1; }
+      }
+      if (!ok)
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint64_t some = make_sdesc_sw128(0, 16, 1024);
+      const uint32_t hi = uint32_t(some >> 32);
+      const uint32_t p_lo = uint32_t(some) + sdesc_addr(sm.p[0]), q_lo = uint32_t(some) + sdesc_addr(sm.q[0]);
+      auto desc = [&](uint32_t lo) { return (uint64_t(hi) << 32) | lo; };
+      constexpr uint32_t kPK = kPMn ? 256 : 2, kQK = kQMn ? 256 : 2;
+      int stage = 0, ph = 0, buf = 0, sph = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if ((kb & 3) == 0) ok = mbar_wait(&sm.scale_full[buf], sph, abort_word);
+        ok = ok && mbar_wait(&sm.full[stage], ph, abort_word);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t idesc = with_scale_byte(args.idesc, kb & 3), scales = tmem + kScaleCol + buf * 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_mx(tmem, desc(p_lo + stage * (kTileBytes >> 4) + k * kPK), desc(q_lo + stage * (kN * 128 >> 4) + k * kQK), idesc, scales,
+                  scales + 4, (kb > kb0 || k > 0) ? 1u : 0u);
+        umma_commit(&sm.empty[stage]);
+        if ((kb & 3) == 3 || kb + 1 == kb1) {
+          umma_commit(&sm.scale_empty[buf]);
+          if (++buf == kScaleBufs) { buf = 0; sph ^= 1; }
+        }
+        if (++stage == kStages) { stage = 0; ph ^= 1; }
+      }
+      umma_commit(&sm.acc_full);
+    }
+  } else if (warp >= 4) {
+    const int quad = warp & 3;
+    int buf = 0, ph = 1;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; kb += 4) {
+      uint32_t wp[4], wq[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wp[j] = scale_word(args.p, p0 + lane + 32 * j, kb, args.n_kb);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wq[j] = 32 * j < kN ? scale_word(args.q, q0 + lane + 32 * j, kb, args.n_kb) : 0u;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sm.scale_empty[buf], ph, abort_word));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t to = tmem + (uint32_t(quad * 32) << 16) + kScaleCol + buf * 8;
+      tmem_st4(to, wp);
+      tmem_st4(to + 4, wq);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.scale_full[buf]);
+      if (++buf == kScaleBufs) { buf = 0; ph ^= 1; }
+    }
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.acc_full, 0, abort_word));
+    const int row = quad * 32 + lane, p = p0 + row;
+    if (ok) {
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = 0; c0 < kN; c0 += 16) {
+        uint32_t acc[16];
+        tmem_ld16(tmem + (uint32_t(quad * 32) << 16) + c0, acc);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          if (splits > 1) sm.part[c0 + c][row] = __uint_as_float(acc[c]);
+          else if (p < args.p.rows && q0 + c0 + c < args.q.rows) store_result(args, q0 + c0 + c, p, __uint_as_float(acc[c]));
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  if (splits > 1) {
+    __syncwarp();
+    cluster_sync();
+    // every CTA adds up its share of the columns, in the order of k
+    if (warp >= 4 && !sm.abort_word) {
+      const int row = threadIdx.x & 127, p = p0 + row, n = min(kN, args.q.rows - q0);
+      const uint32_t at = smem_u32(&sm.part[0][row]);
+      for (int c = n * rank / splits; c < n * (rank + 1) / splits; ++c) {
+        float v[kSplitMax];
+#pragma unroll
+        for (int r = 0; r < kSplitMax; ++r)
+          if (r < splits) v[r] = __uint_as_float(ld_cluster_u32(at + c * 512, r));
+        float sum = v[0];
+#pragma unroll
+        for (int r = 1; r < kSplitMax; ++r)
+          if (r < splits) sum += v[r];
+        if (p < args.p.rows) store_result(args, q0 + c, p, sum);
+      }
+    }
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) tmem_dealloc(tmem, kColumns);
+  if (threadIdx.x == 0 && sm.abort_word) atomicExch(args.status, kStatusBarrierTimeout);
+}
+
+// codes [rows, cols] of `pitch` bytes per row; tiles of 128 bytes x box_rows, 128-byte swizzle, zeros outside
+static int encode_codes_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
+static std::atomic<uint64_t> g_gemm_smem_raised[16];
+
+template <bool kPMn, bool kQMn>
+static int launch_pair(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const GemmArgs& args, cudaStream_t stream) {
+  const int smem = int(sizeof(GemmSmem)) + 1024;
+  auto kernel = fp8_gemm_pair_kernel<kPMn, kQMn>;
+  if (raise_smem_limit(kernel, smem, g_gemm_smem_raised[kPMn * 2 + kQMn]) != cudaSuccess) return -4;
+  const int tiles = args.tiles_p * args.tiles_q;
+  const cudaError_t rc = launch_overlapped(kernel, dim3(2 * std::min(tiles, kGemmPairs)), kGemmThreads, smem, stream, 1, false, tm_p, tm_q, args);
+  return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
+}
+
+template <int kN, bool kPMn, bool kQMn>
+static int launch_split(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const GemmArgs& args, int splits, int slot, cudaStream_t stream) {
+  const int smem = int(sizeof(SplitSmem<kN>)) + 1024;
+  auto kernel = fp8_gemm_split_kernel<kN, kPMn, kQMn>;
+  if (raise_smem_limit(kernel, smem, g_gemm_smem_raised[slot]) != cudaSuccess) return -4;
+  const cudaError_t rc = launch_overlapped(kernel, dim3(args.tiles_p * args.tiles_q * splits), kSplitThreads, smem, stream, splits, false,
+                                           tm_p, tm_q, args, splits);
+  return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
+}
+
+}  // namespace dcpk
+
+using namespace dcpk;
+
+// An operand's codes: `rows` x k with k innermost, or (rows_inner) k x rows; `pitch` bytes per row of memory, a multiple of
+// 16 like the base.  scales[(row >> shift) * row_stride + (k / 128) * k_stride].
+struct DcpkFp8Operand {
+  const void* codes;
+  long pitch;
+  const void* scales;
+  long scale_row_stride, scale_k_stride;
+  int rows, rows_inner, shift, code_type;
+};
+
+// out [q.rows, p.rows] = q p^T + add.  form: 0 the rule below, 1 pairs, 2 split (tests and measurements).
+extern "C" int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, int k, void* out, long out_pitch, const void* add,
+                             long add_pitch, int out_type, int form, int* status, void* stream) {
+  if (q->rows <= 0 || p->rows <= 0) return 0;
+  if (k <= 0 || out_type < 0 || out_type > 2) return -3;
+  GemmArgs args;
+  const DcpkFp8Operand* from[2] = {p, q};
+  GemmOperand* to[2] = {&args.p, &args.q};
+  for (int i = 0; i < 2; ++i) {
+    const DcpkFp8Operand& o = *from[i];
+    if (o.pitch % 16 || reinterpret_cast<uintptr_t>(o.codes) % 16 || (o.shift != 0 && o.shift != 7) || o.code_type < 0 || o.code_type > 1)
+      return -3;
+    *to[i] = {static_cast<const uint8_t*>(o.scales), o.scale_row_stride, o.scale_k_stride, o.shift, o.rows,
+              o.scale_k_stride == 1 && o.scale_row_stride % 4 == 0 && reinterpret_cast<uintptr_t>(o.scales) % 4 == 0};
+  }
+  args.n_kb = (k + 127) / 128;
+  args.out = out;
+  args.add = add;
+  args.out_pitch = out_pitch;
+  args.add_pitch = add_pitch;
+  args.out_type = out_type;
+  args.status = status;
+  const long pair_tiles = long((p->rows + 255) / 256) * ((q->rows + 255) / 256);
+  const bool pairs = form == 1 || (form == 0 && q->rows > 128 && pair_tiles >= 48);
+  const bool small = !pairs && !q->rows_inner;
+  const int n = pairs ? 256 : small && q->rows <= 16 ? 16 : small && q->rows <= 32 ? 32 : small && q->rows <= 64 ? 64 : 128;
+  const auto map = [&](CUtensorMap* m, const DcpkFp8Operand& o, int box) {
+    return o.rows_inner ? encode_codes_map(m, o.codes, k, o.rows, o.pitch, 128) : encode_codes_map(m, o.codes, o.rows, k, o.pitch, box);
+  };
+  CUtensorMap tm_p, tm_q;
+  if (map(&tm_p, *p, 128) || map(&tm_q, *q, n < 128 ? n : 128)) return -1;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int mode = p->rows_inner * 2 + q->rows_inner;
+  if (pairs) {
+    if (pair_tiles > 0x7fffffffl) return -3;
+    args.tiles_p = (p->rows + 255) / 256;
+    args.tiles_q = (q->rows + 255) / 256;
+    args.idesc = make_idesc_mx(256, 256, p->code_type, q->code_type, p->rows_inner, q->rows_inner);
+    return mode == 0 ? launch_pair<false, false>(tm_p, tm_q, args, s) : mode == 1 ? launch_pair<false, true>(tm_p, tm_q, args, s)
+         : mode == 2 ? launch_pair<true, false>(tm_p, tm_q, args, s) : launch_pair<true, true>(tm_p, tm_q, args, s);
+  }
+  args.tiles_p = (p->rows + 127) / 128;
+  args.tiles_q = (q->rows + n - 1) / n;
+  args.idesc = make_idesc_mx(128, n, p->code_type, q->code_type, p->rows_inner, q->rows_inner);
+  const long tiles = long(args.tiles_p) * args.tiles_q;
+  if (tiles * kSplitMax > 0x7fffffffl) return -3;
+  const int groups = (args.n_kb + 3) / 4;
+  const int splits = int(std::max(1l, std::min({148 / tiles, long(groups), long(kSplitMax)})));
+#define DCPK_SPLIT(N, PM, QM, SLOT) launch_split<N, PM, QM>(tm_p, tm_q, args, splits, SLOT, s)
+  if (q->rows_inner) return p->rows_inner ? DCPK_SPLIT(128, true, true, 4) : DCPK_SPLIT(128, false, true, 5);
+  if (p->rows_inner)
+    return n == 16 ? DCPK_SPLIT(16, true, false, 6) : n == 32 ? DCPK_SPLIT(32, true, false, 7) : n == 64 ? DCPK_SPLIT(64, true, false, 8)
+                                                                                               : DCPK_SPLIT(128, true, false, 9);
+  return n == 16 ? DCPK_SPLIT(16, false, false, 10) : n == 32 ? DCPK_SPLIT(32, false, false, 11) : n == 64 ? DCPK_SPLIT(64, false, false, 12)
+                                                                                              : DCPK_SPLIT(128, false, false, 13);
+#undef DCPK_SPLIT
+}

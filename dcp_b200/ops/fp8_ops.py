@@ -1,0 +1,314 @@
+"""Training in 8 bits: block-scaled codes, their makers and their products (csrc/kernels/fp8_quant.cu, fp8_gemm.cu), each
+with a plain fp32 PyTorch form.
+
+A matrix is kept as ``BlockScaled``: codes in ``torch.float8_e4m3fn`` or ``torch.float8_e5m2`` and a power-of-two scale
+(``torch.float8_e8m0fnu``) per block of 1 x 128, 128 x 1 or 128 x 128 values; ``value = code * scale``.  The scale is the
+smallest power of two with which the block's largest magnitude is representable; a block with a value that is not finite
+has the scale NaN and reads back as NaN.
+
+A product's scales have to run along the contraction in blocks of 128, so
+
+* ``y  = x  w^T``   takes x by rows (1 x 128) and w by blocks (128 x 128):  ``matmul(x, w)``
+* ``dx = dy w``     takes dy by rows and the same codes of w:               ``matmul(dy, w, trans_b=False)``
+* ``dw = dy^T x``   takes both by tokens (128 x 1):                         ``matmul(dy, x, trans_a=True, trans_b=False)``
+
+``linear`` and ``norm_linear`` are these three as autograd functions.  On a CUDA tensor the kernels always run (a missing
+library raises); CPU tensors take the plain forms.  All calls run on the current stream of their tensors' device, allocate
+their results there and may be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+
+BLOCK = 128
+E4M3, E5M2, E8M0 = torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e8m0fnu
+MAX_NORM_WIDTH = 16384
+_CODES = {E4M3: 0, E5M2: 1}
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_KINDS = {(1, BLOCK): 1, (BLOCK, 1): 2, (BLOCK, BLOCK): 4}
+_c_int, _c_long, _c_float = ctypes.c_int, ctypes.c_long, ctypes.c_float
+_NULL = ctypes.c_void_p(0)
+
+
+class BlockScaled(NamedTuple):
+    """``codes`` [R, C] and ``scales`` [ceil(R / block[0]), ceil(C / block[1])]."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    block: Tuple[int, int]
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        wide = torch.float64 if dtype == torch.float64 else torch.float32
+        s = self.scales.to(wide)
+        for dim in (0, 1):
+            if self.block[dim] > 1:
+                s = s.repeat_interleave(self.block[dim], dim).narrow(dim, 0, self.codes.shape[dim])
+        return (self.codes.to(wide) * s).to(dtype)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on(t: torch.Tensor):
+    """The tensor's device as the current one."""
+    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _up(n: int, to: int) -> int:
+    return -(-n // to) * to
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D tensor whose rows are contiguous, of any pitch."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+_STATUS = {}
+
+
+def _status(device: torch.device) -> torch.Tensor:
+    if device.index not in _STATUS:
+        _STATUS[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+    return _STATUS[device.index]
+
+
+def check_status() -> None:
+    """Raise if a bounded wait inside a product ran out since the last call (synchronises)."""
+    for index, word in _STATUS.items():
+        code = int(word.item())
+        if code:
+            word.zero_()
+            raise RuntimeError(f"8-bit product on cuda:{index} gave up waiting (status {code}): its results are not complete")
+
+
+# --------------------------------------------------------------------------- plain forms (fp32)
+def _scale_bytes(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    mantissa, exponent = torch.frexp(amax)
+    k = exponent - (9 if dtype == E4M3 else 16) + (mantissa > 0.875).to(exponent.dtype)   # largest code: 0.875 * 2^9 or 2^16
+    k = torch.where(amax > 0, k, torch.full_like(k, -127)).clamp(-127, 127) + 127
+    return torch.where(torch.isfinite(amax), k, torch.full_like(k, 255)).to(torch.uint8)
+
+
+def quantize_reference(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK), dtype: torch.dtype = E4M3) -> BlockScaled:
+    rows, cols = x.shape
+    br, bc = block
+    full = torch.zeros(_up(rows, br), _up(cols, bc), dtype=torch.float32, device=x.device)
+    full[:rows, :cols] = x
+    tiles = full.view(full.shape[0] // br, br, full.shape[1] // bc, bc)
+    scales = _scale_bytes(tiles.abs().amax((1, 3)), dtype).view(E8M0)
+    largest = torch.finfo(dtype).max
+    codes = (tiles / scales.float()[:, None, :, None]).clamp(-largest, largest).view(full.shape)[:rows, :cols]
+    return BlockScaled(codes.to(dtype), scales, (br, bc))
+
+
+def rmsnorm_quant_reference(x, w, eps, residual=None, dtype=E4M3):
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    hf = h.float()
+    rstd = torch.rsqrt(hf.pow(2).mean(-1) + eps)
+    return quantize_reference(hf * rstd[:, None] * w.float(), (1, BLOCK), dtype), h, rstd
+
+
+def rmsnorm_quant_bwd_reference(h, w, rstd, dy, add=None):
+    xh, g = h.float() * rstd[:, None], dy.float() * w.float()
+    dx = rstd[:, None] * (g - xh * (g * xh).mean(-1, keepdim=True))
+    if add is not None:
+        dx = dx + add.float()
+    return dx.to(h.dtype), (dy.float() * xh).sum(0)
+
+
+def matmul_reference(a, b, trans_a=False, trans_b=True, out_dtype=torch.bfloat16, add=None):
+    x, y = a.dequantize(), b.dequantize()
+    out = (x.t() if trans_a else x) @ (y.t() if trans_b else y)
+    return (out if add is None else out + add.float()).to(out_dtype)
+
+
+# --------------------------------------------------------------------------- codes
+def _empty_codes(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """Codes whose rows begin on 16 bytes, as the products read them."""
+    return torch.empty(rows, _up(cols, 16), dtype=dtype, device=device)[:, :cols]
+
+
+def _empty_scales(rows: int, cols: int, block: Tuple[int, int], device) -> torch.Tensor:
+    """Scales with those of neighbouring blocks along the contraction next to one another: a (128, 1) tensor's are stored
+    by columns."""
+    nr, nc = -(-rows // block[0]), -(-cols // block[1])
+    if block == (BLOCK, 1):
+        return torch.empty(nc, _up(nr, 4), dtype=torch.uint8, device=device)[:, :nr].t().view(E8M0)
+    return torch.empty(nr, _up(nc, 4), dtype=torch.uint8, device=device)[:, :nc].view(E8M0)
+
+
+def _check_matrix(x: torch.Tensor, what: str) -> None:
+    _need(x.dim() == 2, f"{what} has to be a matrix, not {tuple(x.shape)}")
+    _need(x.dtype in _TYPES, f"{what} has to be bfloat16, float16 or float32, not {x.dtype}")
+
+
+def _quantize(x: torch.Tensor, ways: int, dtype: torch.dtype):
+    _check_matrix(x, "x")
+    _need(dtype in _CODES, f"codes are float8_e4m3fn or float8_e5m2, not {dtype}")
+    kinds = [k for k, bit in _KINDS.items() if ways & bit]
+    if not x.is_cuda:
+        return [quantize_reference(x, k, dtype) for k in kinds]
+    rows, cols = x.shape
+    with _on(x):
+        x = _rows(x)
+        out = [BlockScaled(_empty_codes(rows, cols, dtype, x.device), _empty_scales(rows, cols, k, x.device), k) for k in kinds]
+        a = next((q for q in out if q.block != (BLOCK, 1)), None)
+        b = next((q for q in out if q.block == (BLOCK, 1)), None)
+        place = lambda q, t, stride: (_NULL, _c_long(0)) if q is None else (_lib.ptr(t(q)), _c_long(stride(q)))  # noqa: E731
+        _lib.check(_lib.load().dcpk_fp8_quantize(
+            _c_int(_TYPES[x.dtype]), _c_int(_CODES[dtype]), _c_int(ways), _lib.ptr(x), _c_long(_pitch(x)),
+            *place(a, lambda q: q.codes, lambda q: _up(cols, 16)), *place(a, lambda q: q.scales, lambda q: _up(q.scales.shape[1], 4)),
+            *place(b, lambda q: q.codes, lambda q: _up(cols, 16)), *place(b, lambda q: q.scales, lambda q: _up(q.scales.shape[0], 4)),
+            _c_long(rows), _c_int(cols), _lib.stream_handle()), "fp8_quantize")
+    return out
+
+
+def quantize(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK), dtype: torch.dtype = E4M3) -> BlockScaled:
+    """Codes of a matrix (bf16, fp16 or fp32, any pitch) with a scale per block: (1, 128), (128, 1) or (128, 128)."""
+    _need(tuple(block) in _KINDS, f"blocks are (1, 128), (128, 1) or (128, 128), not {block}")
+    return _quantize(x, _KINDS[tuple(block)], dtype)[0]
+
+
+def quantize_both(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Tuple[BlockScaled, BlockScaled]:
+    """``quantize`` by rows (1, 128) and by columns (128, 1) from one pass over ``x``: what a gradient needs for the input
+    gradient and for the weight gradient."""
+    return tuple(_quantize(x, 3, dtype))
+
+
+# --------------------------------------------------------------------------- RMSNorm
+def rmsnorm_quant(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None,
+                  dtype: torch.dtype = E4M3):
+    """(y, h, rstd): h = x + residual in x's type (x itself without a residual), y = rmsnorm(h) * w as ``BlockScaled`` by rows,
+    rounded once; rstd fp32 [rows].  x, residual [rows, width] of any pitch, w [width], all of one type; no autograd."""
+    _check_matrix(x, "x")
+    _need(dtype in _CODES, f"codes are float8_e4m3fn or float8_e5m2, not {dtype}")
+    rows, width = x.shape
+    _need(w.shape == (width,) and w.dtype == x.dtype, f"w has to be {x.dtype} of {width} channels")
+    _need(1 <= width <= MAX_NORM_WIDTH, f"rows of 1 to {MAX_NORM_WIDTH} channels, not {width}")
+    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "the residual has to be like x")
+    _need(all(t.device == x.device for t in (w, residual) if t is not None), "all tensors have to be on x's device")
+    if not x.is_cuda:
+        return rmsnorm_quant_reference(x, w, eps, residual, dtype)
+    with _on(x):
+        x, w = _rows(x), w.contiguous()
+        res = None if residual is None else _rows(residual)
+        h = x if res is None else torch.empty(rows, width, dtype=x.dtype, device=x.device)
+        y = BlockScaled(_empty_codes(rows, width, dtype, x.device), _empty_scales(rows, width, (1, BLOCK), x.device), (1, BLOCK))
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+        _lib.check(_lib.load().dcpk_fp8_norm(
+            _c_int(_TYPES[x.dtype]), _c_int(_CODES[dtype]), _lib.ptr(x), _c_long(_pitch(x)), _NULL if res is None else _lib.ptr(res),
+            _c_long(0 if res is None else _pitch(res)), _lib.ptr(w), _lib.ptr(h), _lib.ptr(y.codes), _c_long(_up(width, 16)),
+            _lib.ptr(y.scales), _c_long(_up(y.scales.shape[1], 4)), _lib.ptr(rstd), _c_long(rows), _c_int(width), _c_float(eps),
+            _lib.stream_handle()), "fp8_norm")
+    return y, h, rstd
+
+
+def rmsnorm_quant_bwd(h: torch.Tensor, w: torch.Tensor, rstd: torch.Tensor, dy: torch.Tensor, add: Optional[torch.Tensor] = None):
+    """(dx, dw fp32) for what ``rmsnorm_quant`` returned and the gradient ``dy`` of y (of the values the codes stand for);
+    ``add``, the gradient of h from elsewhere, is added to dx, which is the gradient of x and of the residual.  Sums in fp32
+    and in a fixed order: the same bits in every run."""
+    _check_matrix(h, "h")
+    rows, width = h.shape
+    _need(w.shape == (width,) and w.dtype == h.dtype, f"w has to be {h.dtype} of {width} channels")
+    _need(1 <= width <= MAX_NORM_WIDTH, f"rows of 1 to {MAX_NORM_WIDTH} channels, not {width}")
+    _need(dy.shape == h.shape and dy.dtype == h.dtype, "dy has to be like h")
+    _need(add is None or (add.shape == h.shape and add.dtype == h.dtype), "add has to be like h")
+    _need(rstd.shape == (rows,) and rstd.dtype == torch.float32, f"rstd has to be float32 of {rows} rows")
+    _need(all(t.device == h.device for t in (w, rstd, dy, add) if t is not None), "all tensors have to be on h's device")
+    if not h.is_cuda:
+        return rmsnorm_quant_bwd_reference(h, w, rstd, dy, add)
+    with _on(h):
+        h, w, rstd, dy = _rows(h), w.contiguous(), rstd.contiguous(), _rows(dy)
+        add = None if add is None else _rows(add)
+        lib = _lib.load()
+        dx = torch.empty(rows, width, dtype=h.dtype, device=h.device)
+        dw = torch.empty(width, dtype=torch.float32, device=h.device)
+        part = torch.empty(lib.dcpk_fp8_norm_bwd_parts(_c_long(rows), _c_int(width)), width, dtype=torch.float32, device=h.device)
+        _lib.check(lib.dcpk_fp8_norm_bwd(
+            _c_int(_TYPES[h.dtype]), _lib.ptr(h), _c_long(_pitch(h)), _lib.ptr(w), _lib.ptr(rstd), _lib.ptr(dy), _c_long(_pitch(dy)),
+            _NULL if add is None else _lib.ptr(add), _c_long(0 if add is None else _pitch(add)), _lib.ptr(dx), _lib.ptr(dw),
+            _lib.ptr(part), _c_long(rows), _c_int(width), _lib.stream_handle()), "fp8_norm_bwd")
+    return dx, dw
+
+
+# --------------------------------------------------------------------------- products
+class _Operand(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("pitch", _c_long), ("scales", ctypes.c_void_p), ("scale_row_stride", _c_long),
+                ("scale_k_stride", _c_long), ("rows", _c_int), ("rows_inner", _c_int), ("shift", _c_int), ("code_type", _c_int)]
+
+
+def _check_scaled(q: BlockScaled, what: str) -> None:
+    codes, scales, block = q
+    _need(codes.dim() == 2 and codes.dtype in _CODES, f"{what}: codes have to be a float8_e4m3fn or float8_e5m2 matrix")
+    _need(tuple(block) in _KINDS, f"{what}: blocks are (1, 128), (128, 1) or (128, 128), not {block}")
+    want = tuple(-(-n // s) for n, s in zip(codes.shape, block))
+    _need(scales.dtype == E8M0 and tuple(scales.shape) == want, f"{what}: scales have to be float8_e8m0fnu of shape {want}")
+    _need(scales.device == codes.device, f"{what}: codes and scales on two devices")
+
+
+def _operand(q: BlockScaled, k_dim: int) -> Tuple[_Operand, tuple]:
+    """The operand as the kernel takes it and the tensors that have to live until it is launched."""
+    codes, scales, block = q
+    inner = 1 if codes.stride(1) == 1 or codes.shape[1] == 1 else None
+    if inner is None or codes.data_ptr() % 16 or (codes.shape[0] > 1 and (codes.stride(0) % 16 or codes.stride(0) < codes.shape[1])):
+        codes = _empty_codes(*codes.shape, codes.dtype, codes.device).copy_(codes)
+    pitch = codes.stride(0) if codes.shape[0] > 1 else _up(codes.shape[1], 16)
+    row_dim = 1 - k_dim
+    return _Operand(codes.data_ptr(), pitch, scales.data_ptr(), scales.stride(row_dim), scales.stride(k_dim), codes.shape[row_dim],
+                    k_dim == 0, 7 if block[row_dim] == BLOCK else 0, _CODES[codes.dtype]), (codes, scales)
+
+
+def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bool = True, out_dtype: torch.dtype = torch.bfloat16,
+           add: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, form: int = 0) -> torch.Tensor:
+    """op(a) op(b) of the values the codes stand for, summed in fp32 and rounded once; ``add`` (of the output's type and shape,
+    rows contiguous) is added before the rounding and may be ``out`` itself.
+
+    a: [M, K], or [K, M] with ``trans_a``; b: [N, K], or [K, N] without ``trans_b`` -> [M, N] in bf16, fp16 or fp32.  Along K
+    both need a scale per 128 values; along the other dimension one per value or per 128.  Codes whose rows begin on 16 bytes
+    (as the makers here lay them out) are read where they are, others are copied first.  ``form``: 0 chooses the kernel, 1 and
+    2 name it (measurements)."""
+    _check_scaled(a, "a")
+    _check_scaled(b, "b")
+    ka, kb = (0 if trans_a else 1), (1 if trans_b else 0)
+    m, n, k = a.codes.shape[1 - ka], b.codes.shape[1 - kb], a.codes.shape[ka]
+    _need(k == b.codes.shape[kb], f"contraction over {k} values of a and {b.codes.shape[kb]} of b")
+    _need(a.block[ka] == BLOCK and b.block[kb] == BLOCK, "both operands need a scale per 128 values along the contraction")
+    _need(a.codes.device == b.codes.device, "a and b are on two devices")
+    _need(form in (0, 1, 2), "form is 0, 1 or 2")
+    if out is not None:
+        out_dtype = out.dtype
+        _need(tuple(out.shape) == (m, n) and out.device == a.codes.device, f"out has to be {(m, n)} on a's device")
+        _need(n <= 1 or out.stride(1) == 1, "rows of out have to be contiguous")
+    _need(out_dtype in _TYPES, f"results are bfloat16, float16 or float32, not {out_dtype}")
+    if add is not None:
+        _need(tuple(add.shape) == (m, n) and add.dtype == out_dtype and add.device == a.codes.device,
+              f"add has to be {out_dtype} {(m, n)} on a's device")
+    if not a.codes.is_cuda:
+        got = matmul_reference(a, b, trans_a, trans_b, out_dtype, add)
+        return got if out is None else out.copy_(got)
+    with _on(a.codes):
+        if out is None:
+            out = torch.empty(m, n, dtype=out_dtype, device=a.codes.device)
+        if m == 0 or n == 0:
+            return out
+        if k == 0:
+            return out.zero_() if add is None else out.copy_(add)
+        add = None if add is None else _rows(add)
+        qa, keep_a = _operand(a, ka)
+        qb, keep_b = _operand(b, kb)
+        _lib.check(_lib.load().dcpk_fp8_gemm(
+            ctypes.byref(qa), ctypes.byref(qb), _c_int(k), _lib.ptr(out), _c_long(_pitch(out)), _NULL if add is None else _lib.ptr(add),
+            _c_long(0 if add is None else _pitch(add)), _c_int(_TYPES[out_dtype]), _c_int(form), _lib.ptr(_status(out.device)),
+            _lib.stream_handle()), "fp8_gemm")
+    return out
