@@ -1,0 +1,348 @@
+// One AdamW step over many tensors, moments in 32 or 8 bits.
+//
+//   m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      w -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + wd w)
+//
+// with g the gradient times grad_scale and the clipping coefficient min(1, clip / (norm + 1e-6)).  Bound by HBM: 28 bytes per
+// parameter with moments in 32 bits (bf16 parameter and gradient, fp32 master), 16 with moments in 8.
+//
+// Moments in 8 bits: m and sqrt(v) as e4m3 with a power-of-two scale per 256 values (fp8_common.cuh).  The root, because it
+// is what the update divides by and because it halves v's range of exponents.  A moving average does not survive rounding to
+// nearest: with b2 = 0.999 a step changes sqrt(v) by 0.05 %, half a step of e4m3 is 3 to 6 %, so it would never decay.  So
+// the codes are rounded stochastically: 16 random bits are added behind the code's last place before the cut, which is
+// right on average.  The bits are a hash of seed, step, tensor and element, so a step can be repeated to the bit.  A root
+// that is not zero keeps the smallest code at least: the update never divides by eps alone where there was a gradient.  A
+// moment that is not finite is kept as NaN and leaves its neighbours and the scale alone, as in 32 bits.
+//
+// A warp works on the 256 values of a scale, eight per lane.  The tensors' addresses are kernel arguments: no table has to
+// be brought to the GPU when gradients move, and a captured graph holds its own.  The step counter and the bias corrections
+// are on the GPU, so a replayed graph counts on.
+#include <algorithm>
+
+#include "fp8_common.cuh"
+#include "launch.cuh"
+
+namespace dcpk {
+
+static constexpr int kAdamTensors = 128;   // of a launch
+static constexpr int kStateBlock = 256;
+static constexpr int kAdamThreads = 256;
+static constexpr int kChunk = kAdamThreads * 8;   // values a CTA takes at a time: one block per warp
+
+struct AdamTensor {
+  void* param;
+  const void* grad;
+  float* master;             // null: the parameter is its own master
+  void* m;
+  void* v;
+  uint8_t* m_scale;
+  uint8_t* v_scale;
+  long n;
+};
+struct AdamList {
+  AdamTensor t[kAdamTensors];
+  int first_chunk[kAdamTensors + 1];
+  uint8_t aligned[kAdamTensors];
+  int n, base;               // base: tensors in launches before
+};
+struct AdamScalars { float lr, beta1, beta2, eps, wd, grad_scale; };
+// what a step's kernels hand on, in global memory
+struct AdamShared { float coef, bc1, root_bc2; uint32_t key; };
+
+__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {   // finaliser of MurmurHash3 (A. Appleby, public domain)
+  x ^= x >> 16; x *= 0x85ebca6bu;
+  x ^= x >> 13; x *= 0xc2b2ae35u;
+  return x ^ (x >> 16);
+}
+
+// the tensor a chunk belongs to
+__device__ __forceinline__ int find_tensor(const AdamList& list, int chunk) {
+  int lo = 0, hi = list.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (list.first_chunk[mid] <= chunk) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, long e0, int lane, long n, bool vec, float (&f)[8]) {
+  if (vec) {
+    Raw8<T> raw;
+    load_raw(raw, p + e0 + lane * 8);
+    widen(raw, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = e0 + j * 32 + lane < n ? to_float(p[e0 + j * 32 + lane]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* p, long e0, int lane, long n, bool vec, const float (&f)[8]) {
+  if (vec) {
+    store8(p + e0 + lane * 8, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (e0 + j * 32 + lane < n) p[e0 + j * 32 + lane] = from_float<T>(f[j]);
+  }
+}
+__device__ __forceinline__ float2 from_codes2(uint32_t c) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(c)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ void load_state8(const uint8_t* p, long e0, int lane, long n, bool vec, float scale, float (&f)[8]) {
+  uint32_t w[2] = {0, 0};
+  if (vec) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p + e0 + lane * 8);
+    w[0] = r.x; w[1] = r.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (e0 + j * 32 + lane < n) w[j >> 2] |= uint32_t(p[e0 + j * 32 + lane]) << (8 * (j & 3));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = from_codes2(w[i >> 1] >> (16 * (i & 1)));
+    f[2 * i] = t.x * scale; f[2 * i + 1] = t.y * scale;
+  }
+}
+// Codes of a block's values, at random to one of the two neighbours.  2^-120 takes e4m3's smallest exponent to fp32's: the cut
+// of the bits goes through its denormals too.
+template <bool kRoot>
+__device__ __forceinline__ void store_state8(uint8_t* p, uint8_t* scale, long e0, int lane, long n, bool vec, const float (&f)[8],
+                                             const uint32_t (&random)[8]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
+    amax = max(amax, b < 0x7f800000u ? b : 0u);
+  }
+  const int byte = scale_byte<8>(__reduce_max_sync(0xffffffffu, amax));
+  const float inv = scale_inverse(byte);
+  uint32_t code[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = fabsf(f[j]);
+    uint32_t c = (__float_as_uint(a * inv * 0x1p-120f) + ((kRoot ? random[j] >> 16 : random[j] & 0xffffu) << 4)) >> 20;
+    c = min(c, 0x7eu);
+    if (kRoot && a > 0.f) c = max(c, 1u);
+    if (!(a < INFINITY)) c = 0x7fu;
+    code[j] = c | (kRoot ? 0u : (__float_as_uint(f[j]) >> 31) << 7);
+  }
+  if (vec) {
+    uint2 r;
+    r.x = code[0] | (code[1] << 8) | (code[2] << 16) | (code[3] << 24);
+    r.y = code[4] | (code[5] << 8) | (code[6] << 16) | (code[7] << 24);
+    *reinterpret_cast<uint2*>(p + e0 + lane * 8) = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (e0 + j * 32 + lane < n) p[e0 + j * 32 + lane] = uint8_t(code[j]);
+  }
+  if (lane == 0) *scale = uint8_t(byte);
+}
+
+// sum of squares of a CTA's gradients, from the threads' sums on in 64 bits; `parts` are added up in order
+template <typename G>
+__global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_constant__ AdamList list, float grad_scale, double* __restrict__ parts) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
+  float sq[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  grid_wait();
+  for (int chunk = blockIdx.x; chunk < n_chunks; chunk += gridDim.x) {
+    const int i = find_tensor(list, chunk);
+    const long e0 = long(chunk - list.first_chunk[i]) * kChunk + warp * kStateBlock, n = list.t[i].n;
+    if (e0 >= n) continue;
+    float g[8];
+    load8(static_cast<const G*>(list.t[i].grad), e0, lane, n, list.aligned[i] && e0 + kStateBlock <= n, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      g[j] *= grad_scale;
+      sq[j] += g[j] * g[j];
+    }
+  }
+  grid_let_next();
+  double t = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t += double(sq[j]);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
+  __shared__ double warps[kAdamThreads / 32];
+  if (lane == 0) warps[warp] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kAdamThreads / 32; ++w) t += warps[w];
+    parts[blockIdx.x] = t;
+  }
+}
+
+// step counter, bias corrections, clipping coefficient: one CTA
+__global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __restrict__ parts, int n_parts, int64_t* __restrict__ step, float beta1,
+                                                            float beta2, float grad_scale, float clip, uint32_t seed, float* __restrict__ norm,
+                                                            AdamShared* __restrict__ shared) {
+  __shared__ double sums[8];
+  grid_wait();
+  grid_let_next();
+  double t = 0.0;
+  for (int i = threadIdx.x; i < n_parts; i += 256) t += parts[i];
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) t += sums[w];
+  const int64_t now = *step + 1;
+  *step = now;
+  float coef = grad_scale;
+  if (n_parts > 0) {
+    const double length = sqrt(t);
+    *norm = float(length);
+    const float c = float(double(clip) / (length + 1e-6));
+    coef *= c > 1.f ? 1.f : c;   // a NaN norm gives NaN
+  }
+  shared->coef = coef;
+  shared->bc1 = float(1.0 / (1.0 - pow(double(beta1), double(now))));
+  shared->root_bc2 = float(sqrt(1.0 / (1.0 - pow(double(beta2), double(now)))));
+  shared->key = mix32(seed + uint32_t(now) * 0x9e3779b1u);
+}
+
+template <typename P, typename G, bool kMaster, bool kEight>
+__global__ void __launch_bounds__(kAdamThreads) adamw_multi_kernel(const __grid_constant__ AdamList list, const AdamScalars s,
+                                                                   const AdamShared* __restrict__ shared) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
+  grid_wait();
+  const AdamShared now = *shared;
+  for (int chunk = blockIdx.x; chunk < n_chunks; chunk += gridDim.x) {
+    const int i = find_tensor(list, chunk);
+    const AdamTensor& t = list.t[i];
+    const long e0 = long(chunk - list.first_chunk[i]) * kChunk + warp * kStateBlock, n = t.n, block = e0 / kStateBlock;
+    if (e0 >= n) continue;
+    const bool vec = list.aligned[i] && e0 + kStateBlock <= n;
+    float g[8], w[8], m[8], v[8];
+    load8(static_cast<const G*>(t.grad), e0, lane, n, vec, g);
+    if (kMaster) load8(static_cast<const float*>(t.master), e0, lane, n, vec, w);
+    else load8(static_cast<const P*>(t.param), e0, lane, n, vec, w);
+    if (kEight) {
+      load_state8(static_cast<const uint8_t*>(t.m), e0, lane, n, vec, scale_value(t.m_scale[block]), m);
+      load_state8(static_cast<const uint8_t*>(t.v), e0, lane, n, vec, scale_value(t.v_scale[block]), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= v[j];
+    } else {
+      load8(static_cast<const float*>(t.m), e0, lane, n, vec, m);
+      load8(static_cast<const float*>(t.v), e0, lane, n, vec, v);
+    }
+    float root[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      g[j] *= now.coef;
+      m[j] = s.beta1 * m[j] + (1.f - s.beta1) * g[j];
+      v[j] = s.beta2 * v[j] + (1.f - s.beta2) * g[j] * g[j];
+      root[j] = sqrtf(v[j]);
+      w[j] -= s.lr * (m[j] * now.bc1 / (root[j] * now.root_bc2 + s.eps) + s.wd * w[j]);
+    }
+    if (kMaster) put8(t.master, e0, lane, n, vec, w);
+    put8(static_cast<P*>(t.param), e0, lane, n, vec, w);
+    if (kEight) {
+      uint32_t random[8];
+      const uint32_t key = mix32(now.key + uint32_t(list.base + i) * 0x85ebca77u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) random[j] = mix32(uint32_t(e0 + (vec ? lane * 8 + j : j * 32 + lane)) * 0x9e3779b1u + key);
+      store_state8<false>(static_cast<uint8_t*>(t.m), t.m_scale + block, e0, lane, n, vec, m, random);
+      store_state8<true>(static_cast<uint8_t*>(t.v), t.v_scale + block, e0, lane, n, vec, root, random);
+    } else {
+      put8(static_cast<float*>(t.m), e0, lane, n, vec, m);
+      put8(static_cast<float*>(t.v), e0, lane, n, vec, v);
+    }
+  }
+}
+
+}  // namespace dcpk
+
+using namespace dcpk;
+
+static int adam_norm_ctas(int chunks) { return std::min(chunks, 148 * 4); }
+
+// doubles of `work` a call needs: what the kernels hand on, and a sum per CTA of each launch of the norm
+extern "C" long dcpk_adamw_multi_work(int n_tensors) { return 2 + long((n_tensors + kAdamTensors - 1) / kAdamTensors) * 148 * 4; }
+
+// Tensors of one parameter type and one gradient type (0 fp32, 1 fp16, 2 bf16); an entry of `masters` may be null for fp32
+// parameters only.  m_scales null: moments in fp32; otherwise codes with ceil(n / 256) scales.  step: one int64 on the
+// device, counted up.  clip <= 0: none, and norm is not written.
+extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* const* grads, void* const* masters, void* const* ms,
+                                void* const* vs, void* const* m_scales, void* const* v_scales, const long* sizes, int param_type, int grad_type,
+                                int64_t* step, float lr, float beta1, float beta2, float eps, float wd, float grad_scale, float clip,
+                                unsigned seed, float* norm, double* work, void* stream) {
+  if (n_tensors < 0 || param_type < 0 || param_type > 2 || grad_type < 0 || grad_type > 2) return -3;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  AdamShared* shared = reinterpret_cast<AdamShared*>(work);
+  double* parts = work + 2;
+  static_assert(sizeof(AdamShared) <= 16, "work begins with it");
+  const bool eight = m_scales != nullptr, has_master = masters != nullptr;
+  if (!has_master && param_type != kTypeF32) return -3;
+  for (int i = 0; i < n_tensors; ++i)
+    if (sizes[i] < 0 || sizes[i] / kChunk >= 0x7fffffffl - kAdamTensors) return -3;
+  const auto fill = [&](AdamList& list, int base) -> int {   // the next launch's tensors; returns how many it took
+    list.base = base;
+    list.n = 0;
+    list.first_chunk[0] = 0;
+    int i = base;
+    for (; i < n_tensors && list.n < kAdamTensors; ++i) {
+      const long chunks = (sizes[i] + kChunk - 1) / kChunk;
+      if (list.first_chunk[list.n] + chunks > 0x7fffffffl) break;
+      AdamTensor& t = list.t[list.n];
+      t = {params[i], grads[i], has_master ? static_cast<float*>(masters[i]) : nullptr, ms[i], vs[i],
+           eight ? static_cast<uint8_t*>(m_scales[i]) : nullptr, eight ? static_cast<uint8_t*>(v_scales[i]) : nullptr, sizes[i]};
+      const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+      list.aligned[list.n] = (at(t.param) | at(t.grad) | at(t.master)) % 16 == 0 && (at(t.m) | at(t.v)) % (eight ? 8 : 16) == 0;
+      list.first_chunk[list.n + 1] = int(list.first_chunk[list.n] + chunks);
+      ++list.n;
+    }
+    return i - base;
+  };
+  const auto by_type = [](int type, auto f) {
+    return type == kTypeBf16 ? f(static_cast<__nv_bfloat16*>(nullptr)) : type == kTypeF16 ? f(static_cast<__half*>(nullptr)) : f(static_cast<float*>(nullptr));
+  };
+  AdamList list;
+  int n_parts = 0;
+  bool first = true;   // of the call: what ran before is not told apart from a kernel that does not wait
+  if (clip > 0.f)
+    for (int base = 0; base < n_tensors;) {
+      base += fill(list, base);
+      const int chunks = list.first_chunk[list.n];
+      if (chunks == 0) continue;
+      const int ctas = adam_norm_ctas(chunks);
+      const cudaError_t rc = by_type(grad_type, [&](auto* g) {
+        using G = std::remove_pointer_t<decltype(g)>;
+        return launch_overlapped(adamw_norm_kernel<G>, dim3(ctas), kAdamThreads, 0, s, 1, !first, list, grad_scale, parts + n_parts);
+      });
+      if (rc != cudaSuccess || cudaGetLastError() != cudaSuccess) return -5;
+      n_parts += ctas;
+      first = false;
+    }
+  if (clip > 0.f && n_parts == 0 && cudaMemsetAsync(norm, 0, 4, s) != cudaSuccess) return -5;
+  if (launch_overlapped(adamw_prepare_kernel, dim3(1), 256, 0, s, 1, !first, static_cast<const double*>(parts), n_parts, step, beta1, beta2,
+                        grad_scale, clip, uint32_t(seed), norm, shared) != cudaSuccess || cudaGetLastError() != cudaSuccess)
+    return -5;
+  const AdamScalars scalars = {lr, beta1, beta2, eps, wd, grad_scale};
+  for (int base = 0; base < n_tensors;) {
+    base += fill(list, base);
+    const int chunks = list.first_chunk[list.n];
+    if (chunks == 0) continue;
+    const cudaError_t rc = by_type(param_type, [&](auto* p) {
+      using P = std::remove_pointer_t<decltype(p)>;
+      return by_type(grad_type, [&](auto* g) {
+        using G = std::remove_pointer_t<decltype(g)>;
+        const auto launch = [&](auto kernel) {
+          return launch_overlapped(kernel, dim3(std::min(chunks, 148 * 8)), kAdamThreads, 0, s, 1, true, list, scalars, static_cast<const AdamShared*>(shared));
+        };
+        if constexpr (std::is_same_v<P, float>) {
+          if (!has_master) return eight ? launch(adamw_multi_kernel<P, G, false, true>) : launch(adamw_multi_kernel<P, G, false, false>);
+        }
+        return eight ? launch(adamw_multi_kernel<P, G, true, true>) : launch(adamw_multi_kernel<P, G, true, false>);
+      });
+    });
+    if (rc != cudaSuccess || cudaGetLastError() != cudaSuccess) return -5;
+  }
+  return 0;
+}

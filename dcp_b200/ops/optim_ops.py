@@ -1,0 +1,151 @@
+"""AdamW over many tensors at once, moments in 32 or 8 bits (csrc/kernels/adamw_multi.cu), with a plain PyTorch form.
+
+``adamw_multi`` is the operator; ``MultiTensorAdamW`` keeps the state of a list of parameters for it.
+``parallel.dist_optimizer.ShardedAdamW`` is the optimizer for flat buffers that are shared between ranks.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional, Sequence
+
+import torch
+
+from . import _lib
+from .fp8_ops import E4M3, E8M0, _need, _on, _scale_bytes
+
+STATE_BLOCK = 256       # values that share a scale in an 8-bit moment
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _mix32(x):
+    x = ((x ^ (x >> 16)) * 0x85EBCA6B) & 0xFFFFFFFF
+    x = ((x ^ (x >> 13)) * 0xC2B2AE35) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def state_scales(n: int) -> int:
+    """Scales of an 8-bit moment of ``n`` values."""
+    return -(-n // STATE_BLOCK)
+
+
+def encode_state(x: torch.Tensor, random: Optional[torch.Tensor] = None, root: bool = False):
+    """(codes, scales) of an fp32 moment: to nearest, or with ``random`` (16 bits per value) as a step rounds.  Values that
+    are not finite become NaN codes and do not count for their block's scale."""
+    n = x.numel()
+    flat = x.detach().reshape(-1).float()
+    blocks = torch.zeros(state_scales(n) * STATE_BLOCK, device=x.device)
+    blocks[:n] = torch.where(torch.isfinite(flat), flat.abs(), torch.zeros_like(flat))
+    blocks = blocks.view(-1, STATE_BLOCK)
+    scales = _scale_bytes(blocks.amax(1), E4M3).view(E8M0)
+    y = (blocks / scales.float()[:, None]).view(-1)[:n]
+    if random is None:
+        code = y.to(E4M3).view(torch.uint8).long()
+    else:
+        # 2^-120 takes e4m3's smallest exponent to fp32's: the cut goes through its denormals too
+        code = ((y * 2.0 ** -120).contiguous().view(torch.int32).long() + (random << 4) >> 20).clamp(max=0x7E)
+    if root:
+        code = torch.where(flat > 0, code.clamp(min=1), code)
+    code = torch.where(torch.isfinite(flat), code, torch.full_like(code, 0x7F))
+    code = code | (torch.signbit(flat).long() << 7)
+    return code.to(torch.uint8).view(E4M3).view(x.shape), scales
+
+
+def decode_state(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """fp32 values of an 8-bit moment."""
+    flat = codes.reshape(-1)
+    return (flat.float() * scales.float().repeat_interleave(STATE_BLOCK)[:flat.numel()]).view(codes.shape)
+
+
+def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta2, eps, weight_decay, grad_scale=1.0, clip=None,
+                          m_scales=None, v_scales=None, seed=0):
+    step += 1
+    t = step.double()
+    bc1, root_bc2 = (1 / (1 - beta1 ** t)).float(), (1 / (1 - beta2 ** t)).sqrt().float()
+    coef, norm = grad_scale, None
+    if clip is not None:
+        total = torch.zeros(1, dtype=torch.float64, device=step.device)
+        for g in grads:
+            total += (g.double() * grad_scale).square().sum()
+        norm = total.sqrt()
+        coef = grad_scale * (clip / (norm + 1e-6)).float().clamp(max=1.0)
+        norm = norm.float()
+    key = _mix32((seed + int(step) * 0x9E3779B1) & 0xFFFFFFFF)
+    for i, g in enumerate(grads):
+        w = params[i] if masters is None else masters[i]
+        g = g.float() * coef
+        m32, v32 = (m[i], v[i]) if m_scales is None else (decode_state(m[i], m_scales[i]), decode_state(v[i], v_scales[i]).square())
+        m32 = beta1 * m32 + (1 - beta1) * g
+        v32 = beta2 * v32 + (1 - beta2) * g * g
+        root = v32.sqrt()
+        w -= lr * (m32 * bc1 / (root * root_bc2 + eps) + weight_decay * w)
+        if masters is not None:
+            params[i].copy_(w)
+        if m_scales is None:
+            m[i].copy_(m32), v[i].copy_(v32)
+            continue
+        at = torch.arange(g.numel(), device=g.device) & 0xFFFFFFFF
+        r = _mix32((at * 0x9E3779B1 + _mix32((key + i * 0x85EBCA77) & 0xFFFFFFFF)) & 0xFFFFFFFF)
+        for codes, scales, new, bits, root_ in ((m[i], m_scales[i], m32, r & 0xFFFF, False), (v[i], v_scales[i], root, r >> 16, True)):
+            c, s = encode_state(new, bits, root_)
+            codes.copy_(c), scales.view(torch.uint8).copy_(s.view(torch.uint8))
+    return norm
+
+
+def _pointers(ts: Optional[Sequence[torch.Tensor]]):
+    return None if ts is None else (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
+
+
+def _check_lists(params, grads, masters, m, v, step, m_scales, v_scales):
+    n = len(params)
+    _need(n > 0, "no parameters")
+    for name, ts in (("grads", grads), ("masters", masters), ("m", m), ("v", v), ("m_scales", m_scales), ("v_scales", v_scales)):
+        _need(ts is None or len(ts) == n, f"{n} parameters, but {0 if ts is None else len(ts)} {name}")
+    _need((m_scales is None) == (v_scales is None), "8-bit moments have scales of m and of v")
+    dev, ptype, gtype = params[0].device, params[0].dtype, grads[0].dtype
+    _need(ptype in _TYPES and gtype in _TYPES, f"parameters and gradients are bfloat16, float16 or float32, not {ptype} and {gtype}")
+    _need(masters is not None or ptype == torch.float32, f"{ptype} parameters need fp32 masters")
+    _need(step.dtype == torch.int64 and step.numel() == 1 and step.device == dev, "step has to be one int64 on the parameters' device")
+    state = torch.float32 if m_scales is None else E4M3
+    for i in range(n):
+        size = params[i].numel()
+        group = [(params[i], ptype, size), (grads[i], gtype, size), (m[i], state, size), (v[i], state, size)]
+        if masters is not None:
+            group.append((masters[i], torch.float32, size))
+        if m_scales is not None:
+            group += [(m_scales[i], E8M0, state_scales(size)), (v_scales[i], E8M0, state_scales(size))]
+        for t, dtype, count in group:
+            if not (t.dtype == dtype and t.numel() == count and t.device == dev and t.is_contiguous()):
+                raise ValueError(f"tensor {i}: {tuple(t.shape)} {t.dtype} on {t.device} where a contiguous one of {count} {dtype} on {dev} belongs")
+
+
+def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], masters: Optional[Sequence[torch.Tensor]],
+                m: Sequence[torch.Tensor], v: Sequence[torch.Tensor], step: torch.Tensor, *, lr: float, beta1: float, beta2: float,
+                eps: float, weight_decay: float, grad_scale: float = 1.0, clip: Optional[float] = None,
+                m_scales: Optional[Sequence[torch.Tensor]] = None, v_scales: Optional[Sequence[torch.Tensor]] = None,
+                seed: int = 0) -> Optional[torch.Tensor]:
+    """One AdamW step over lists of contiguous tensors, in place; returns the norm of the scaled gradients (fp32, one element)
+    where ``clip`` limits it, else None.
+
+    params: bf16, fp16 or fp32, all of one type; grads: of one type; masters: fp32 (None: fp32 parameters are their own).
+    m, v: fp32 moments; with ``m_scales`` and ``v_scales`` (float8_e8m0fnu, one per 256 values) codes in float8_e4m3fn of m and
+    of sqrt(v), rounded stochastically by a hash of ``seed``, step, tensor and element: right on average, and the same bits
+    for the same inputs.  ``step``: one int64 on the device, counted up by the call, so a captured step can be replayed; all
+    other numbers are the call's.  A gradient that is not finite makes its own element NaN, and with ``clip`` all."""
+    _check_lists(params, grads, masters, m, v, step, m_scales, v_scales)
+    _need(clip is None or clip > 0, "clip has to be positive")
+    if not params[0].is_cuda:
+        return adamw_multi_reference(params, grads, masters, m, v, step, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
+                                     weight_decay=weight_decay, grad_scale=grad_scale, clip=clip, m_scales=m_scales, v_scales=v_scales, seed=seed)
+    n, lib = len(params), _lib.load()
+    lib.dcpk_adamw_multi_work.restype = ctypes.c_long
+    f = ctypes.c_float
+    with _on(step):
+        work = torch.empty(lib.dcpk_adamw_multi_work(ctypes.c_int(n)), dtype=torch.float64, device=step.device)
+        norm = torch.empty(1, dtype=torch.float32, device=step.device) if clip is not None else None
+        sizes = (ctypes.c_long * n)(*[p.numel() for p in params])
+        _lib.check(lib.dcpk_adamw_multi(
+            ctypes.c_int(n), _pointers(params), _pointers(grads), _pointers(masters), _pointers(m), _pointers(v), _pointers(m_scales),
+            _pointers(v_scales), sizes, ctypes.c_int(_TYPES[params[0].dtype]), ctypes.c_int(_TYPES[grads[0].dtype]), _lib.ptr(step), f(lr),
+            f(beta1), f(beta2), f(eps), f(weight_decay), f(grad_scale), f(clip or 0.0), ctypes.c_uint(seed & 0xFFFFFFFF),
+            None if norm is None else _lib.ptr(norm), _lib.ptr(work), _lib.stream_handle()), "adamw_multi")
+    return norm
