@@ -44,7 +44,7 @@ struct AdamList {
   uint8_t aligned[kAdamTensors];
   int n, base;               // base: tensors in launches before
 };
-struct AdamScalars { float lr, beta1, beta2, eps, wd, grad_scale; };
+struct AdamScalars { float lr, beta1, rest1, beta2, rest2, eps, wd; };   // rest: 1 - beta
 // what a step's kernels hand on, in global memory
 struct AdamShared { float coef, bc1, root_bc2; uint32_t key; };
 
@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
 }
 
 // step counter, bias corrections, clipping coefficient: one CTA
-__global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __restrict__ parts, int n_parts, int64_t* __restrict__ step, float beta1,
-                                                            float beta2, float grad_scale, float clip, uint32_t seed, float* __restrict__ norm,
+__global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __restrict__ parts, int n_parts, int64_t* __restrict__ step, double beta1,
+                                                            double beta2, float grad_scale, float clip, uint32_t seed, float* __restrict__ norm,
                                                             AdamShared* __restrict__ shared) {
   __shared__ double sums[8];
   grid_wait();
@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __rest
     coef *= c > 1.f ? 1.f : c;   // a NaN norm gives NaN
   }
   shared->coef = coef;
-  shared->bc1 = float(1.0 / (1.0 - pow(double(beta1), double(now))));
-  shared->root_bc2 = float(sqrt(1.0 / (1.0 - pow(double(beta2), double(now)))));
+  shared->bc1 = float(1.0 / (1.0 - pow(beta1, double(now))));
+  shared->root_bc2 = float(sqrt(1.0 / (1.0 - pow(beta2, double(now)))));
   shared->key = mix32(seed + uint32_t(now) * 0x9e3779b1u);
 }
 
@@ -236,8 +236,10 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_multi_kernel(const __grid_
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       g[j] *= now.coef;
-      m[j] = s.beta1 * m[j] + (1.f - s.beta1) * g[j];
-      v[j] = s.beta2 * v[j] + (1.f - s.beta2) * g[j] * g[j];
+      // each rounded by itself: old moments and gradients are short numbers, so blocks whose largest value lies on the very
+      // border between two scales are not rare, and a fused product would take them to the other side than the formula
+      m[j] = __fadd_rn(__fmul_rn(s.beta1, m[j]), __fmul_rn(s.rest1, g[j]));
+      v[j] = __fadd_rn(__fmul_rn(s.beta2, v[j]), __fmul_rn(__fmul_rn(s.rest2, g[j]), g[j]));
       root[j] = sqrtf(v[j]);
       w[j] -= s.lr * (m[j] * now.bc1 / (root[j] * now.root_bc2 + s.eps) + s.wd * w[j]);
     }
@@ -271,7 +273,7 @@ extern "C" long dcpk_adamw_multi_work(int n_tensors) { return 2 + long((n_tensor
 // device, counted up.  clip <= 0: none, and norm is not written.
 extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* const* grads, void* const* masters, void* const* ms,
                                 void* const* vs, void* const* m_scales, void* const* v_scales, const long* sizes, int param_type, int grad_type,
-                                int64_t* step, float lr, float beta1, float beta2, float eps, float wd, float grad_scale, float clip,
+                                int64_t* step, float lr, double beta1, double beta2, float eps, float wd, float grad_scale, float clip,
                                 unsigned seed, float* norm, double* work, void* stream) {
   if (n_tensors < 0 || param_type < 0 || param_type > 2 || grad_type < 0 || grad_type > 2) return -3;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -324,7 +326,7 @@ extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* 
   if (launch_overlapped(adamw_prepare_kernel, dim3(1), 256, 0, s, 1, !first, static_cast<const double*>(parts), n_parts, step, beta1, beta2,
                         grad_scale, clip, uint32_t(seed), norm, shared) != cudaSuccess || cudaGetLastError() != cudaSuccess)
     return -5;
-  const AdamScalars scalars = {lr, beta1, beta2, eps, wd, grad_scale};
+  const AdamScalars scalars = {lr, float(beta1), float(1.0 - beta1), float(beta2), float(1.0 - beta2), eps, wd};
   for (int base = 0; base < n_tensors;) {
     base += fill(list, base);
     const int chunks = list.first_chunk[list.n];

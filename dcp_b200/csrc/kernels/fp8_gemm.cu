@@ -109,19 +109,24 @@ __device__ __forceinline__ uint32_t scale_word(const GemmOperand& o, int row, in
   return v;
 }
 
-// one result (and what it is added to) in the output's type
-__device__ __forceinline__ void store_result(const GemmArgs& a, int q, int p, float v) {
-  const size_t at = size_t(q) * a.out_pitch + p, from = size_t(q) * a.add_pitch + p;
-  if (a.out_type == kTypeBf16) {
-    if (a.add) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.add)[from]);
-    static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
-  } else if (a.out_type == kTypeF16) {
-    if (a.add) v += __half2float(static_cast<const __half*>(a.add)[from]);
-    static_cast<__half*>(a.out)[at] = __float2half_rn(v);
-  } else {
-    if (a.add) v += static_cast<const float*>(a.add)[from];
-    static_cast<float*>(a.out)[at] = v;
-  }
+template <int kType> struct OutType;
+template <> struct OutType<kTypeF32> { using T = float; };
+template <> struct OutType<kTypeF16> { using T = __half; };
+template <> struct OutType<kTypeBf16> { using T = __nv_bfloat16; };
+
+// f(type, added) with the output's type and whether there is something to add as constants: a test per store made a tile's
+// stores take 50000 cycles
+template <typename F>
+__device__ __forceinline__ void by_output(const GemmArgs& a, F f) {
+  if (a.out_type == kTypeBf16) a.add ? f(OutType<kTypeBf16>(), std::true_type()) : f(OutType<kTypeBf16>(), std::false_type());
+  else if (a.out_type == kTypeF16) a.add ? f(OutType<kTypeF16>(), std::true_type()) : f(OutType<kTypeF16>(), std::false_type());
+  else a.add ? f(OutType<kTypeF32>(), std::true_type()) : f(OutType<kTypeF32>(), std::false_type());
+}
+// one result, rounded once; `from` is read where something is added
+template <bool kAdd, typename T>
+__device__ __forceinline__ void store_result(T* to, const T* from, float v) {
+  if (kAdd) v += to_float(*from);
+  *to = from_float<T>(v);
 }
 
 struct __align__(1024) GemmSmem {
@@ -197,11 +202,16 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(empty_bar);   // the results are in registers: the next tile's products may come
       const int p = (tp * 2 + X) * 128 + quad * 32 + lane, q0 = tq * 256 + half * 128;
-      if (p < args.p.rows) {
+      if (p < args.p.rows)
+        by_output(args, [&](auto type, auto added) {
+          using T = typename decltype(type)::T;
+          T* to = static_cast<T*>(args.out) + size_t(q0) * args.out_pitch + p;
+          const T* from = static_cast<const T*>(args.add) + size_t(q0) * args.add_pitch + p;
+          const int n = args.q.rows - q0;
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (q0 + c < args.q.rows) store_result(args, q0 + c, p, __uint_as_float(acc[c]));
-      }
+          for (int c = 0; c < 128; ++c, to += args.out_pitch, from += args.add_pitch)
+            if (c < n) store_result<decltype(added)::value>(to, from, __uint_as_float(acc[c]));
+        });
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ scales: every warp to its quarter of the lanes
@@ -410,6 +420,8 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
         if (++stage == kStages) { stage = 0; ph ^= 1; }
       }
       umma_commit(&sm.acc_full);
+      // TMEM and operands stay until all has retired
+      for (int spin = 0; spin < 200000 && !mbar_try_wait(&sm.acc_full, 0); ++spin) {}
     }
   } else if (warp >= 4) {
     const int quad = warp & 3;
@@ -442,10 +454,19 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
         uint32_t acc[16];
         tmem_ld16(tmem + (uint32_t(quad * 32) << 16) + c0, acc);
         tmem_wait_ld();
+        if (splits > 1) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          if (splits > 1) sm.part[c0 + c][row] = __uint_as_float(acc[c]);
-          else if (p < args.p.rows && q0 + c0 + c < args.q.rows) store_result(args, q0 + c0 + c, p, __uint_as_float(acc[c]));
+          for (int c = 0; c < 16; ++c) sm.part[c0 + c][row] = __uint_as_float(acc[c]);
+        } else if (p < args.p.rows) {
+          by_output(args, [&](auto type, auto added) {
+            using T = typename decltype(type)::T;
+            T* to = static_cast<T*>(args.out) + size_t(q0 + c0) * args.out_pitch + p;
+            const T* from = static_cast<const T*>(args.add) + size_t(q0 + c0) * args.add_pitch + p;
+            const int n = args.q.rows - q0 - c0;
+#pragma unroll
+            for (int c = 0; c < 16; ++c, to += args.out_pitch, from += args.add_pitch)
+              if (c < n) store_result<decltype(added)::value>(to, from, __uint_as_float(acc[c]));
+          });
         }
       }
       tc_fence_before();
@@ -458,17 +479,22 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
     if (warp >= 4 && !sm.abort_word) {
       const int row = threadIdx.x & 127, p = p0 + row, n = min(kN, args.q.rows - q0);
       const uint32_t at = smem_u32(&sm.part[0][row]);
-      for (int c = n * rank / splits; c < n * (rank + 1) / splits; ++c) {
-        float v[kSplitMax];
+      by_output(args, [&](auto type, auto added) {
+        using T = typename decltype(type)::T;
+        for (int c = n * rank / splits; c < n * (rank + 1) / splits; ++c) {
+          float v[kSplitMax];
 #pragma unroll
-        for (int r = 0; r < kSplitMax; ++r)
-          if (r < splits) v[r] = __uint_as_float(ld_cluster_u32(at + c * 512, r));
-        float sum = v[0];
+          for (int r = 0; r < kSplitMax; ++r)
+            if (r < splits) v[r] = __uint_as_float(ld_cluster_u32(at + c * 512, r));
+          float sum = v[0];
 #pragma unroll
-        for (int r = 1; r < kSplitMax; ++r)
-          if (r < splits) sum += v[r];
-        if (p < args.p.rows) store_result(args, q0 + c, p, sum);
-      }
+          for (int r = 1; r < kSplitMax; ++r)
+            if (r < splits) sum += v[r];
+          if (p < args.p.rows)
+            store_result<decltype(added)::value>(static_cast<T*>(args.out) + size_t(q0 + c) * args.out_pitch + p,
+                                                 static_cast<const T*>(args.add) + size_t(q0 + c) * args.add_pitch + p, sum);
+        }
+      });
     }
     cluster_sync();
   } else {

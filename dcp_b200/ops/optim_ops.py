@@ -138,7 +138,7 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
                                      weight_decay=weight_decay, grad_scale=grad_scale, clip=clip, m_scales=m_scales, v_scales=v_scales, seed=seed)
     n, lib = len(params), _lib.load()
     lib.dcpk_adamw_multi_work.restype = ctypes.c_long
-    f = ctypes.c_float
+    f, d = ctypes.c_float, ctypes.c_double
     with _on(step):
         work = torch.empty(lib.dcpk_adamw_multi_work(ctypes.c_int(n)), dtype=torch.float64, device=step.device)
         norm = torch.empty(1, dtype=torch.float32, device=step.device) if clip is not None else None
@@ -146,6 +146,6 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
         _lib.check(lib.dcpk_adamw_multi(
             ctypes.c_int(n), _pointers(params), _pointers(grads), _pointers(masters), _pointers(m), _pointers(v), _pointers(m_scales),
             _pointers(v_scales), sizes, ctypes.c_int(_TYPES[params[0].dtype]), ctypes.c_int(_TYPES[grads[0].dtype]), _lib.ptr(step), f(lr),
-            f(beta1), f(beta2), f(eps), f(weight_decay), f(grad_scale), f(clip or 0.0), ctypes.c_uint(seed & 0xFFFFFFFF),
+            d(beta1), d(beta2), f(eps), f(weight_decay), f(grad_scale), f(clip or 0.0), ctypes.c_uint(seed & 0xFFFFFFFF),
             None if norm is None else _lib.ptr(norm), _lib.ptr(work), _lib.stream_handle()), "adamw_multi")
     return norm
