@@ -20,6 +20,7 @@
 
 #include "fp8_common.cuh"
 #include "launch.cuh"
+#include "ptx.cuh"
 
 namespace dcpk {
 
@@ -48,9 +49,14 @@ struct AdamScalars { float lr, beta1, rest1, beta2, rest2, eps, wd; };   // rest
 // what a step's kernels hand on, in global memory
 struct AdamShared { float coef, bc1, root_bc2; uint32_t key; };
 
-__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {   // finaliser of MurmurHash3 (A. Appleby, public domain)
+// finaliser of MurmurHash3 (A. Appleby, public domain), and without its last step
+__device__ __forceinline__ uint32_t mix32_open(uint32_t x) {
   x ^= x >> 16; x *= 0x85ebca6bu;
   x ^= x >> 13; x *= 0xc2b2ae35u;
+  return x;
+}
+__device__ __forceinline__ uint32_t mix32(uint32_t x) {
+  x = mix32_open(x);
   return x ^ (x >> 16);
 }
 
@@ -64,12 +70,34 @@ __device__ __forceinline__ int find_tensor(const AdamList& list, int chunk) {
   return lo;
 }
 
+// Eight neighbours, a 16-byte access in 16-bit types and one of 32 bytes in fp32 (two of 16 bytes, each of which touches all
+// sectors of the warp's 1024 bytes: see the kernel's figures); otherwise one by one, every 32nd.
+__device__ __forceinline__ void load_near(const float* p, float (&f)[8]) {
+  uint32_t r[8];
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p) : "memory");
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(r[j]);
+}
+template <typename T>
+__device__ __forceinline__ void load_near(const T* p, float (&f)[8]) {
+  Raw8<T> raw;
+  load_raw(raw, p);
+  widen(raw, f);
+}
+__device__ __forceinline__ void store_near(float* p, const float (&f)[8]) {
+  uint32_t r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(f[j]);
+  st_global_v8(p, r);
+}
+template <typename T>
+__device__ __forceinline__ void store_near(T* p, const float (&f)[8]) { store8(p, f); }
+
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, long e0, int lane, long n, bool vec, float (&f)[8]) {
   if (vec) {
-    Raw8<T> raw;
-    load_raw(raw, p + e0 + lane * 8);
-    widen(raw, f);
+    load_near(p + e0 + lane * 8, f);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = e0 + j * 32 + lane < n ? to_float(p[e0 + j * 32 + lane]) : 0.f;
@@ -78,7 +106,7 @@ __device__ __forceinline__ void load8(const T* p, long e0, int lane, long n, boo
 template <typename T>
 __device__ __forceinline__ void put8(T* p, long e0, int lane, long n, bool vec, const float (&f)[8]) {
   if (vec) {
-    store8(p + e0 + lane * 8, f);
+    store_near(p + e0 + lane * 8, f);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -90,7 +118,8 @@ __device__ __forceinline__ float2 from_codes2(uint32_t c) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(c)));
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-__device__ __forceinline__ void load_state8(const uint8_t* p, long e0, int lane, long n, bool vec, float scale, float (&f)[8]) {
+// codes as values, without their scale
+__device__ __forceinline__ void load_codes8(const uint8_t* p, long e0, int lane, long n, bool vec, float (&f)[8]) {
   uint32_t w[2] = {0, 0};
   if (vec) {
     const uint2 r = *reinterpret_cast<const uint2*>(p + e0 + lane * 8);
@@ -103,62 +132,123 @@ __device__ __forceinline__ void load_state8(const uint8_t* p, long e0, int lane,
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 t = from_codes2(w[i >> 1] >> (16 * (i & 1)));
-    f[2 * i] = t.x * scale; f[2 * i + 1] = t.y * scale;
+    f[2 * i] = t.x; f[2 * i + 1] = t.y;
   }
 }
-// Codes of a block's values, at random to one of the two neighbours.  2^-120 takes e4m3's smallest exponent to fp32's: the cut
-// of the bits goes through its denormals too.
-template <bool kRoot>
-__device__ __forceinline__ void store_state8(uint8_t* p, uint8_t* scale, long e0, int lane, long n, bool vec, const float (&f)[8],
-                                             const uint32_t (&random)[8]) {
-  uint32_t amax = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
-    amax = max(amax, b < 0x7f800000u ? b : 0u);
-  }
-  const int byte = scale_byte<8>(__reduce_max_sync(0xffffffffu, amax));
-  const float inv = scale_inverse(byte);
-  uint32_t code[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float a = fabsf(f[j]);
-    uint32_t c = (__float_as_uint(a * inv * 0x1p-120f) + ((kRoot ? random[j] >> 16 : random[j] & 0xffffu) << 4)) >> 20;
-    c = min(c, 0x7eu);
-    if (kRoot && a > 0.f) c = max(c, 1u);
-    if (!(a < INFINITY)) c = 0x7fu;
-    code[j] = c | (kRoot ? 0u : (__float_as_uint(f[j]) >> 31) << 7);
-  }
+__device__ __forceinline__ void store_codes8(uint8_t* p, long e0, int lane, long n, bool vec, uint2 r) {
   if (vec) {
-    uint2 r;
-    r.x = code[0] | (code[1] << 8) | (code[2] << 16) | (code[3] << 24);
-    r.y = code[4] | (code[5] << 8) | (code[6] << 16) | (code[7] << 24);
     *reinterpret_cast<uint2*>(p + e0 + lane * 8) = r;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (e0 + j * 32 + lane < n) p[e0 + j * 32 + lane] = uint8_t(code[j]);
+      if (e0 + j * 32 + lane < n) p[e0 + j * 32 + lane] = uint8_t((j < 4 ? r.x : r.y) >> (8 * (j & 3)));
   }
-  if (lane == 0) *scale = uint8_t(byte);
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {   // NaN if one is
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Square root by one step of Newton's iteration with the residual of a fused product: to nearest but for one value in a
+// million, without sqrtf's branch for the ends of the range.  Zero for zero; below 2^-126 too small.
+__device__ __forceinline__ float root_of(float v) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(v, 1.17549435e-38f)));
+  const float r = v * y;
+  return fmaf(fmaf(-r, r, v), 0.5f * y, r);
+}
+__device__ __forceinline__ float inverse_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Codes of a block's values, at random to one of the two neighbours; `amax` is the block's largest magnitude.  A product
+// with 2^-120 / scale takes e4m3's smallest exponent to fp32's: the code is bits 20 to 26 then, for its denormals too, and
+// the cut is a shift.  The largest magnitude is at most 448 * scale, whose bits below the code are zero: no sum goes past the
+// code 0x7e.
+template <bool kRoot>
+__device__ __forceinline__ uint2 encode8(float amax, const float (&f)[8], const uint32_t (&random)[8], int& byte) {
+  uint32_t top[8];   // the code in the upper byte
+  // 16 random bits are added behind the code, the upper ones of the hash or the lower, whose last step (x ^ x >> 16) is done
+  // here.  Not as (bits << 4) + __byte_perm(...), which is an instruction less: ptxas of CUDA 12.9 makes codes of zero of that.
+  const auto cut = [](uint32_t bits, uint32_t x) { return (bits + ((kRoot ? x >> 12 : (x << 4) ^ (x >> 12)) & 0xffff0u)) << 4; };
+  byte = scale_byte<8>(__float_as_uint(amax));
+  if (byte <= 156) {   // 2^-120 / scale is a float
+    const float inv = byte <= 133 ? __uint_as_float(uint32_t(134 - byte) << 23) : __uint_as_float(0x00400000u >> (byte - 134));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t bits = __float_as_uint(fabsf(f[j]) * inv);
+      if (kRoot) bits = max(bits, min(__float_as_uint(f[j]), 0x00100000u));
+      top[j] = cut(bits, random[j]);
+      if (!kRoot) top[j] |= __float_as_uint(f[j]) & 0x80000000u;
+    }
+  } else {             // huge, or something that is not finite: those become NaN and do not count for the scale
+    uint32_t finite = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
+      finite = max(finite, b < 0x7f800000u ? b : 0u);
+    }
+    byte = scale_byte<8>(__reduce_max_sync(0xffffffffu, finite));
+    const float inv = scale_inverse(byte);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = fabsf(f[j]);
+      uint32_t bits = __float_as_uint(a * inv * 0x1p-120f);
+      if (kRoot && a > 0.f) bits = max(bits, 0x00100000u);
+      top[j] = cut(bits, random[j]);
+      if (!(a < INFINITY)) top[j] = 0x7f000000u;
+      if (!kRoot) top[j] |= __float_as_uint(f[j]) & 0x80000000u;
+    }
+  }
+  const auto four = [&](int i) {
+    return __byte_perm(__byte_perm(top[i], top[i + 1], 0x0073), __byte_perm(top[i + 2], top[i + 3], 0x0073), 0x5410);
+  };
+  return make_uint2(four(0), four(4));
 }
 
-// sum of squares of a CTA's gradients, from the threads' sums on in 64 bits; `parts` are added up in order
+// Sum of squares of a CTA's gradients, from the threads' sums on in 64 bits; `parts` are added up in order.  A CTA has a
+// run of chunks, so that it looks for its tensor once and has four loads per thread under way (a chunk at a time from a
+// grid of CTAs: 436 MB in 144 us).
 template <typename G>
 __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_constant__ AdamList list, float grad_scale, double* __restrict__ parts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
   float sq[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   grid_wait();
-  for (int chunk = blockIdx.x; chunk < n_chunks; chunk += gridDim.x) {
-    const int i = find_tensor(list, chunk);
-    const long e0 = long(chunk - list.first_chunk[i]) * kChunk + warp * kStateBlock, n = list.t[i].n;
-    if (e0 >= n) continue;
-    float g[8];
-    load8(static_cast<const G*>(list.t[i].grad), e0, lane, n, list.aligned[i] && e0 + kStateBlock <= n, g);
+  int chunk = int(long(n_chunks) * blockIdx.x / gridDim.x);
+  const int stop = int(long(n_chunks) * (blockIdx.x + 1) / gridDim.x);
+  for (int i = find_tensor(list, chunk); chunk < stop; ++i) {
+    const int last = min(stop, list.first_chunk[i + 1]);   // of this tensor
+    const long n = list.t[i].n;
+    const G* grad = static_cast<const G*>(list.t[i].grad);
+    long e0 = long(chunk - list.first_chunk[i]) * kChunk;
+    const long end = min(n, long(last - list.first_chunk[i]) * kChunk);
+    const auto add = [&](const float (&g)[8]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      g[j] *= grad_scale;
-      sq[j] += g[j] * g[j];
+      for (int j = 0; j < 8; ++j) {
+        const float x = g[j] * grad_scale;
+        sq[j] += x * x;
+      }
+    };
+    if (list.aligned[i])
+      for (; e0 + 4 * kChunk <= end; e0 += 4 * kChunk) {
+        Raw8<G> raw[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) load_raw(raw[u], grad + e0 + u * kChunk + threadIdx.x * 8);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float g[8];
+          widen(raw[u], g);
+          add(g);
+        }
+      }
+    for (; e0 < end; e0 += kChunk) {
+      const long at = e0 + warp * kStateBlock;
+      float g[8];
+      load8(grad, at, lane, n, list.aligned[i] && at + kStateBlock <= n, g);
+      add(g);
     }
+    chunk = last;
   }
   grid_let_next();
   double t = 0.0;
@@ -207,54 +297,89 @@ __global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __rest
   shared->key = mix32(seed + uint32_t(now) * 0x9e3779b1u);
 }
 
+// All CTAs walk the chunks together: neighbours in time are neighbours in memory (a run of chunks for each CTA: 896 -> 979 us
+// for 218M parameters in 8 bits).
 template <typename P, typename G, bool kMaster, bool kEight>
-__global__ void __launch_bounds__(kAdamThreads) adamw_multi_kernel(const __grid_constant__ AdamList list, const AdamScalars s,
-                                                                   const AdamShared* __restrict__ shared) {
+__global__ void __launch_bounds__(kAdamThreads, kEight ? 4 : 5) adamw_multi_kernel(const __grid_constant__ AdamList list, const AdamScalars s,
+                                                                                   const AdamShared* __restrict__ shared) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
   grid_wait();
-  const AdamShared now = *shared;
-  for (int chunk = blockIdx.x; chunk < n_chunks; chunk += gridDim.x) {
-    const int i = find_tensor(list, chunk);
+  const float coef = shared->coef, bc1 = shared->bc1, root_bc2 = shared->root_bc2;
+  int chunk = blockIdx.x;
+  for (int i = find_tensor(list, chunk); chunk < n_chunks; ++i) {
     const AdamTensor& t = list.t[i];
-    const long e0 = long(chunk - list.first_chunk[i]) * kChunk + warp * kStateBlock, n = t.n, block = e0 / kStateBlock;
-    if (e0 >= n) continue;
-    const bool vec = list.aligned[i] && e0 + kStateBlock <= n;
-    float g[8], w[8], m[8], v[8];
-    load8(static_cast<const G*>(t.grad), e0, lane, n, vec, g);
-    if (kMaster) load8(static_cast<const float*>(t.master), e0, lane, n, vec, w);
-    else load8(static_cast<const P*>(t.param), e0, lane, n, vec, w);
-    if (kEight) {
-      load_state8(static_cast<const uint8_t*>(t.m), e0, lane, n, vec, scale_value(t.m_scale[block]), m);
-      load_state8(static_cast<const uint8_t*>(t.v), e0, lane, n, vec, scale_value(t.v_scale[block]), v);
+    const long n = t.n;
+    const uint32_t key = kEight ? mix32(shared->key + uint32_t(list.base + i) * 0x85ebca77u) : 0u;
+    const auto block = [&](long e0, auto whole) {
+      const bool vec = whole;
+      float g[8], w[8], m[8], v[8];
+      load8(static_cast<const G*>(t.grad), e0, lane, n, vec, g);
+      if (kMaster) load8(static_cast<const float*>(t.master), e0, lane, n, vec, w);
+      else load8(static_cast<const P*>(t.param), e0, lane, n, vec, w);
+      if (kEight) {
+        const long at = e0 / kStateBlock;
+        // the scales are powers of two: they go into the factors the codes are multiplied with anyway
+        load_codes8(static_cast<const uint8_t*>(t.m), e0, lane, n, vec, m);
+        load_codes8(static_cast<const uint8_t*>(t.v), e0, lane, n, vec, v);
+        const float m_scale = scale_value(t.m_scale[at]), v_scale = scale_value(t.v_scale[at]);
+        const float keep_m = s.beta1 * m_scale, keep_v = s.beta2 * v_scale * v_scale;
+        uint32_t random[8];
+        float root[8];
+        float m_max = 0.f, v_max = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= v[j];
-    } else {
-      load8(static_cast<const float*>(t.m), e0, lane, n, vec, m);
-      load8(static_cast<const float*>(t.v), e0, lane, n, vec, v);
-    }
-    float root[8];
+        for (int j = 0; j < 8; ++j) {
+          g[j] *= coef;
+          // each rounded by itself: old moments and gradients are short numbers, so blocks whose largest value lies on the
+          // very border between two scales are not rare, and a fused product would take them to the other side than the
+          // formula
+          m[j] = __fadd_rn(__fmul_rn(keep_m, m[j]), __fmul_rn(s.rest1, g[j]));
+          v[j] = __fadd_rn(__fmul_rn(keep_v, v[j] * v[j]), __fmul_rn(__fmul_rn(s.rest2, g[j]), g[j]));
+          if (j & 1) {
+            m_max = max3_abs(m_max, m[j - 1], m[j]);
+            v_max = max3_abs(v_max, v[j - 1], v[j]);
+          }
+          root[j] = root_of(v[j]);
+          w[j] -= s.lr * (m[j] * bc1 * inverse_approx(root[j] * root_bc2 + s.eps) + s.wd * w[j]);
+          random[j] = mix32_open(uint32_t(e0 + (vec ? lane * 8 + j : j * 32 + lane)) * 0x9e3779b1u + key);
+        }
+        if (kMaster) put8(t.master, e0, lane, n, vec, w);
+        put8(static_cast<P*>(t.param), e0, lane, n, vec, w);
+        int m_byte, v_byte;
+        m_max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m_max)));
+        v_max = sqrtf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v_max))));
+        store_codes8(static_cast<uint8_t*>(t.m), e0, lane, n, vec, encode8<false>(m_max, m, random, m_byte));
+        store_codes8(static_cast<uint8_t*>(t.v), e0, lane, n, vec, encode8<true>(v_max, root, random, v_byte));
+        if (lane == 0) {
+          t.m_scale[at] = uint8_t(m_byte);
+          t.v_scale[at] = uint8_t(v_byte);
+        }
+      } else {
+        load8(static_cast<const float*>(t.m), e0, lane, n, vec, m);
+        load8(static_cast<const float*>(t.v), e0, lane, n, vec, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      g[j] *= now.coef;
-      // each rounded by itself: old moments and gradients are short numbers, so blocks whose largest value lies on the very
-      // border between two scales are not rare, and a fused product would take them to the other side than the formula
-      m[j] = __fadd_rn(__fmul_rn(s.beta1, m[j]), __fmul_rn(s.rest1, g[j]));
-      v[j] = __fadd_rn(__fmul_rn(s.beta2, v[j]), __fmul_rn(__fmul_rn(s.rest2, g[j]), g[j]));
-      root[j] = sqrtf(v[j]);
-      w[j] -= s.lr * (m[j] * now.bc1 / (root[j] * now.root_bc2 + s.eps) + s.wd * w[j]);
-    }
-    if (kMaster) put8(t.master, e0, lane, n, vec, w);
-    put8(static_cast<P*>(t.param), e0, lane, n, vec, w);
-    if (kEight) {
-      uint32_t random[8];
-      const uint32_t key = mix32(now.key + uint32_t(list.base + i) * 0x85ebca77u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) random[j] = mix32(uint32_t(e0 + (vec ? lane * 8 + j : j * 32 + lane)) * 0x9e3779b1u + key);
-      store_state8<false>(static_cast<uint8_t*>(t.m), t.m_scale + block, e0, lane, n, vec, m, random);
-      store_state8<true>(static_cast<uint8_t*>(t.v), t.v_scale + block, e0, lane, n, vec, root, random);
-    } else {
-      put8(static_cast<float*>(t.m), e0, lane, n, vec, m);
-      put8(static_cast<float*>(t.v), e0, lane, n, vec, v);
+        for (int j = 0; j < 8; ++j) {
+          g[j] *= coef;
+          m[j] = s.beta1 * m[j] + s.rest1 * g[j];
+          v[j] = s.beta2 * v[j] + s.rest2 * g[j] * g[j];
+          w[j] -= s.lr * (m[j] * bc1 / (sqrtf(v[j]) * root_bc2 + s.eps) + s.wd * w[j]);
+        }
+        if (kMaster) put8(t.master, e0, lane, n, vec, w);
+        put8(static_cast<P*>(t.param), e0, lane, n, vec, w);
+        put8(static_cast<float*>(t.m), e0, lane, n, vec, m);
+        put8(static_cast<float*>(t.v), e0, lane, n, vec, v);
+      }
+    };
+    const bool aligned = list.aligned[i];
+    for (; chunk < list.first_chunk[i + 1]; chunk += gridDim.x) {
+      const long e0 = long(chunk - list.first_chunk[i]) * kChunk + warp * kStateBlock;
+      if (e0 >= n) continue;
+      const bool vec = aligned && e0 + kStateBlock <= n;
+      if constexpr (kEight) {   // a body for either: the tests inside one take more than the loads
+        if (vec) block(e0, std::true_type());
+        else block(e0, std::false_type());
+      } else {
+        block(e0, vec);
+      }
     }
   }
 }
@@ -296,7 +421,8 @@ extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* 
       t = {params[i], grads[i], has_master ? static_cast<float*>(masters[i]) : nullptr, ms[i], vs[i],
            eight ? static_cast<uint8_t*>(m_scales[i]) : nullptr, eight ? static_cast<uint8_t*>(v_scales[i]) : nullptr, sizes[i]};
       const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-      list.aligned[list.n] = (at(t.param) | at(t.grad) | at(t.master)) % 16 == 0 && (at(t.m) | at(t.v)) % (eight ? 8 : 16) == 0;
+      list.aligned[list.n] = at(t.param) % (param_type ? 16 : 32) == 0 && at(t.grad) % (grad_type ? 16 : 32) == 0 && at(t.master) % 32 == 0 &&
+                             (at(t.m) | at(t.v)) % (eight ? 8 : 32) == 0;
       list.first_chunk[list.n + 1] = int(list.first_chunk[list.n] + chunks);
       ++list.n;
     }

@@ -14,6 +14,8 @@
 
 #include "fp8_common.cuh"
 #include "launch.cuh"
+#include "ptx.cuh"
+#include "smem_limit.h"
 
 namespace dcpk {
 
@@ -39,6 +41,21 @@ __device__ __forceinline__ void load_chunk(const T* row, int chunk, int width, f
       const int c = column(false, chunk, j);
       f[j] = c < width ? to_float(row[c]) : 0.f;
     }
+  }
+}
+template <typename T, bool kAligned>
+__device__ __forceinline__ void load_packed(const T* row, int chunk, int width, Raw8<T>& r) {
+  if (kAligned) {
+    if (chunk * 8 < width) load_raw(r, row + chunk * 8);
+    else r = Raw8<T>{};
+  } else {
+    T v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = column(false, chunk, j);
+      v[j] = c < width ? row[c] : from_float<T>(0.f);
+    }
+    r = *reinterpret_cast<const Raw8<T>*>(v);
   }
 }
 template <bool kAligned, typename T>
@@ -85,6 +102,8 @@ __device__ __forceinline__ float row_sum(float v, float* scratch, int warps) {
 
 static constexpr int kNormThreads = 512;
 static constexpr int kNormWidth = 16384;   // four chunks of eight channels per thread at most
+static constexpr int kMaxStages = 8;       // rows under way in the backward pass
+static constexpr int kRingBytes = 200 * 1024;   // of an SM's shared memory, for all its CTAs
 
 template <typename T, int kVecs, bool kAligned, int kCode>
 __global__ void __launch_bounds__(kNormThreads)
@@ -137,49 +156,92 @@ fp8_norm_kernel(const T* __restrict__ x, long x_pitch, const T* __restrict__ res
 }
 
 // Persistent CTAs: each walks rows blockIdx.x, + gridDim.x, ... and keeps its part of dW in registers; the parts go to
-// `part` [gridDim.x, width], which a second kernel adds up in order: the same bits in every run.  The next row's loads are
-// under way while this one is summed.
-template <typename T, int kVecs, bool kAligned, bool kAdd>
-__global__ void __launch_bounds__(kNormThreads)
+// `part` [gridDim.x, width], which a second kernel adds up in order: the same bits in every run.
+//
+// kRing (rows on 16 bytes): the rows of h, dy and add come by bulk copies into a ring of `stages` rows in shared memory, so
+// that what is under way does not depend on the registers; the barrier inside the row's sum is also what frees the stage.
+// With plain loads at the beginning of a row 5003 rows of 5120 took 62 us (2.9 TB/s).
+template <typename T, int kVecs, bool kRing, bool kAdd>
+__global__ void __launch_bounds__(kVecs == 1 ? 1024 : kVecs == 2 ? 768 : 512)   // 64, 80 and 128 registers
 fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__ w, const float* __restrict__ rstd, const T* __restrict__ dy,
                     long dy_pitch, const T* __restrict__ add, long add_pitch, T* __restrict__ dx, float* __restrict__ part, int n_rows,
-                    int width) {
+                    int width, int stages, int* __restrict__ status) {
   __shared__ float scratch[2][kNormThreads / 32];
-  float wv[kVecs][8], dw[kVecs][8];
-  float xh[kVecs][8], g[kVecs][8], a[kVecs][8];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ int abort_word;
+  extern __shared__ __align__(128) uint8_t ring[];
+  constexpr bool kAligned = kRing;
+  const uint32_t row_bytes = uint32_t(width) * sizeof(T), stage_bytes = row_bytes * (kAdd ? 3 : 2);
+  float dw[kVecs][8];
+  Raw8<T> wv[kVecs];
+  if (kRing) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) mbar_init(&full[i], 1);
+      abort_word = 0;
+      mbar_fence_init();
+    }
+    __syncthreads();
+  }
   grid_wait();
+  const auto fetch = [&](long row, int stage) {   // by one thread
+    if (row >= n_rows) return;
+    uint8_t* to = ring + size_t(stage) * stage_bytes;
+    mbar_expect_tx(&full[stage], stage_bytes);
+    bulk_load(to, h + row * h_pitch, row_bytes, &full[stage]);
+    bulk_load(to + row_bytes, dy + row * dy_pitch, row_bytes, &full[stage]);
+    if (kAdd) bulk_load(to + 2 * row_bytes, add + row * add_pitch, row_bytes, &full[stage]);
+  };
+  if (kRing && threadIdx.x == 0)
+    for (int i = 0; i < stages; ++i) fetch(blockIdx.x + long(i) * gridDim.x, i);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    load_chunk<kAligned>(w, threadIdx.x + i * blockDim.x, width, wv[i]);
+    load_packed<T, kAligned>(w, threadIdx.x + i * blockDim.x, width, wv[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
   }
-  int turn = 0;
+  int turn = 0, stage = 0, parity = 0;
+  bool ok = true;
   for (long row = blockIdx.x; row < n_rows; row += gridDim.x, turn ^= 1) {
     const float r = rstd[row];
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int chunk = threadIdx.x + i * blockDim.x;
-      load_chunk<kAligned>(h + row * h_pitch, chunk, width, xh[i]);
-      load_chunk<kAligned>(dy + row * dy_pitch, chunk, width, g[i]);
-      if (kAdd) load_chunk<kAligned>(add + row * add_pitch, chunk, width, a[i]);
+    float xh[kVecs][8], g[kVecs][8];
+    const T *hr = h + row * h_pitch, *gr = dy + row * dy_pitch, *ar = add + row * add_pitch;
+    if (kRing) {
+      ok = ok && mbar_wait(&full[stage], parity, &abort_word);
+      hr = reinterpret_cast<const T*>(ring + size_t(stage) * stage_bytes);
+      gr = hr + width;
+      ar = gr + width;
     }
     float dot = 0.f;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
+    for (int i = 0; i < kVecs; ++i) {
+      const int chunk = threadIdx.x + i * blockDim.x;
+      float wf[8];
+      load_chunk<kAligned>(hr, chunk, width, xh[i]);
+      load_chunk<kAligned>(gr, chunk, width, g[i]);
+      widen(wv[i], wf);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         xh[i][j] *= r;
         dw[i][j] += g[i][j] * xh[i][j];
-        g[i][j] *= wv[i][j];
+        g[i][j] *= wf[j];
         dot += g[i][j] * xh[i][j];
       }
+    }
     dot = row_sum(dot, scratch[turn], blockDim.x >> 5) / width;   // alternating scratch: one barrier per row
+    if (kRing) {
+      // all are through with the row before: its stage is free
+      const int before = stage == 0 ? stages - 1 : stage - 1;
+      if (threadIdx.x == 0 && row != blockIdx.x) fetch(row + long(stages - 1) * gridDim.x, before);
+      if (++stage == stages) { stage = 0; parity ^= 1; }
+    }
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
+      const int chunk = threadIdx.x + i * blockDim.x;
+      float a[8];
+      if (kAdd) load_chunk<kAligned>(ar, chunk, width, a);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[i][j] = r * (g[i][j] - xh[i][j] * dot) + (kAdd ? a[i][j] : 0.f);
-      store_chunk<kAligned>(dx + row * width, threadIdx.x + i * blockDim.x, width, g[i]);
+      for (int j = 0; j < 8; ++j) g[i][j] = r * (g[i][j] - xh[i][j] * dot) + (kAdd ? a[j] : 0.f);
+      store_chunk<kAligned>(dx + row * width, chunk, width, g[i]);
     }
   }
   grid_let_next();
@@ -190,6 +252,10 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
       const int c = column(kAligned, threadIdx.x + i * blockDim.x, j);
       if (c < width) part[size_t(blockIdx.x) * width + c] = dw[i][j];
     }
+  if (kRing && !ok) {   // copies under way get a millisecond to land
+    atomicExch(status, kStatusBarrierTimeout);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
 }
 
 // 32 columns per CTA, eight threads of a column take every eighth of the parts
@@ -218,90 +284,156 @@ struct QuantizeOut {
   long pitch, scale_pitch;   // of cols: scales[column * scale_pitch + tile row]
 };
 
+// Eight values as they lie in memory and their magnitudes, two to a word in 16-bit types: magnitudes order like their bits
+// there too, so one instruction masks two and one compares two.
+template <typename T> struct Magnitudes { uint32_t m[4]; };
+template <> struct Magnitudes<float> { uint32_t m[8]; };
+
+template <typename T>
+__device__ __forceinline__ Magnitudes<T> magnitudes(const Raw8<T>& r) {
+  constexpr uint32_t kMask = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+  Magnitudes<T> m;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < int(sizeof(m) / 4); ++i) m.m[i] = w[i] & kMask;
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {   // of each half in 16-bit types
+  if (sizeof(T) == 4) return max(a, b);
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <typename T> __device__ __forceinline__ uint32_t as_float_bits(uint32_t m);   // of a magnitude in the low bits
+template <> __device__ __forceinline__ uint32_t as_float_bits<float>(uint32_t m) { return m; }
+template <> __device__ __forceinline__ uint32_t as_float_bits<__nv_bfloat16>(uint32_t m) { return m << 16; }
+template <> __device__ __forceinline__ uint32_t as_float_bits<__half>(uint32_t m) {
+  return __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
+}
+
+// Bound by HBM where rows begin on 16 bytes.  The tile stays packed, so that the registers of four CTAs (two in fp32) fit an
+// SM and their loads, maxima and stores overlap.
 template <typename T, int kWays, bool kAligned, int kCode>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4)
 fp8_quantize_kernel(const T* __restrict__ x, long pitch, QuantizeOut by_rows, QuantizeOut by_cols, int n_rows, int width, int tiles_x) {
   constexpr int kTop = kCode == kCodeE4m3 ? 8 : 15;
-  __shared__ uint32_t column_max[(kWays & kCols) ? 16 : 1][kBlock + 8];
+  constexpr int kWords = sizeof(Magnitudes<T>) / 4, kPer = 8 / kWords;   // values to a word
+  __shared__ uint32_t column_max[(kWays & kCols) ? 16 : 1][kBlock / kPer + 4];
+  __shared__ float column_inv[(kWays & kCols) ? kBlock : 1];
   __shared__ uint32_t warp_max[8];
   const int tile_x = blockIdx.x % tiles_x, tile_y = blockIdx.x / tiles_x;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, chunk = tile_x * 16 + tx;
-  float v[8][8];
+  const int row0 = tile_y * kBlock + ty, rows_left = n_rows - row0;   // thread's rows: row0 + 16 i, i < 8
+  Raw8<T> v[8];
   grid_wait();
+  {
+    const T* p = x + row0 * pitch;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long row = long(tile_y) * kBlock + ty + 16 * i;
-    if (row < n_rows) {
-      load_chunk<kAligned>(x + row * pitch, chunk, width, v[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    for (int i = 0; i < 8; ++i, p += 16 * pitch) {
+      if (16 * i < rows_left) load_packed<T, kAligned>(p, chunk, width, v[i]);
+      else v[i] = Raw8<T>{};
     }
   }
   grid_let_next();
-  if (kWays & kRows) {
+  if (kWays & kCols) {
+    Magnitudes<T> m = magnitudes(v[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long row = long(tile_y) * kBlock + ty + 16 * i;
+    for (int i = 1; i < 8; ++i) {
+      const Magnitudes<T> n = magnitudes(v[i]);
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) m.m[k] = larger<T>(m.m[k], n.m[k]);
+    }
+    // word tx + 16 k: of channels in the order the threads hold them
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) column_max[ty][tx + 16 * k] = m.m[k];
+    __syncthreads();
+    if (threadIdx.x < kBlock) {
+      const int t = threadIdx.x & 15, j = threadIdx.x >> 4;   // the j-th value of thread t
       uint32_t amax = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = amax_bits(amax, v[i][j]);
-      const int byte = scale_byte<kTop>(max_of_16(amax));
-      if (row < n_rows) {
-        store_codes<kAligned>(by_rows.codes + row * by_rows.pitch, chunk, width, to_codes8<kCode>(v[i], scale_inverse(byte)));
-        if (tx == 0) by_rows.scales[row * by_rows.scale_pitch + tile_x] = uint8_t(byte);
+      for (int i = 0; i < 16; ++i) amax = larger<T>(amax, column_max[i][t + 16 * (j / kPer)]);
+      if (sizeof(T) == 2) amax = j & 1 ? amax >> 16 : amax & 0xffffu;
+      const int byte = scale_byte<kTop>(as_float_bits<T>(amax)), c = tile_x * kBlock + column(kAligned, t, j);
+      if (c < width) by_cols.scales[c * by_cols.scale_pitch + tile_y] = uint8_t(byte);
+      column_inv[t + 16 * j] = scale_inverse(byte);
+    }
+  }
+  if (kWays & kRows) {
+    uint8_t* to = by_rows.codes + row0 * by_rows.pitch;
+    uint8_t* scale = by_rows.scales + row0 * by_rows.scale_pitch + tile_x;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {   // two rows at a time: in 16-bit types their maxima share a word
+      uint32_t m[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Magnitudes<T> n = magnitudes(v[i + h]);
+        m[h] = n.m[0];
+#pragma unroll
+        for (int k = 1; k < kWords; ++k) m[h] = larger<T>(m[h], n.m[k]);
+      }
+      if (sizeof(T) == 2) {
+        uint32_t both = larger<T>(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1) both = larger<T>(both, __shfl_xor_sync(0xffffffffu, both, s));
+        m[0] = both & 0xffffu;
+        m[1] = both >> 16;
+      } else {
+        m[0] = max_of_16(m[0]);
+        m[1] = max_of_16(m[1]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h, to += 16 * by_rows.pitch, scale += 16 * by_rows.scale_pitch) {
+        if (16 * (i + h) >= rows_left) continue;
+        const int byte = scale_byte<kTop>(as_float_bits<T>(m[h]));
+        float f[8];
+        widen(v[i + h], f);
+        store_codes<kAligned>(to, chunk, width, to_codes8<kCode>(f, scale_inverse(byte)));
+        if (tx == 0) *scale = uint8_t(byte);
       }
     }
   }
   if (kWays & kBlocks) {
     uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+      const Magnitudes<T> n = magnitudes(v[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = amax_bits(amax, v[i][j]);
+      for (int k = 0; k < kWords; ++k) amax = larger<T>(amax, n.m[k]);
+    }
+    if (sizeof(T) == 2) amax = max(amax >> 16, amax & 0xffffu);
     amax = __reduce_max_sync(0xffffffffu, amax);
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
     __syncthreads();
     amax = warp_max[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) amax = max(amax, warp_max[i]);
-    const int byte = scale_byte<kTop>(amax);
+    const int byte = scale_byte<kTop>(as_float_bits<T>(amax));
     const float inv = scale_inverse(byte);
+    uint8_t* to = by_rows.codes + row0 * by_rows.pitch;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long row = long(tile_y) * kBlock + ty + 16 * i;
-      if (row < n_rows) store_codes<kAligned>(by_rows.codes + row * by_rows.pitch, chunk, width, to_codes8<kCode>(v[i], inv));
+    for (int i = 0; i < 8; ++i, to += 16 * by_rows.pitch) {
+      if (16 * i >= rows_left) continue;
+      float f[8];
+      widen(v[i], f);
+      store_codes<kAligned>(to, chunk, width, to_codes8<kCode>(f, inv));
     }
-    if (threadIdx.x == 0) by_rows.scales[long(tile_y) * by_rows.scale_pitch + tile_x] = uint8_t(byte);
+    if (threadIdx.x == 0) by_rows.scales[tile_y * by_rows.scale_pitch + tile_x] = uint8_t(byte);
   }
   if (kWays & kCols) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t amax = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = amax_bits(amax, v[i][j]);
-      column_max[ty][column(kAligned, tx, j)] = amax;
-    }
-    __syncthreads();
-    if (threadIdx.x < kBlock) {
-      uint32_t amax = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) amax = max(amax, column_max[i][threadIdx.x]);
-      const int byte = scale_byte<kTop>(amax), c = tile_x * kBlock + threadIdx.x;
-      if (c < width) by_cols.scales[c * by_cols.scale_pitch + tile_y] = uint8_t(byte);
-      column_max[0][threadIdx.x] = __float_as_uint(scale_inverse(byte));   // read by this thread alone so far
-    }
     __syncthreads();
     float inv[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) inv[j] = __uint_as_float(column_max[0][column(kAligned, tx, j)]);
+    for (int j = 0; j < 8; ++j) inv[j] = column_inv[tx + 16 * j];
+    uint8_t* to = by_cols.codes + row0 * by_cols.pitch;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long row = long(tile_y) * kBlock + ty + 16 * i;
-      if (row >= n_rows) continue;
+    for (int i = 0; i < 8; ++i, to += 16 * by_cols.pitch) {
+      if (16 * i >= rows_left) continue;
+      float f[8];
+      widen(v[i], f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= inv[j];
-      store_codes<kAligned>(by_cols.codes + row * by_cols.pitch, chunk, width, to_codes8<kCode>(v[i], 1.f));
+      for (int j = 0; j < 8; ++j) f[j] *= inv[j];
+      store_codes<kAligned>(to, chunk, width, to_codes8<kCode>(f, 1.f));
     }
   }
 }
@@ -355,37 +487,48 @@ extern "C" int dcpk_fp8_norm(int type, int code, const void* x, long x_pitch, co
   });
 }
 
-// CTAs of the backward pass, which is also how many rows of `width` floats `part` has
+// CTAs of the backward pass, which is also how many rows of `width` floats `part` has.  As many threads to an SM as the
+// registers allow at two chunks each.
+static int norm_bwd_per_sm(int width) { return std::max(1, std::min(8, 768 / threads_for(width, 2))); }
 extern "C" int dcpk_fp8_norm_bwd_parts(long n_rows, int width) {
-  const long most = threads_for(width, 2) <= 256 ? 148 * 4 : 148 * 2;
-  return int(std::max(1l, std::min(n_rows, most)));
+  return int(std::max(1l, std::min(n_rows, 148l * norm_bwd_per_sm(width))));
 }
+
+static std::atomic<uint64_t> g_ring_raised[18];
 
 // dx [n_rows, width]; dw fp32 [width], written; add: null, or what is added to dx
 extern "C" int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const void* w, const float* rstd, const void* dy, long dy_pitch,
-                                 const void* add, long add_pitch, void* dx, float* dw, float* part, long n_rows, int width, void* stream) {
+                                 const void* add, long add_pitch, void* dx, float* dw, float* part, long n_rows, int width, int* status,
+                                 void* stream) {
   if (width <= 0 || width > kNormWidth || n_rows > 0x7fffffffl || n_rows < 0) return -3;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (n_rows == 0) return cudaMemsetAsync(dw, 0, size_t(width) * 4, s) == cudaSuccess ? 0 : -5;
   const bool aligned = width % 8 == 0 && h_pitch % 8 == 0 && dy_pitch % 8 == 0 && on_16(h) && on_16(w) && on_16(dy) && on_16(dx) &&
                        (!add || (add_pitch % 8 == 0 && on_16(add)));
   const int ctas = dcpk_fp8_norm_bwd_parts(n_rows, width);
-  int vecs = 1;
+  int vecs = threads_for(width, 2) <= 256 && threads_for(width, 1) <= 128 ? 1 : 2;
   while (threads_for(width, vecs) > kNormThreads) vecs <<= 1;
   const int rc = by_type(type, [&](auto* t) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-    const auto launch = [&](auto kernel) {
-      const cudaError_t rc = launch_overlapped(kernel, dim3(ctas), threads_for(width, vecs), 0, s, 1, false, static_cast<const T*>(h), h_pitch,
+    const int stage_bytes = width * int(sizeof(T)) * (add ? 3 : 2);
+    const int stages = std::min(kMaxStages, kRingBytes / norm_bwd_per_sm(width) / stage_bytes);
+    const bool ring = aligned && stages >= 2;
+    const auto launch = [&](auto kernel, int slot) {
+      const int smem = ring ? stages * stage_bytes : 0;
+      if (smem > 48 * 1024 - 512 && raise_smem_limit(kernel, kRingBytes, g_ring_raised[slot]) != cudaSuccess) return -4;
+      const cudaError_t rc = launch_overlapped(kernel, dim3(ctas), threads_for(width, vecs), smem, s, 1, false, static_cast<const T*>(h), h_pitch,
                                                static_cast<const T*>(w), rstd, static_cast<const T*>(dy), dy_pitch, static_cast<const T*>(add),
-                                               add_pitch, static_cast<T*>(dx), part, int(n_rows), width);
+                                               add_pitch, static_cast<T*>(dx), part, int(n_rows), width, stages, status);
       return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
     };
     const auto sized = [&](auto al, auto ad) {
       constexpr bool A = decltype(al)::value, D = decltype(ad)::value;
-      return vecs == 1 ? launch(fp8_norm_bwd_kernel<T, 1, A, D>) : vecs == 2 ? launch(fp8_norm_bwd_kernel<T, 2, A, D>) : launch(fp8_norm_bwd_kernel<T, 4, A, D>);
+      constexpr int base = (std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 6 : 12) + D * 3;
+      return vecs == 1 ? launch(fp8_norm_bwd_kernel<T, 1, A, D>, base) : vecs == 2 ? launch(fp8_norm_bwd_kernel<T, 2, A, D>, base + 1)
+                                                                                  : launch(fp8_norm_bwd_kernel<T, 4, A, D>, base + 2);
     };
     const auto added = [&](auto al) { return add ? sized(al, std::true_type()) : sized(al, std::false_type()); };
-    return aligned ? added(std::true_type()) : added(std::false_type());
+    return ring ? added(std::true_type()) : added(std::false_type());
   });
   if (rc) return rc;
   const cudaError_t rc2 = launch_overlapped(fp8_norm_dw_kernel, dim3((width + 31) / 32), 256, 0, s, 1, true, static_cast<const float*>(part), dw, ctas, width);

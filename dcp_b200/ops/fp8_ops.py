@@ -238,7 +238,7 @@ def rmsnorm_quant_bwd(h: torch.Tensor, w: torch.Tensor, rstd: torch.Tensor, dy: 
         _lib.check(lib.dcpk_fp8_norm_bwd(
             _c_int(_TYPES[h.dtype]), _lib.ptr(h), _c_long(_pitch(h)), _lib.ptr(w), _lib.ptr(rstd), _lib.ptr(dy), _c_long(_pitch(dy)),
             _NULL if add is None else _lib.ptr(add), _c_long(0 if add is None else _pitch(add)), _lib.ptr(dx), _lib.ptr(dw),
-            _lib.ptr(part), _c_long(rows), _c_int(width), _lib.stream_handle()), "fp8_norm_bwd")
+            _lib.ptr(part), _c_long(rows), _c_int(width), _lib.ptr(_status(h.device)), _lib.stream_handle()), "fp8_norm_bwd")
     return dx, dw
 
 
