@@ -104,6 +104,17 @@ __device__ __forceinline__ void load8(const T* p, long e0, int lane, long n, boo
   }
 }
 template <typename T>
+__device__ __forceinline__ void load8(const T* p, long e0, int lane, long n, bool vec, Raw8<T>& r) {   // as they lie in memory
+  if (vec) {
+    load_raw(r, p + e0 + lane * 8);
+  } else {
+    T v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = e0 + j * 32 + lane < n ? p[e0 + j * 32 + lane] : from_float<T>(0.f);
+    r = *reinterpret_cast<const Raw8<T>*>(v);
+  }
+}
+template <typename T>
 __device__ __forceinline__ void put8(T* p, long e0, int lane, long n, bool vec, const float (&f)[8]) {
   if (vec) {
     store_near(p + e0 + lane * 8, f);
@@ -118,17 +129,17 @@ __device__ __forceinline__ float2 from_codes2(uint32_t c) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(c)));
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-// codes as values, without their scale
-__device__ __forceinline__ void load_codes8(const uint8_t* p, long e0, int lane, long n, bool vec, float (&f)[8]) {
+__device__ __forceinline__ uint2 load_codes8(const uint8_t* p, long e0, int lane, long n, bool vec) {
+  if (vec) return *reinterpret_cast<const uint2*>(p + e0 + lane * 8);
   uint32_t w[2] = {0, 0};
-  if (vec) {
-    const uint2 r = *reinterpret_cast<const uint2*>(p + e0 + lane * 8);
-    w[0] = r.x; w[1] = r.y;
-  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (e0 + j * 32 + lane < n) w[j >> 2] |= uint32_t(p[e0 + j * 32 + lane]) << (8 * (j & 3));
-  }
+  for (int j = 0; j < 8; ++j)
+    if (e0 + j * 32 + lane < n) w[j >> 2] |= uint32_t(p[e0 + j * 32 + lane]) << (8 * (j & 3));
+  return make_uint2(w[0], w[1]);
+}
+// codes as values, without their scale
+__device__ __forceinline__ void widen_codes(uint2 r, float (&f)[8]) {
+  const uint32_t w[2] = {r.x, r.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 t = from_codes2(w[i >> 1] >> (16 * (i & 1)));
@@ -297,10 +308,18 @@ __global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __rest
   shared->key = mix32(seed + uint32_t(now) * 0x9e3779b1u);
 }
 
+template <typename G>
+struct Block8 {   // a lane's part of a block with moments in 8 bits
+  Raw8<G> grad;
+  float w[8];
+  uint2 m, v;
+  int m_byte, v_byte;
+};
+
 // All CTAs walk the chunks together: neighbours in time are neighbours in memory (a run of chunks for each CTA: 896 -> 979 us
 // for 218M parameters in 8 bits).
 template <typename P, typename G, bool kMaster, bool kEight>
-__global__ void __launch_bounds__(kAdamThreads, kEight ? 4 : 5) adamw_multi_kernel(const __grid_constant__ AdamList list, const AdamScalars s,
+__global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 5) adamw_multi_kernel(const __grid_constant__ AdamList list, const AdamScalars s,
                                                                                    const AdamShared* __restrict__ shared) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
   grid_wait();
@@ -310,21 +329,27 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 4 : 5) adamw_multi_kern
     const AdamTensor& t = list.t[i];
     const long n = t.n;
     const uint32_t key = kEight ? mix32(shared->key + uint32_t(list.base + i) * 0x85ebca77u) : 0u;
-    const auto block = [&](long e0, auto whole) {
-      const bool vec = whole;
-      float g[8], w[8], m[8], v[8];
-      load8(static_cast<const G*>(t.grad), e0, lane, n, vec, g);
-      if (kMaster) load8(static_cast<const float*>(t.master), e0, lane, n, vec, w);
-      else load8(static_cast<const P*>(t.param), e0, lane, n, vec, w);
-      if (kEight) {
-        const long at = e0 / kStateBlock;
+    const bool aligned = list.aligned[i];
+    const auto start_of = [&](int c) { return long(c - list.first_chunk[i]) * kChunk + warp * kStateBlock; };
+    if constexpr (kEight) {
+      Block8<G> next;
+      const auto fetch = [&](Block8<G>& b, long e0, bool vec) {
+        load8(static_cast<const G*>(t.grad), e0, lane, n, vec, b.grad);
+        if (kMaster) load8(static_cast<const float*>(t.master), e0, lane, n, vec, b.w);
+        else load8(static_cast<const P*>(t.param), e0, lane, n, vec, b.w);
+        b.m = load_codes8(static_cast<const uint8_t*>(t.m), e0, lane, n, vec);
+        b.v = load_codes8(static_cast<const uint8_t*>(t.v), e0, lane, n, vec);
+        b.m_byte = t.m_scale[e0 / kStateBlock];
+        b.v_byte = t.v_scale[e0 / kStateBlock];
+      };
+      const auto update = [&](const Block8<G>& b, long e0, bool vec) {
+        float w[8], m[8], v[8], root[8], g[8];
         // the scales are powers of two: they go into the factors the codes are multiplied with anyway
-        load_codes8(static_cast<const uint8_t*>(t.m), e0, lane, n, vec, m);
-        load_codes8(static_cast<const uint8_t*>(t.v), e0, lane, n, vec, v);
-        const float m_scale = scale_value(t.m_scale[at]), v_scale = scale_value(t.v_scale[at]);
-        const float keep_m = s.beta1 * m_scale, keep_v = s.beta2 * v_scale * v_scale;
+        const float keep_m = s.beta1 * scale_value(b.m_byte), v_scale = scale_value(b.v_byte), keep_v = s.beta2 * v_scale * v_scale;
+        widen(b.grad, g);
+        widen_codes(b.m, m);
+        widen_codes(b.v, v);
         uint32_t random[8];
-        float root[8];
         float m_max = 0.f, v_max = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -339,7 +364,7 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 4 : 5) adamw_multi_kern
             v_max = max3_abs(v_max, v[j - 1], v[j]);
           }
           root[j] = root_of(v[j]);
-          w[j] -= s.lr * (m[j] * bc1 * inverse_approx(root[j] * root_bc2 + s.eps) + s.wd * w[j]);
+          w[j] = b.w[j] - s.lr * (m[j] * bc1 * inverse_approx(root[j] * root_bc2 + s.eps) + s.wd * b.w[j]);
           random[j] = mix32_open(uint32_t(e0 + (vec ? lane * 8 + j : j * 32 + lane)) * 0x9e3779b1u + key);
         }
         if (kMaster) put8(t.master, e0, lane, n, vec, w);
@@ -350,10 +375,33 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 4 : 5) adamw_multi_kern
         store_codes8(static_cast<uint8_t*>(t.m), e0, lane, n, vec, encode8<false>(m_max, m, random, m_byte));
         store_codes8(static_cast<uint8_t*>(t.v), e0, lane, n, vec, encode8<true>(v_max, root, random, v_byte));
         if (lane == 0) {
-          t.m_scale[at] = uint8_t(m_byte);
-          t.v_scale[at] = uint8_t(v_byte);
+          t.m_scale[e0 / kStateBlock] = uint8_t(m_byte);
+          t.v_scale[e0 / kStateBlock] = uint8_t(v_byte);
         }
-      } else {
+      };
+      // whole blocks, the next one's loads under way while this one is worked on; then the tensor's end, or all of it where
+      // it is not aligned
+      const auto whole = [&](int c) { return aligned && c < list.first_chunk[i + 1] && start_of(c) + kStateBlock <= n; };
+      if (whole(chunk)) fetch(next, start_of(chunk), true);
+      for (; whole(chunk); chunk += gridDim.x) {
+        const Block8<G> now = next;
+        if (whole(chunk + gridDim.x)) fetch(next, start_of(chunk + gridDim.x), true);
+        update(now, start_of(chunk), true);
+      }
+      for (; chunk < list.first_chunk[i + 1]; chunk += gridDim.x)
+        if (start_of(chunk) < n) {
+          fetch(next, start_of(chunk), false);
+          update(next, start_of(chunk), false);
+        }
+    } else {
+      for (; chunk < list.first_chunk[i + 1]; chunk += gridDim.x) {
+        const long e0 = start_of(chunk);
+        if (e0 >= n) continue;
+        const bool vec = aligned && e0 + kStateBlock <= n;
+        float g[8], w[8], m[8], v[8];
+        load8(static_cast<const G*>(t.grad), e0, lane, n, vec, g);
+        if (kMaster) load8(static_cast<const float*>(t.master), e0, lane, n, vec, w);
+        else load8(static_cast<const P*>(t.param), e0, lane, n, vec, w);
         load8(static_cast<const float*>(t.m), e0, lane, n, vec, m);
         load8(static_cast<const float*>(t.v), e0, lane, n, vec, v);
 #pragma unroll
@@ -367,18 +415,6 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 4 : 5) adamw_multi_kern
         put8(static_cast<P*>(t.param), e0, lane, n, vec, w);
         put8(static_cast<float*>(t.m), e0, lane, n, vec, m);
         put8(static_cast<float*>(t.v), e0, lane, n, vec, v);
-      }
-    };
-    const bool aligned = list.aligned[i];
-    for (; chunk < list.first_chunk[i + 1]; chunk += gridDim.x) {
-      const long e0 = long(chunk - list.first_chunk[i]) * kChunk + warp * kStateBlock;
-      if (e0 >= n) continue;
-      const bool vec = aligned && e0 + kStateBlock <= n;
-      if constexpr (kEight) {   // a body for either: the tests inside one take more than the loads
-        if (vec) block(e0, std::true_type());
-        else block(e0, std::false_type());
-      } else {
-        block(e0, vec);
       }
     }
   }
@@ -462,7 +498,7 @@ extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* 
       return by_type(grad_type, [&](auto* g) {
         using G = std::remove_pointer_t<decltype(g)>;
         const auto launch = [&](auto kernel) {
-          return launch_overlapped(kernel, dim3(std::min(chunks, 148 * 8)), kAdamThreads, 0, s, 1, true, list, scalars, static_cast<const AdamShared*>(shared));
+          return launch_overlapped(kernel, dim3(std::min(chunks, 148 * (eight ? 3 : 8))), kAdamThreads, 0, s, 1, true, list, scalars, static_cast<const AdamShared*>(shared));
         };
         if constexpr (std::is_same_v<P, float>) {
           if (!has_master) return eight ? launch(adamw_multi_kernel<P, G, false, true>) : launch(adamw_multi_kernel<P, G, false, false>);
