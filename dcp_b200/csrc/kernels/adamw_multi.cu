@@ -47,7 +47,7 @@ struct AdamList {
 };
 struct AdamScalars { float lr, beta1, rest1, beta2, rest2, eps, wd; };   // rest: 1 - beta
 // what a step's kernels hand on, in global memory
-struct AdamShared { float coef, bc1, root_bc2; uint32_t key; };
+struct AdamShared { float coef, bc1, root_bc2; uint32_t key; int skip; };
 
 // finaliser of MurmurHash3 (A. Appleby, public domain), and without its last step
 __device__ __forceinline__ uint32_t mix32_open(uint32_t x) {
@@ -279,8 +279,9 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
 
 // step counter, bias corrections, clipping coefficient: one CTA
 __global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __restrict__ parts, int n_parts, int64_t* __restrict__ step, double beta1,
-                                                            double beta2, float grad_scale, float clip, uint32_t seed, float* __restrict__ norm,
-                                                            AdamShared* __restrict__ shared) {
+                                                            double beta2, float grad_scale, float clip, const float* __restrict__ factor,
+                                                            uint32_t seed, float* __restrict__ norm, const int* __restrict__ status_a,
+                                                            const int* __restrict__ status_b, AdamShared* __restrict__ shared) {
   __shared__ double sums[8];
   grid_wait();
   grid_let_next();
@@ -293,9 +294,11 @@ __global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __rest
   if (threadIdx.x) return;
 #pragma unroll
   for (int w = 1; w < 8; ++w) t += sums[w];
+  const bool skip = (status_a && *status_a != 0) || (status_b && *status_b != 0);
   const int64_t now = *step + 1;
-  *step = now;
-  float coef = grad_scale;
+  if (!skip) *step = now;
+  shared->skip = skip;
+  float coef = factor ? grad_scale * *factor : grad_scale;
   if (n_parts > 0) {
     const double length = sqrt(t);
     *norm = float(length);
@@ -323,6 +326,7 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 5) adamw_multi_kern
                                                                                    const AdamShared* __restrict__ shared) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
   grid_wait();
+  if (shared->skip) return;
   const float coef = shared->coef, bc1 = shared->bc1, root_bc2 = shared->root_bc2;
   int chunk = blockIdx.x;
   for (int i = find_tensor(list, chunk); chunk < n_chunks; ++i) {
@@ -424,23 +428,26 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 5) adamw_multi_kern
 
 using namespace dcpk;
 
+static constexpr int kAdamHead = 4;   // doubles
 static int adam_norm_ctas(int chunks) { return std::min(chunks, 148 * 4); }
 
 // doubles of `work` a call needs: what the kernels hand on, and a sum per CTA of each launch of the norm
-extern "C" long dcpk_adamw_multi_work(int n_tensors) { return 2 + long((n_tensors + kAdamTensors - 1) / kAdamTensors) * 148 * 4; }
+extern "C" long dcpk_adamw_multi_work(int n_tensors) { return kAdamHead + long((n_tensors + kAdamTensors - 1) / kAdamTensors) * 148 * 4; }
 
 // Tensors of one parameter type and one gradient type (0 fp32, 1 fp16, 2 bf16); an entry of `masters` may be null for fp32
 // parameters only.  m_scales null: moments in fp32; otherwise codes with ceil(n / 256) scales.  step: one int64 on the
-// device, counted up.  clip <= 0: none, and norm is not written.
+// device, counted up.  clip <= 0: none, and norm is not written.  factor: null, or one float on the device that the gradients
+// are multiplied with.  status_a, status_b: null, or words that, when one is not zero, leave everything as it is.
 extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* const* grads, void* const* masters, void* const* ms,
                                 void* const* vs, void* const* m_scales, void* const* v_scales, const long* sizes, int param_type, int grad_type,
                                 int64_t* step, float lr, double beta1, double beta2, float eps, float wd, float grad_scale, float clip,
-                                unsigned seed, float* norm, double* work, void* stream) {
+                                const float* factor, unsigned seed, float* norm, const int* status_a, const int* status_b, double* work,
+                                void* stream) {
   if (n_tensors < 0 || param_type < 0 || param_type > 2 || grad_type < 0 || grad_type > 2) return -3;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   AdamShared* shared = reinterpret_cast<AdamShared*>(work);
-  double* parts = work + 2;
-  static_assert(sizeof(AdamShared) <= 16, "work begins with it");
+  double* parts = work + kAdamHead;
+  static_assert(sizeof(AdamShared) <= kAdamHead * 8, "work begins with it");
   const bool eight = m_scales != nullptr, has_master = masters != nullptr;
   if (!has_master && param_type != kTypeF32) return -3;
   for (int i = 0; i < n_tensors; ++i)
@@ -486,7 +493,7 @@ extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* 
     }
   if (clip > 0.f && n_parts == 0 && cudaMemsetAsync(norm, 0, 4, s) != cudaSuccess) return -5;
   if (launch_overlapped(adamw_prepare_kernel, dim3(1), 256, 0, s, 1, !first, static_cast<const double*>(parts), n_parts, step, beta1, beta2,
-                        grad_scale, clip, uint32_t(seed), norm, shared) != cudaSuccess || cudaGetLastError() != cudaSuccess)
+                        grad_scale, clip, factor, uint32_t(seed), norm, status_a, status_b, shared) != cudaSuccess || cudaGetLastError() != cudaSuccess)
     return -5;
   const AdamScalars scalars = {lr, float(beta1), float(1.0 - beta1), float(beta2), float(1.0 - beta2), eps, wd};
   for (int base = 0; base < n_tensors;) {

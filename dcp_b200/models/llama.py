@@ -25,7 +25,7 @@ import torch
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
-from ..ops import model_ops
+from ..ops import fp8_ops, model_ops
 
 
 @dataclass
@@ -228,6 +228,120 @@ class _DecoderLayerFn(torch.autograd.Function):
         return dx, None, None, None, None, None
 
 
+class _DecoderLayerFp8Fn(torch.autograd.Function):
+    """``_DecoderLayerFn`` with its four matrices' products in 8 bits (``ops.fp8_ops``), forward and backward: activations
+    and gradients with a scale per 1 x 128 along the contraction, weights per 128 x 128.  The norms write 8-bit results
+    themselves, the one before the MLP with the residual's addition; everything between the products stays in bf16, as do
+    the saved tensors and their levels."""
+
+    @staticmethod
+    def _qkv(x, model, l):
+        h1, _, rstd1 = fp8_ops.rmsnorm_quant(x, model.p[f"l{l}.norm1"], model.cfg.eps)
+        return fp8_ops.matmul(h1, model.weight8(f"l{l}.wqkv")), rstd1
+
+    @staticmethod
+    def _mid(x, a, model, l):
+        """(norm of the residual stream after attention in 8 bits, that stream, its rstd)"""
+        o = model.tp_sum(fp8_ops.matmul(fp8_ops.quantize(a), model.weight8(f"l{l}.wo")))
+        return fp8_ops.rmsnorm_quant(o, model.p[f"l{l}.norm2"], model.cfg.eps, x)
+
+    @staticmethod
+    def forward(ctx, x, model, l, cos, sin, level):
+        fn, cfg, ex = _DecoderLayerFp8Fn, model.cfg, model.executor
+        T = x.shape[0]
+        qkv, rstd1 = fn._qkv(x, model, l)
+        model_ops.qkv_rope_split(qkv, cos, sin, ex.q, ex.kv, cfg.n_heads, cfg.n_kv_heads)
+        ex.inputs_written()
+        if ex.world == 1:
+            out, lse_c = ex.forward(None, None, *ex.new_results())
+            a = out.view(T, -1)
+        else:
+            out, lse = ex.forward()
+            a = out.reshape(T, -1).clone()
+            lse_c = lse.clone()
+        h2, x_mid, rstd2 = fn._mid(x, a, model, l)
+        gu = fp8_ops.matmul(h2, model.weight8(f"l{l}.wgu"))
+        act, wd = fp8_ops.quantize(model_ops.swiglu_fwd_raw(gu)), model.weight8(f"l{l}.wd")
+        if model.tp_group is None:
+            y = fp8_ops.matmul(act, wd, add=x_mid)
+        else:
+            y = model.tp_sum(fp8_ops.matmul(act, wd)).add_(x_mid)
+        ctx.model, ctx.l, ctx.level, ctx.epoch = model, l, level, ex.arena_epoch
+        keep = [x, cos, sin, a, lse_c, rstd1]
+        if level >= 1:
+            keep += [qkv, x_mid, rstd2]
+        if level >= 2:
+            keep.append(gu)
+        ctx.save_for_backward(*keep)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        fn, model, l, level = _DecoderLayerFp8Fn, ctx.model, ctx.l, ctx.level
+        p, cfg, ex = model.p, model.cfg, model.executor
+        saved = ctx.saved_tensors
+        x, cos, sin, a, lse_c, rstd1 = saved[:6]
+        T = x.shape[0]
+        dy = dy.contiguous()
+        w1, w2 = p[f"l{l}.norm1"], p[f"l{l}.norm2"]
+        by_tokens = lambda t: fp8_ops.quantize(t, (fp8_ops.BLOCK, 1))  # noqa: E731
+
+        def products(name, d, rhs):
+            """Weight gradient of a matrix and the gradient of its input, from the gradient of its output and its input."""
+            rows, cols = fp8_ops.quantize_both(d)
+            grad = p[f"l{l}.{name}"].grad
+            fp8_ops.matmul(cols, by_tokens(rhs), trans_a=True, trans_b=False, out=grad, add=grad if model.accumulate_grads else None)
+            return fp8_ops.matmul(rows, model.weight8(f"l{l}.{name}"), trans_b=False)
+
+        def ngrad(param, dw):
+            if model.accumulate_grads:
+                param.grad.add_(dw.to(param.grad.dtype))
+            else:
+                param.grad.copy_(dw)
+
+        h2 = None
+        if level >= 1:
+            qkv, x_mid, rstd2 = saved[6:9]
+        else:
+            qkv, _ = fn._qkv(x, model, l)
+            h2, x_mid, rstd2 = fn._mid(x, a, model, l)
+        # ---- MLP
+        if level >= 2:
+            gu = saved[9]
+        else:
+            if h2 is None:
+                h2 = fp8_ops.rmsnorm_quant(x_mid, w2, cfg.eps)[0]
+            gu = fp8_ops.matmul(h2, model.weight8(f"l{l}.wgu"))
+        del h2
+        dact = products("wd", dy, model_ops.swiglu_fwd_raw(gu))
+        dgu = model_ops.swiglu_bwd_raw(gu, dact)
+        del dact, gu
+        dh2 = model.tp_sum(products("wgu", dgu, model_ops.rmsnorm_fwd_raw(x_mid, w2, cfg.eps)[0]))
+        del dgu
+        dx_mid, dw2 = fp8_ops.rmsnorm_quant_bwd(x_mid, w2, rstd2, dh2, dy)
+        del dh2
+        ngrad(w2, dw2)
+        # ---- attention
+        da = products("wo", dx_mid, a)
+        if ex.arena_epoch != ctx.epoch:
+            model_ops.qkv_rope_split(qkv, cos, sin, ex.q, ex.kv, cfg.n_heads, cfg.n_kv_heads)
+            ex.inputs_written()
+            if ex.world > 1:
+                ex.out_local().copy_(a.view(-1, cfg.n_heads, cfg.head_dim))
+                ex.lse_local().copy_(lse_c)
+        heads = lambda t: t.view(-1, cfg.n_heads, cfg.head_dim)  # noqa: E731
+        dq, dkv = ex.backward(heads(da), None, None, heads(a), lse_c) if ex.world == 1 else ex.backward(heads(da))
+        del da, qkv
+        dqkv = model_ops.qkv_rope_pack_bwd(dq, dkv, cos, sin, T, cfg.n_heads, cfg.n_kv_heads)
+        dh1 = model.tp_sum(products("wqkv", dqkv, model_ops.rmsnorm_fwd_raw(x, w1, cfg.eps)[0]))
+        del dqkv
+        dx, dw1 = fp8_ops.rmsnorm_quant_bwd(x, w1, rstd1, dh1, dx_mid)
+        ngrad(w1, dw1)
+        if model.grad_ready_hook is not None and not model.accumulate_grads:
+            model.grad_ready_hook(model.layer_bucket(l))
+        return dx, None, None, None, None, None
+
+
 def _direct_grad(weight: torch.Tensor) -> bool:
     """May a backward add to ``weight.grad`` itself?  Only a gradient buffer that is there when the backward runs, of a
     form the kernels write, and of a weight that no hook waits for; anything else goes through autograd."""
@@ -300,8 +414,11 @@ class LlamaModel:
 
     def __init__(self, cfg: LlamaConfig, device: torch.device, params_flat: Optional[torch.Tensor] = None,
                  grads_flat: Optional[torch.Tensor] = None, seed: int = 0, recompute: bool = True,
-                 lm_head_chunk: int = 4096, tp_group=None, tp_rank: int = 0, tp_size: int = 1):
+                 lm_head_chunk: int = 4096, tp_group=None, tp_rank: int = 0, tp_size: int = 1, fp8: bool = False):
+        """``fp8``: the products of the decoder layers' matrices run in 8 bits (``ops.fp8_ops``)."""
         self.cfg, self.device = cfg, device
+        self.fp8 = fp8
+        self._weights8: Dict[str, fp8_ops.BlockScaled] = {}
         self.set_tensor_parallel(tp_group, tp_rank, tp_size)
         self.n_replicated = 0
         self.recompute = recompute
@@ -454,9 +571,22 @@ class LlamaModel:
     def set_executor(self, executor) -> None:
         self.executor = executor
 
+    def weight8(self, name: str) -> fp8_ops.BlockScaled:
+        """8-bit codes of a decoder layer's matrix, made at its first use after ``loss`` was called and kept until the next
+        ``loss``: the forward pass, a recomputation and the backward pass share them."""
+        if name not in self._weights8:
+            self._weights8[name] = fp8_ops.quantize(self.p[name].detach(), (fp8_ops.BLOCK, fp8_ops.BLOCK))
+        return self._weights8[name]
+
     # ---- forward
     def _layer(self, x, l: int, cos, sin):
         p, cfg = self.p, self.cfg
+        if self.fp8:
+            assert self.tp_group is None, "tensor parallelism needs the hand-written layer backward (CUDA)"
+            qkv, _ = fp8_ops.norm_linear(x, p[f"l{l}.norm1"], p[f"l{l}.wqkv"], cfg.eps)
+            a = _AttentionFn.apply(qkv, self, cos, sin, l)
+            gu, x = fp8_ops.norm_linear(fp8_ops.linear(a, p[f"l{l}.wo"]), p[f"l{l}.norm2"], p[f"l{l}.wgu"], cfg.eps, x)
+            return x + fp8_ops.linear(model_ops.swiglu(gu), p[f"l{l}.wd"])
         h = model_ops.rmsnorm(x, p[f"l{l}.norm1"], cfg.eps)
         qkv = F.linear(h, p[f"l{l}.wqkv"])
         a = _AttentionFn.apply(qkv, self, cos, sin, l)
@@ -477,6 +607,7 @@ class LlamaModel:
         missing ``.grad`` and one that was replaced in between are respected either way."""
         cfg = self.cfg
         self._attn_stash.clear()
+        self._weights8.clear()
         self._stash_enabled = self.cache_attention and self.recompute and torch.is_grad_enabled()
         cos, sin = model_ops.rope_tables(positions, cfg.rope_theta, cfg.head_dim)
         embed = self.p["embed"]
@@ -485,7 +616,8 @@ class LlamaModel:
         x = _EmbeddingFn.apply(tokens, embed) if write_grads else F.embedding(tokens, embed)
         for l in range(cfg.n_layers):
             if manual:
-                x = _DecoderLayerFn.apply(x, self, l, cos, sin, self.layer_levels[l])
+                layer = _DecoderLayerFp8Fn if self.fp8 else _DecoderLayerFn
+                x = layer.apply(x, self, l, cos, sin, self.layer_levels[l])
             elif self.recompute and torch.is_grad_enabled():
                 x = checkpoint(self._layer, x, l, cos, sin, use_reentrant=False)
             else:

@@ -312,3 +312,74 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
             _c_long(0 if add is None else _pitch(add)), _c_int(_TYPES[out_dtype]), _c_int(form), _lib.ptr(_status(out.device)),
             _lib.stream_handle()), "fp8_gemm")
     return out
+
+
+# --------------------------------------------------------------------------- autograd
+def _grad_products(dy: torch.Tensor, x: torch.Tensor, wq: BlockScaled, need_x: bool, need_w: bool):
+    """(dx, dw) of y = x w^T in 8 bits, in the types of dy."""
+    if need_x and need_w:
+        by_rows, by_cols = quantize_both(dy)
+    else:
+        by_rows, by_cols = (quantize(dy) if need_x else None), (quantize(dy, (BLOCK, 1)) if need_w else None)
+    dx = matmul(by_rows, wq, trans_b=False, out_dtype=dy.dtype) if need_x else None
+    dw = matmul(by_cols, quantize(x, (BLOCK, 1)), trans_a=True, trans_b=False, out_dtype=dy.dtype) if need_w else None
+    return dx, dw
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight):
+        x2 = x.reshape(-1, x.shape[-1])
+        wq = quantize(weight, (BLOCK, BLOCK))
+        ctx.save_for_backward(x2, wq.codes, wq.scales)
+        return matmul(quantize(x2), wq, out_dtype=x.dtype).view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, codes, scales = ctx.saved_tensors
+        dx, dw = _grad_products(dy.reshape(-1, dy.shape[-1]), x2, BlockScaled(codes, scales, (BLOCK, BLOCK)), *ctx.needs_input_grad)
+        return None if dx is None else dx.view(*dy.shape[:-1], x2.shape[1]), dw
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """x weight^T with all three products (result, input gradient, weight gradient) in 8 bits; x [..., K], weight [N, K] of one
+    type."""
+    _need(x.dtype == weight.dtype and weight.dim() == 2 and x.shape[-1] == weight.shape[1], "x [..., K] and weight [N, K] of one type")
+    return _Linear.apply(x, weight)
+
+
+class _NormLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, norm_weight, weight, eps, residual):
+        x2 = x.reshape(-1, x.shape[-1])
+        y, h, rstd = rmsnorm_quant(x2, norm_weight, eps, None if residual is None else residual.reshape(x2.shape))
+        wq = quantize(weight, (BLOCK, BLOCK))
+        ctx.save_for_backward(h, norm_weight, rstd, wq.codes, wq.scales)
+        ctx.with_residual = residual is not None
+        ctx.set_materialize_grads(False)
+        out = matmul(y, wq, out_dtype=x.dtype).view(*x.shape[:-1], weight.shape[0])
+        return out, (h.view(x.shape) if residual is not None else x.view(x.shape))
+
+    @staticmethod
+    def backward(ctx, dout, dh):
+        if dout is None:   # only h was used
+            return dh, None, None, None, dh if ctx.with_residual else None
+        h, norm_weight, rstd, codes, scales = ctx.saved_tensors
+        d2 = dout.reshape(-1, dout.shape[-1])
+        need_w = ctx.needs_input_grad[2]
+        # the weight gradient needs the norm's result by tokens: made again, in h's type
+        y = (h.float() * rstd[:, None] * norm_weight.float()).to(h.dtype) if need_w else None
+        dy, dw = _grad_products(d2, y, BlockScaled(codes, scales, (BLOCK, BLOCK)), True, need_w)
+        dx, dnorm = rmsnorm_quant_bwd(h, norm_weight, rstd, dy, None if dh is None else dh.reshape(h.shape).contiguous())
+        dx = dx.view(dout.shape[:-1] + h.shape[1:])
+        return dx, dnorm.to(norm_weight.dtype), dw, None, dx if ctx.with_residual else None
+
+
+def norm_linear(x: torch.Tensor, norm_weight: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
+                residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(rmsnorm(h) norm_weight weight^T, h) with h = x + residual, all products in 8 bits; the gradient of h from elsewhere is
+    added in the norm's backward pass.  All tensors of one type."""
+    _need(x.dtype == weight.dtype == norm_weight.dtype and weight.dim() == 2 and x.shape[-1] == weight.shape[1],
+          "x [..., K], norm_weight [K] and weight [N, K] of one type")
+    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "the residual has to be like x")
+    return _NormLinear.apply(x, norm_weight, weight, eps, residual)

@@ -70,6 +70,8 @@ def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta
         coef = grad_scale * (clip / (norm + 1e-6)).float().clamp(max=1.0)
         norm = norm.float()
     key = _mix32((seed + int(step) * 0x9E3779B1) & 0xFFFFFFFF)
+    flat = lambda ts: None if ts is None else [t.view(-1) for t in ts]  # noqa: E731
+    params, grads, masters, m, v = flat(params), flat(grads), flat(masters), flat(m), flat(v)
     for i, g in enumerate(grads):
         w = params[i] if masters is None else masters[i]
         g = g.float() * coef
@@ -122,7 +124,7 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
                 m: Sequence[torch.Tensor], v: Sequence[torch.Tensor], step: torch.Tensor, *, lr: float, beta1: float, beta2: float,
                 eps: float, weight_decay: float, grad_scale: float = 1.0, clip: Optional[float] = None,
                 m_scales: Optional[Sequence[torch.Tensor]] = None, v_scales: Optional[Sequence[torch.Tensor]] = None,
-                seed: int = 0) -> Optional[torch.Tensor]:
+                seed: int = 0, factor: Optional[torch.Tensor] = None, status: Sequence[torch.Tensor] = ()) -> Optional[torch.Tensor]:
     """One AdamW step over lists of contiguous tensors, in place; returns the norm of the scaled gradients (fp32, one element)
     where ``clip`` limits it, else None.
 
@@ -133,9 +135,15 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
     other numbers are the call's.  A gradient that is not finite makes its own element NaN, and with ``clip`` all."""
     _check_lists(params, grads, masters, m, v, step, m_scales, v_scales)
     _need(clip is None or clip > 0, "clip has to be positive")
+    _need(factor is None or (factor.dtype == torch.float32 and factor.numel() == 1 and factor.device == step.device),
+          "factor has to be one float32 on the parameters' device")
+    _need(len(status) <= 2 and all(s.dtype == torch.int32 and s.device == step.device for s in status), "status: up to two int32 words")
     if not params[0].is_cuda:
+        if any(int(s.reshape(-1)[0]) for s in status):
+            return None if clip is None else torch.zeros(1)
         return adamw_multi_reference(params, grads, masters, m, v, step, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
-                                     weight_decay=weight_decay, grad_scale=grad_scale, clip=clip, m_scales=m_scales, v_scales=v_scales, seed=seed)
+                                     weight_decay=weight_decay, grad_scale=grad_scale if factor is None else grad_scale * float(factor),
+                                     clip=clip, m_scales=m_scales, v_scales=v_scales, seed=seed)
     n, lib = len(params), _lib.load()
     lib.dcpk_adamw_multi_work.restype = ctypes.c_long
     f, d = ctypes.c_float, ctypes.c_double
@@ -146,6 +154,63 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
         _lib.check(lib.dcpk_adamw_multi(
             ctypes.c_int(n), _pointers(params), _pointers(grads), _pointers(masters), _pointers(m), _pointers(v), _pointers(m_scales),
             _pointers(v_scales), sizes, ctypes.c_int(_TYPES[params[0].dtype]), ctypes.c_int(_TYPES[grads[0].dtype]), _lib.ptr(step), f(lr),
-            d(beta1), d(beta2), f(eps), f(weight_decay), f(grad_scale), f(clip or 0.0), ctypes.c_uint(seed & 0xFFFFFFFF),
-            None if norm is None else _lib.ptr(norm), _lib.ptr(work), _lib.stream_handle()), "adamw_multi")
+            d(beta1), d(beta2), f(eps), f(weight_decay), f(grad_scale), f(clip or 0.0), None if factor is None else _lib.ptr(factor),
+            ctypes.c_uint(seed & 0xFFFFFFFF), None if norm is None else _lib.ptr(norm), *[_lib.ptr(s) for s in status], *[None] * (2 - len(status)),
+            _lib.ptr(work), _lib.stream_handle()), "adamw_multi")
     return norm
+
+
+class MultiTensorAdamW:
+    """AdamW over a list of parameters with ``adamw_multi``: fp32 masters (for 16-bit parameters), moments in 32 or 8 bits.
+
+    ``step()`` takes the parameters' ``.grad`` (all of them set, contiguous, of one type).  State of the whole list lies in
+    flat tensors: ``master``, ``m``, ``v`` (in 8 bits: codes of m and of sqrt(v), with ``m_scale`` and ``v_scale``); each
+    parameter's part begins at a multiple of 256 values."""
+
+    def __init__(self, params: Sequence[torch.Tensor], lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8, weight_decay: float = 0.1,
+                 clip_grad: Optional[float] = None, state_bits: int = 32, seed: int = 0):
+        self.params: List[torch.Tensor] = list(params)
+        _need(len(self.params) > 0, "no parameters")
+        _need(state_bits in (8, 32), "moments are kept in 8 or 32 bits")
+        self.lr, self.betas, self.eps, self.wd, self.clip, self.bits, self.seed = lr, betas, eps, weight_decay, clip_grad, state_bits, seed
+        p0 = self.params[0]
+        starts, at = [], 0
+        for p in self.params:
+            starts.append(at)
+            at += state_scales(p.numel()) * STATE_BLOCK
+        flat = lambda dtype, per=1: torch.zeros(at // per, dtype=dtype, device=p0.device)  # noqa: E731
+        cut = lambda t, per=1: [t[s // per:-(-(s + p.numel()) // per)] for s, p in zip(starts, self.params)]  # noqa: E731
+        self.master = flat(torch.float32) if p0.dtype != torch.float32 else None
+        self._masters = None if self.master is None else cut(self.master)
+        if self._masters is not None:
+            for w, p in zip(self._masters, self.params):
+                w.copy_(p.detach().reshape(-1))
+        state = torch.float32 if state_bits == 32 else torch.uint8
+        self.m, self.v = (flat(state) if state_bits == 32 else flat(state).view(E4M3) for _ in range(2))
+        self.m_scale, self.v_scale = (None, None) if state_bits == 32 else (flat(torch.uint8, STATE_BLOCK).view(E8M0) for _ in range(2))
+        self._m, self._v = cut(self.m), cut(self.v)
+        self._m_scales, self._v_scales = (None, None) if state_bits == 32 else (cut(self.m_scale, STATE_BLOCK), cut(self.v_scale, STATE_BLOCK))
+        self.step_count = torch.zeros(1, dtype=torch.int64, device=p0.device)
+
+    @torch.no_grad()
+    def step(self, grad_scale: float = 1.0) -> Optional[torch.Tensor]:
+        """One update; returns the norm of the scaled gradients where it is clipped."""
+        grads = [p.grad for p in self.params]
+        _need(all(g is not None for g in grads), "a parameter has no gradient")
+        return adamw_multi([p.detach() for p in self.params], grads, self._masters, self._m, self._v, self.step_count, lr=self.lr,
+                           beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, weight_decay=self.wd, grad_scale=grad_scale,
+                           clip=self.clip, m_scales=self._m_scales, v_scales=self._v_scales, seed=self.seed)
+
+    def state_dict(self) -> dict:
+        keep = ("master", "m", "v", "m_scale", "v_scale", "step_count")
+        return {"bits": self.bits, "sizes": [p.numel() for p in self.params], **{k: getattr(self, k) for k in keep}}
+
+    def load_state_dict(self, sd: dict) -> None:
+        _need(sd["bits"] == self.bits and list(sd["sizes"]) == [p.numel() for p in self.params], "state of other parameters or another width")
+        for k in ("master", "m", "v", "m_scale", "v_scale", "step_count"):
+            mine = getattr(self, k)
+            if mine is not None:
+                mine.copy_(sd[k]) if mine.dtype != E8M0 else mine.view(torch.uint8).copy_(sd[k].view(torch.uint8))
+        if self._masters is not None:
+            for w, p in zip(self._masters, self.params):
+                p.detach().copy_(w.view(p.shape))

@@ -32,7 +32,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from ..ops import _lib
+from ..ops import _lib, optim_ops
 from ..ops.attention import _ptr_array
 from ..runtime.symm import SymmetricArena
 
@@ -115,7 +115,7 @@ class ShardedAdamW:
     def __init__(self, bufs: FlatBuffers, lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8,
                  weight_decay: float = 0.1, clip_grad: Optional[float] = 1.0, group=None, tp_group=None,
                  n_replicated: int = 0, buckets: Optional[Sequence[Tuple[int, int]]] = None,
-                 extra_status: Optional[torch.Tensor] = None, overlap_ctas: int = 24):
+                 extra_status: Optional[torch.Tensor] = None, overlap_ctas: int = 24, state_bits: int = 32, seed: int = 0):
         """``group`` = the ranks that hold the same parameters (they share the sharded state and
         their gradients are summed).  With tensor parallelism ``tp_group`` links the ranks that hold
         different shards of one model replica and ``n_replicated`` is the length of the leading
@@ -123,7 +123,11 @@ class ShardedAdamW:
         that part once and the sharded part once per tensor-parallel rank (a bucket lies entirely
         in one of the two parts).  ``buckets``: (offset, length) ranges covering the flat buffer
         (default: one bucket).  ``extra_status``: status word of another arena (the attention
-        executor's) that, when nonzero, also makes the update kernels leave the weights alone."""
+        executor's) that, when nonzero, also makes the update kernels leave the weights alone.
+        ``state_bits``: 8 keeps m and sqrt(v) as 8-bit codes with a scale per 256 values (2 instead of 8 bytes per
+        parameter), rounded stochastically by a hash of ``seed``, step, slice and element (``ops.optim_ops``)."""
+        if state_bits not in (8, 32):
+            raise ValueError("moments are kept in 8 or 32 bits")
         self.bufs, self.group = bufs, group
         self.tp_group, self.n_replicated = tp_group, n_replicated
         self.lr, self.betas, self.eps, self.wd, self.clip = lr, betas, eps, weight_decay, clip_grad
@@ -137,8 +141,19 @@ class ShardedAdamW:
         self.master = torch.empty(n_state, dtype=torch.float32, device=dev)
         for s in self.shards:
             self.master[s.state_off:s.state_off + s.length].copy_(bufs.params[s.flat_off:s.flat_off + s.length])
-        self.m = torch.zeros_like(self.master)
-        self.v = torch.zeros_like(self.master)
+        self.state_bits, self.seed = state_bits, seed
+        if state_bits == 32:
+            self.m = torch.zeros_like(self.master)
+            self.v = torch.zeros_like(self.master)
+        else:
+            # a slice's scales follow those of the slices before it; codes and scales of zero are zeros
+            self.scale_offs = [0]
+            for s in self.shards:
+                self.scale_offs.append(self.scale_offs[-1] + optim_ops.state_scales(s.length))
+            zeros = lambda n, dtype: torch.zeros(n, dtype=torch.uint8, device=dev).view(dtype)  # noqa: E731
+            self.m, self.v = (zeros(n_state, torch.float8_e4m3fn) for _ in range(2))
+            self.m_scale, self.v_scale = (zeros(self.scale_offs[-1], torch.float8_e8m0fnu) for _ in range(2))
+            self.step_tensor = torch.zeros(1, dtype=torch.int64, device=dev)
         # fp32 main gradients exist only when there is a reduction to overlap
         self.overlap = world > 1
         self.main_grad = torch.zeros(n_state, dtype=torch.float32, device=dev) if self.overlap else None
@@ -157,14 +172,56 @@ class ShardedAdamW:
 
     # ---- checkpoint state
     def state_dict(self) -> dict:
-        return {"master": self.master, "m": self.m, "v": self.v, "step": self.step_count,
+        """m and v in 32 bits whatever they are kept in (from 8 bits: in host memory), so that a checkpoint can be loaded
+        with either width and cut for another number of ranks; 8-bit state comes back from it value for value, as long as
+        the slices stay the same."""
+        if self.state_bits == 32:
+            m, v = self.m, self.v
+        else:
+            m, v = (torch.empty(self.master.numel(), dtype=torch.float32) for _ in range(2))
+            for s, part in self._state_parts():
+                m[part] = optim_ops.decode_state(self.m[part], self._scales(self.m_scale, s)).cpu()
+                v[part] = optim_ops.decode_state(self.v[part], self._scales(self.v_scale, s)).square_().cpu()
+        return {"master": self.master, "m": m, "v": v, "step": self.step_count,
                 "buckets": list(self.buckets), "world": self.bufs.world, "rank": self.bufs.rank}
+
+    def _state_parts(self):
+        return [(i, slice(s.state_off, s.state_off + s.length)) for i, s in enumerate(self.shards) if s.length > 0]
+
+    def _scales(self, t: torch.Tensor, shard: int) -> torch.Tensor:
+        return t[self.scale_offs[shard]:self.scale_offs[shard + 1]]
 
     def load_state_dict(self, sd: dict) -> None:
         assert [tuple(b) for b in sd["buckets"]] == list(self.buckets) and sd["world"] == self.bufs.world and \
             sd["rank"] == self.bufs.rank, "checkpoint was written with another sharding"
-        self.master.copy_(sd["master"]); self.m.copy_(sd["m"]); self.v.copy_(sd["v"])
+        self.master.copy_(sd["master"])
         self.step_count = int(sd["step"])
+        if self.state_bits == 32:
+            self.m.copy_(sd["m"]); self.v.copy_(sd["v"])
+            return
+        self.step_tensor.fill_(self.step_count)
+        for i, part in self._state_parts():
+            for codes, scales, value, root in ((self.m, self.m_scale, sd["m"], False), (self.v, self.v_scale, sd["v"], True)):
+                value = value[part].to(self.master.device, torch.float32)
+                c, sc = optim_ops.encode_state(value.sqrt() if root else value, root=root)
+                codes[part].copy_(c)
+                self._scales(scales, i).view(torch.uint8).copy_(sc.view(torch.uint8))
+
+    def _update_8bit(self, grads: torch.Tensor, at: str, grad_scale: float, clipped: bool) -> None:
+        """AdamW on this rank's slices, all in one launch: gradients from ``grads`` (the flat buffer or the reduced slices),
+        new parameters into this rank's buffer."""
+        parts = self._state_parts()
+        shards = [self.shards[i] for i, _ in parts]
+        if not parts:
+            return
+        cut = lambda t, off: [t[getattr(s, off):getattr(s, off) + s.length] for s in shards]  # noqa: E731
+        optim_ops.adamw_multi(
+            cut(self.bufs.params, "flat_off"), cut(grads, at), cut(self.master, "state_off"), cut(self.m, "state_off"),
+            cut(self.v, "state_off"), self.step_tensor, lr=self.lr, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps,
+            weight_decay=self.wd, grad_scale=grad_scale, m_scales=[self._scales(self.m_scale, i) for i, _ in parts],
+            v_scales=[self._scales(self.v_scale, i) for i, _ in parts], seed=self.seed, factor=self.clip_coef if clipped else None,
+            status=[t for t in (self.bufs.arena.status, self.extra_status) if t is not None])
+        self.kernel_launches += 2
 
     def _status_ptrs(self):
         a = _lib.ptr(self.bufs.arena.status)
@@ -229,6 +286,10 @@ class ShardedAdamW:
                 self.sq_parts.copy_(self.sq_sum)
             self._finish_norm(self.tp_group is None)
             clip_ptr = _lib.ptr(self.clip_coef)
+        if self.state_bits == 8:
+            self._update_8bit(b.grads, "flat_off", grad_scale, self.clip is not None)
+            self.kernel_launches += len(self.shards) if self.clip is not None else 0
+            return
         for s in self.shards:
             _lib.check(lib.dcpk_fused_rs_adamw_ag(
                 grads, params, ctypes.c_int(b.world), ctypes.c_long(s.flat_off), ctypes.c_long(s.length),
@@ -267,7 +328,13 @@ class ShardedAdamW:
             self._finish_norm()
             clip_ptr = _lib.ptr(self.clip_coef)
         params = _ptr_array(a.peer_ptrs("params"))
+        if self.state_bits == 8:
+            self._update_8bit(self.main_grad, "state_off", 1.0, self.clip is not None)
         for s in self.shards:
+            if self.state_bits == 8:   # the new parameters to every rank
+                _lib.check(lib.dcpk_cast_all_gather(_lib.ptr(self.master[s.state_off:]), params, ctypes.c_int(b.world), ctypes.c_long(s.flat_off),
+                                                    ctypes.c_long(s.length), _lib.stream_handle()), "cast_all_gather")
+                continue
             _lib.check(lib.dcpk_adamw_all_gather(
                 _lib.ptr(self.master[s.state_off:]), _lib.ptr(self.m[s.state_off:]), _lib.ptr(self.v[s.state_off:]),
                 _lib.ptr(self.main_grad[s.state_off:]), params, ctypes.c_int(b.world), ctypes.c_long(s.flat_off),

@@ -21,7 +21,7 @@ import torch
 from .data import synth
 from .data.plan_service import PlanService, PlanSpec, RankPlan
 from .models.llama import LLAMA3_8B, LlamaConfig, LlamaModel, tiny_config
-from .ops import _lib
+from .ops import _lib, fp8_ops
 from .parallel.dist_optimizer import FlatBuffers, ShardedAdamW
 from .runtime.executor_fused import FusedAttentionExecutor
 
@@ -55,6 +55,8 @@ class EngineConfig:
     cost_model: Optional[dict] = None
     plan_cache_dir: Optional[str] = None     # reuse plans by batch signature (saved next to checkpoints on resume)
     tp_size: int = 1                # tensor-parallel ranks per model replica (adjacent ranks)
+    fp8: bool = False               # products of the decoder layers' matrices in 8 bits (ops.fp8_ops)
+    optimizer_state_bits: int = 32  # 8: AdamW moments as 8-bit codes, 6 bytes per parameter less
     overlap_grad_reduce: bool = True   # reduce each layer's gradient bucket during the backward pass
     # plan every batch once (on global rank 0, in its worker pool) and hand each rank its share through a
     # TCP key-value store instead of planning on every rank; None = on whenever there are several ranks
@@ -117,7 +119,8 @@ class TrainEngine:
         n_flat = LlamaModel.flat_size(m)
         self.bufs = FlatBuffers(n_flat, device, self.opt_group if n_cp > 1 else None)
         self.model = LlamaModel(m, device, self.bufs.params, self.bufs.grads, seed=cfg.seed, recompute=cfg.recompute,
-                                lm_head_chunk=cfg.lm_head_chunk, tp_group=self.tp_group, tp_rank=self.tp_rank, tp_size=tp)
+                                lm_head_chunk=cfg.lm_head_chunk, tp_group=self.tp_group, tp_rank=self.tp_rank, tp_size=tp,
+                                fp8=cfg.fp8)
         group_tokens = cfg.tokens_per_step // (n_cp // dcp)
         cap = int(group_tokens * 1.3) + 4 * cfg.block_size
         self.executor = FusedAttentionExecutor(m.n_heads, m.n_kv_heads, cap, cap, 2 * cap, device,
@@ -128,7 +131,7 @@ class TrainEngine:
         self.optimizer = ShardedAdamW(self.bufs, cfg.lr, weight_decay=cfg.weight_decay, clip_grad=cfg.clip_grad,
                                       group=self.opt_group if n_cp > 1 else None, tp_group=self.tp_group,
                                       n_replicated=self.model.n_replicated, buckets=self.model.grad_buckets(),
-                                      extra_status=self.executor.arena.status)
+                                      extra_status=self.executor.arena.status, state_bits=cfg.optimizer_state_bits, seed=cfg.seed)
         if self.optimizer.overlap and cfg.overlap_grad_reduce:
             self.model.grad_ready_hook = self.optimizer.reduce_bucket
         self.activation_levels = self._plan_activations(group_tokens // dcp)
@@ -194,6 +197,10 @@ class TrainEngine:
             level0 = m.n_layers * tokens * (2 * m.hidden * 2 + m.n_heads * 4)
             transient = tokens * (2 * 2 * m.ffn * 2 + 2 * m.ffn * 2 + 6 * m.hidden * 2)
             lm_head = cfg.lm_head_chunk * m.vocab * 8 + m.vocab * m.hidden * 2 + 2 * tokens * m.hidden * 2
+            if cfg.fp8:
+                # the matrices' codes, kept through a step; codes of a product's operands
+                level0 += m.n_layers * (m.hidden * (m.qkv_dim + m.n_heads * m.head_dim + 3 * m.ffn))
+                transient += tokens * 2 * (2 * m.ffn + m.hidden)
             budget = free - level0 - transient - lm_head - int(16e9)
         levels = self.model.plan_activation_levels(tokens, max(0, budget))
         self.model.layer_levels = levels
@@ -275,6 +282,8 @@ class TrainEngine:
         The update kernels read the same status words and leave the weights alone when one is set."""
         self.executor.check_status()
         self.optimizer.check_status()
+        if self.cfg.fp8:
+            fp8_ops.check_status()
 
     def reconfigure(self, tokens_per_step: int, length_dist=None, mask: Optional[str] = None) -> None:
         """Switch the synthetic workload (token budget, length distribution, mask) without rebuilding
@@ -430,6 +439,8 @@ def main(argv=None):
     ap.add_argument("--log-interval", type=int, default=1)
     ap.add_argument("--save", default=None)
     ap.add_argument("--load", default=None)
+    ap.add_argument("--fp8", action="store_true", help="products of the decoder layers' matrices in 8 bits")
+    ap.add_argument("--optimizer-state-bits", type=int, default=32, choices=[8, 32], help="width of the AdamW moments")
     ap.add_argument("--activation-budget-gb", type=float, default=None)
     ap.add_argument("--dataset", default="none", choices=["none", "synthetic"],
                     help="none: batches are synthesised inside the plan service; synthetic: a Dataset of seeded "
@@ -453,7 +464,8 @@ def main(argv=None):
                        comp_imbalance_epsilon=args.dcp_comp_imbalance_epsilon,
                        inter_node_comp_imbalance_factor=args.dcp_inter_node_comp_imbalance_factor,
                        cost_model=cost if any(v is not None for v in cost.values()) else None,
-                       activation_budget_gb=args.activation_budget_gb, tp_size=args.tp_size)
+                       activation_budget_gb=args.activation_budget_gb, tp_size=args.tp_size, fp8=args.fp8,
+                       optimizer_state_bits=args.optimizer_state_bits)
     eng = TrainEngine(cfg, torch.device("cuda", local), group)
     if args.load:
         eng.load_checkpoint(args.load)

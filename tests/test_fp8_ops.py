@@ -1,0 +1,258 @@
+"""8-bit operators on the CPU: their plain forms against 64-bit arithmetic, their gradients against the formulas and against
+differences, and what they refuse.  The kernels themselves are in test_gpu_fp8.py."""
+import pytest
+import torch
+
+from dcp_b200.ops import fp8_ops as F
+from dcp_b200.ops import optim_ops as O
+
+E4M3, E5M2, E8M0 = F.E4M3, F.E5M2, F.E8M0
+
+
+def _scale_bounds(x, q):
+    """The scale is the smallest power of two with amax <= largest code * scale."""
+    largest = torch.finfo(q.codes.dtype).max
+    rows, cols = x.shape
+    for i in range(q.scales.shape[0]):
+        for j in range(q.scales.shape[1]):
+            part = x[i * q.block[0]:(i + 1) * q.block[0], j * q.block[1]:(j + 1) * q.block[1]].double().abs().max().item()
+            s = q.scales[i, j].double().item()
+            assert part <= largest * s and (part > largest * s / 2 or s == 2.0 ** -127), (i, j, part, s)
+
+
+@pytest.mark.parametrize("block", [(1, 128), (128, 1), (128, 128)])
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 127), (130, 257)])
+def test_quantize_reference(block, dtype, shape):
+    torch.manual_seed(0)
+    x = torch.randn(shape) * torch.exp2(torch.randint(-20, 20, (shape[0], 1)).float())
+    x[0] = 0
+    q = F.quantize(x, block, dtype)
+    _scale_bounds(x, q)
+    s = q._replace(codes=torch.ones_like(q.codes)).dequantize(torch.float64)
+    step, least = (2.0 ** -4, 2.0 ** -10) if dtype == E4M3 else (2.0 ** -3, 2.0 ** -17)   # half a step; of the denormals
+    err = (q.dequantize(torch.float64) - x.double()).abs()
+    assert (err <= torch.maximum(x.double().abs() * step, s * least)).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_a_block_with_a_value_that_is_not_finite_reads_back_as_nan(bad):
+    x = torch.ones(2, 300)
+    x[1, 130] = bad
+    d = F.quantize(x).dequantize()
+    assert torch.isnan(d[1, 128:256]).all() and torch.equal(d[0], x[0]) and torch.equal(d[1, :128], x[1, :128]) and \
+        torch.equal(d[1, 256:], x[1, 256:])
+
+
+def test_extreme_magnitudes_are_representable():
+    x = torch.zeros(4, 128)
+    x[0, 0], x[1, 0], x[2, 0] = 3.4028234e38, 1e-38, 2.0 ** -149
+    q = F.quantize(x)
+    d = q.dequantize(torch.float64)
+    assert abs(d[0, 0].item() / 3.4028234663852886e38 - 1) <= 2.0 ** -4 and abs(d[1, 0].item() / 1e-38 - 1) <= 2.0 ** -4
+    assert d[2, 0] == 0 and q.scales.view(torch.uint8).tolist() == [[247], [0], [0], [0]]   # 2^-149 is below half a step of 2^-136
+
+
+def _numeric(f, x, i, eps):
+    a, b = x.clone(), x.clone()
+    a.view(-1)[i] += eps
+    b.view(-1)[i] -= eps
+    return (f(a) - f(b)) / (2 * eps)
+
+
+@pytest.mark.parametrize("with_add", [False, True])
+def test_norm_backward_against_formula_and_differences(with_add):
+    torch.manual_seed(1)
+    rows, width, eps = 3, 40, 1e-5
+    h, w, dy, add = (torch.randn(s, dtype=torch.float64) for s in ((rows, width), (width,), (rows, width), (rows, width)))
+    norm = lambda t, u: t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + eps) * u  # noqa: E731
+    f = lambda t, u: ((norm(t, u) * dy).sum() + ((t * add).sum() if with_add else 0.0))  # noqa: E731
+    rstd = torch.rsqrt(h.pow(2).mean(-1) + eps)
+    dx, dw = F.rmsnorm_quant_bwd(h.float(), w.float(), rstd.float(), dy.float(), add.float() if with_add else None)
+    leaf, leaf_w = h.clone().requires_grad_(), w.clone().requires_grad_()
+    gx, gw = torch.autograd.grad(f(leaf, leaf_w), (leaf, leaf_w))
+    # a few dozen fp32 roundings of values of order one
+    assert (dx.double() - gx).abs().max() < 2e-5 and (dw.double() - gw).abs().max() < 2e-5
+    for i in (0, 17, 63, rows * width - 1):
+        assert abs(_numeric(lambda t: f(t, w), h, i, 1e-5) - gx.view(-1)[i]) < 1e-7
+    assert abs(_numeric(lambda u: f(h, u), w, 5, 1e-5) - gw[5]) < 1e-7
+
+
+def test_linear_and_norm_linear_are_their_products():
+    torch.manual_seed(2)
+    x, w, nw = torch.randn(5, 7, 200), torch.randn(48, 200), torch.randn(200)
+    res, d_out, d_h = torch.randn(5, 7, 200), torch.randn(5, 7, 48), torch.randn(5, 7, 200)
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    out = F.linear(*leaves)
+    out.backward(d_out)
+    deq = lambda t, b: F.quantize(t.reshape(-1, t.shape[-1]), b).dequantize(torch.float64)  # noqa: E731
+    near = lambda a, b: torch.testing.assert_close(a.double().reshape(b.shape), b, rtol=1e-5, atol=1e-4)  # fp32 sums of up to 200 products
+    near(out, deq(x, (1, 128)) @ deq(w, (128, 128)).t())
+    near(leaves[0].grad, deq(d_out, (1, 128)) @ deq(w, (128, 128)))
+    near(leaves[1].grad, deq(d_out, (128, 1)).t() @ deq(x, (128, 1)))
+    # the norm's, with the gradient of the sum from elsewhere
+    lx, lr, lw, ln = (t.clone().requires_grad_() for t in (x, res, w, nw))
+    out, h = F.norm_linear(lx, ln, lw, 1e-5, lr)
+    torch.autograd.backward([out, h], [d_out, d_h])
+    h2 = (x + res).reshape(-1, 200)
+    y, _, rstd = F.rmsnorm_quant(h2, nw, 1e-5)
+    near(out, y.dequantize(torch.float64) @ deq(w, (128, 128)).t())
+    assert torch.equal(h.reshape(-1, 200), h2)
+    dy = (deq(d_out, (1, 128)) @ deq(w, (128, 128))).float()
+    dx, dn = F.rmsnorm_quant_bwd(h2, nw, rstd, dy, d_h.reshape(-1, 200))
+    near(lx.grad, dx.double()), near(ln.grad, dn.double())
+    assert torch.equal(lx.grad, lr.grad)
+    near(lw.grad, deq(d_out, (128, 1)).t() @ deq(h2 * rstd[:, None] * nw, (128, 1)))
+    # only the sum is used
+    lx, lr = x.clone().requires_grad_(), res.clone().requires_grad_()
+    F.norm_linear(lx, nw, w, 1e-5, lr)[1].backward(d_h)
+    assert torch.equal(lx.grad, d_h) and torch.equal(lr.grad, d_h)
+
+
+def test_refusals_of_the_8_bit_operators():
+    x, w = torch.zeros(4, 256), torch.zeros(8, 256)
+    q, wq = F.quantize(x), F.quantize(w, (128, 128))
+    for call, words in [
+            (lambda: F.quantize(x, (1, 64)), "blocks are"),
+            (lambda: F.quantize(x[0]), "matrix"),
+            (lambda: F.quantize(x.double()), "bfloat16, float16 or float32"),
+            (lambda: F.quantize(x, dtype=torch.float16), "codes are"),
+            (lambda: F.quantize_both(x.int()), "bfloat16, float16 or float32"),
+            (lambda: F.rmsnorm_quant(x, torch.zeros(255)), "w has to be"),
+            (lambda: F.rmsnorm_quant(x, torch.zeros(256, dtype=torch.bfloat16)), "w has to be"),
+            (lambda: F.rmsnorm_quant(x, torch.zeros(256), residual=torch.zeros(4, 255)), "residual"),
+            (lambda: F.rmsnorm_quant(torch.zeros(1, 16385), torch.zeros(16385)), "16384"),
+            (lambda: F.rmsnorm_quant(torch.zeros(3, 0), torch.zeros(0)), "16384"),
+            (lambda: F.rmsnorm_quant_bwd(x, torch.zeros(256), torch.zeros(4), torch.zeros(4, 255)), "dy"),
+            (lambda: F.rmsnorm_quant_bwd(x, torch.zeros(256), torch.zeros(5), x), "rstd"),
+            (lambda: F.rmsnorm_quant_bwd(x, torch.zeros(256), torch.zeros(4), x, x.bfloat16()), "add"),
+            (lambda: F.matmul(q, F.quantize(torch.zeros(8, 128))), "contraction"),
+            (lambda: F.matmul(F.quantize(x, (128, 1)), wq), "scale per 128"),
+            (lambda: F.matmul(q, wq, trans_a=True, trans_b=False), "contraction"),
+            (lambda: F.matmul(q._replace(codes=x), wq), "codes"),
+            (lambda: F.matmul(q._replace(scales=q.scales[:2]), wq), "scales"),
+            (lambda: F.matmul(q._replace(scales=q.scales.float()), wq), "scales"),
+            (lambda: F.matmul(q._replace(block=(2, 128)), wq), "blocks are"),
+            (lambda: F.matmul(q, wq, out_dtype=torch.float64), "results are"),
+            (lambda: F.matmul(q, wq, out=torch.zeros(4, 9)), "out has to be"),
+            (lambda: F.matmul(q, wq, out=torch.zeros(8, 4).t()), "contiguous"),
+            (lambda: F.matmul(q, wq, add=torch.zeros(4, 8)), "add has to be"),
+            (lambda: F.matmul(q, wq, form=3), "form"),
+            (lambda: F.linear(x, w.bfloat16()), "of one type"),
+            (lambda: F.norm_linear(x, torch.zeros(256), w, 1e-5, x[:2]), "residual")]:
+        with pytest.raises(ValueError, match=words):
+            call()
+
+
+def test_empty_operands():
+    q, wq = F.quantize(torch.zeros(0, 256)), F.quantize(torch.zeros(8, 256), (128, 128))
+    assert F.matmul(q, wq).shape == (0, 8) and q.scales.shape == (0, 2)
+    none = F.quantize(torch.zeros(3, 0)), F.quantize(torch.zeros(5, 0), (128, 128))
+    assert torch.equal(F.matmul(*none, out_dtype=torch.float32), torch.zeros(3, 5))
+
+
+# --------------------------------------------------------------------------- AdamW
+def _state(sizes, bits, ptype, gtype, seed=0, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda n: torch.randn(n, generator=g)  # noqa: E731
+    params = [rnd(n).to(ptype).to(device) for n in sizes]
+    st = {"params": params, "grads": [(rnd(n) * 1e-2).to(gtype).to(device) for n in sizes],
+          "masters": None if ptype == torch.float32 else [p.float() for p in params], "step": torch.full((1,), 4, device=device)}
+    m, v = [rnd(n).to(device) * 1e-2 for n in sizes], [(rnd(n).to(device) * 1e-2).square() for n in sizes]
+    if bits == 32:
+        return {**st, "m": m, "v": v}
+    em, ev = [O.encode_state(t) for t in m], [O.encode_state(t.sqrt(), root=True) for t in v]
+    return {**st, "m": [c for c, _ in em], "v": [c for c, _ in ev], "m_scales": [s for _, s in em], "v_scales": [s for _, s in ev]}
+
+
+HYPER = dict(lr=1e-2, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1)
+
+
+def test_plain_adamw_is_torchs():
+    p0 = [torch.randn(7, 3), torch.randn(11)]
+    mine = [p.clone() for p in p0]
+    leaves = [p.clone().requires_grad_() for p in p0]
+    opt = torch.optim.AdamW(leaves, lr=1e-2, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+    m, v, step = [torch.zeros_like(p) for p in mine], [torch.zeros_like(p) for p in mine], torch.zeros(1, dtype=torch.int64)
+    for i in range(4):
+        grads = [torch.randn(p.shape, generator=torch.Generator().manual_seed(i)) for p in p0]
+        for leaf, g in zip(leaves, grads):
+            leaf.grad = g.clone() * 0.5
+        norm = torch.nn.utils.clip_grad_norm_(leaves, 1.0)
+        opt.step()
+        got = O.adamw_multi(mine, grads, None, m, v, step, **HYPER, grad_scale=0.5, clip=1.0)
+        assert abs(got.item() - norm.item()) < 1e-5
+    for a, b in zip(mine, leaves):
+        assert (a - b).abs().max() < 1e-6       # ten roundings of values of order one, four times
+
+
+def test_stochastic_rounding_is_right_on_average():
+    torch.manual_seed(3)
+    x = torch.randn(256)
+    bits = torch.arange(0, 65536, 37)[:, None].expand(-1, 256)
+    n = bits.shape[0]
+    codes, scales = O.encode_state(x.repeat(n), bits.reshape(-1))
+    mean = O.decode_state(codes, scales).view(n, 256).double().mean(0)
+    # random bits at distances of 37 of 65536 and cut at 16 bits: a step (2^-3 of the value at most) is hit within 38 / 65536
+    s = O.decode_state(torch.ones(256).to(E4M3), scales[:1]).double()
+    assert ((mean - x.double()).abs() <= torch.maximum(x.abs().double() * 2.0 ** -3, s * 2.0 ** -9) * 40 / 65536).all()
+
+
+def test_state_codes_come_back_to_the_bit():
+    torch.manual_seed(4)
+    for root in (False, True):
+        x = torch.randn(5000) * torch.exp2(torch.randint(-30, 5, (5000,)).float())
+        x = x.abs() if root else x
+        x[::7] = 0
+        c, s = O.encode_state(x, torch.randint(0, 65536, (5000,)), root)
+        value = O.decode_state(c, s)
+        c2, s2 = O.encode_state(value, root=root)
+        assert torch.equal(O.decode_state(c2, s2), value)
+        assert not root or ((value > 0) == (x > 0)).all()
+
+
+def test_optimizer_class_on_the_cpu():
+    torch.manual_seed(5)
+    params = [torch.randn(300, dtype=torch.bfloat16), torch.randn(4, 5, dtype=torch.bfloat16)]
+    opts = [O.MultiTensorAdamW([p.clone() for p in params], lr=1e-2, state_bits=b, clip_grad=1.0) for b in (8, 32)]
+    for i in range(3):
+        for o in opts:
+            for p in o.params:
+                p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(i)).bfloat16()
+            o.step()
+    eight, full = opts
+    assert int(eight.step_count) == 3 and eight.m.dtype == E4M3 and eight.master.dtype == torch.float32
+    # steps of lr each, whose direction differs by the roundings of m and of sqrt(v): each within a step of 2^-3
+    assert (eight.master - full.master).abs().max() < 3 * 1e-2 * 0.6
+    other = O.MultiTensorAdamW([p.clone() for p in params], lr=1e-2, state_bits=8, clip_grad=1.0)
+    other.load_state_dict(eight.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(other.params, eight.params)) and torch.equal(other.m.view(torch.uint8), eight.m.view(torch.uint8))
+    with pytest.raises(ValueError, match="another width"):
+        full.load_state_dict(eight.state_dict())
+
+
+def test_refusals_of_adamw():
+    ok = lambda **kw: {**_state([5, 300], 8, torch.bfloat16, torch.bfloat16), **HYPER, **kw}  # noqa: E731
+    st = ok()
+    for bad, words in [(dict(params=[], grads=[]), "no parameters"), (dict(grads=st["grads"][:1]), "2 parameters"),
+                       (dict(masters=None), "need fp32 masters"), (dict(v_scales=None), "scales of m and of v"),
+                       (dict(step=torch.zeros(1)), "int64"), (dict(m=[t.float() for t in st["m"]]), "tensor 0"),
+                       (dict(m_scales=[s[:1] for s in st["m_scales"]]), "tensor 1"),
+                       (dict(grads=[torch.zeros(10)[::2], torch.zeros(300)]), "tensor 0"),
+                       (dict(grads=[st["grads"][0], st["grads"][1].float()]), "tensor 1"),
+                       (dict(params=[p.double() for p in st["params"]]), "parameters and gradients"),
+                       (dict(clip=0.0), "positive"), (dict(factor=torch.zeros(2)), "factor"),
+                       (dict(status=[torch.zeros(1)]), "status")]:
+        with pytest.raises(ValueError, match=words):
+            O.adamw_multi(**ok(**bad))
+    with pytest.raises(ValueError, match="8 or 32"):
+        O.MultiTensorAdamW([torch.zeros(3)], state_bits=16)
+    with pytest.raises(ValueError, match="no gradient"):
+        O.MultiTensorAdamW([torch.zeros(3)]).step()
+
+
+def test_a_status_word_stops_the_step():
+    st = _state([5, 300], 8, torch.bfloat16, torch.bfloat16)
+    before = [p.clone() for p in st["params"]]
+    O.adamw_multi(**st, **HYPER, status=[torch.zeros(1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)])
+    assert all(torch.equal(a, b) for a, b in zip(before, st["params"])) and int(st["step"]) == 4
