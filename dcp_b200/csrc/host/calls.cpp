@@ -234,7 +234,10 @@ class SingleRankAttention {
 
 }  // namespace
 
+void bind_ops8(py::module_& m);   // ops8.cpp
+
 PYBIND11_MODULE(_calls, m) {
+  bind_ops8(m);
   using A = SingleRankAttention;
   auto free_gil = py::call_guard<py::gil_scoped_release>();   // a launch may wait for room in the stream's queue
   py::class_<A>(m, "SingleRankAttention")

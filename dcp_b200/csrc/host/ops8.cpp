@@ -1,0 +1,225 @@
+// Host side of the 8-bit operators, in native code: checks, results, workspaces and the launch of a call.
+//
+// Small calls wait for the host: driven from Python, the norm of 8 rows took 26 us for a kernel of 3, most of it checks,
+// views of the results and argument objects.  A function here takes a call whose tensors the kernels read as they lie, on
+// whatever device they are; for anything else it returns nothing before it allocates or launches anything, and the caller
+// says what is wrong or brings the tensors into shape and asks again.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <pybind11/stl.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <optional>
+#include <stdexcept>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "entries.h"
+
+namespace py = pybind11;
+using at::Tensor;
+
+namespace {
+
+constexpr long kBlock = 128, kStateBlock = 256, kNormWidth = 16384;
+
+void check(int rc, const char* what) {
+  if (rc != 0) throw std::runtime_error(std::string(what) + " failed with code " + std::to_string(rc));
+}
+void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }   // of the current device
+
+int value_type(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1; }
+int code_type(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? 0 : t == at::kFloat8_e5m2 ? 1 : -1; }
+long up(long n, long to) { return (n + to - 1) / to * to; }
+long blocks(long n, long size) { return (n + size - 1) / size; }
+
+bool dense(const Tensor& t) { return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !t.is_conj(); }
+// a matrix whose rows are contiguous, of any pitch that leaves them apart
+bool rows_of(const Tensor& t) {
+  return dense(t) && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+}
+long pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+bool on_16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
+// codes whose rows begin on 16 bytes
+Tensor empty_codes(long rows, long cols, at::ScalarType type, const Tensor& like) {
+  const Tensor t = at::empty({rows, up(cols, 16)}, like.options().dtype(type));
+  return t.size(1) == cols ? t : t.narrow(1, 0, cols);
+}
+// scales of neighbouring blocks along the contraction lie next to one another: by_cols, those of 128 x 1 blocks, by columns
+Tensor empty_scales(long rows, long cols, long br, long bc, const Tensor& like) {
+  const long nr = blocks(rows, br), nc = blocks(cols, bc);
+  const bool by_cols = bc == 1;
+  const long inner = by_cols ? nr : nc;
+  Tensor t = at::empty({by_cols ? nc : nr, up(inner, 4)}, like.options().dtype(at::kFloat8_e8m0fnu));
+  if (t.size(1) != inner) t = t.narrow(1, 0, inner);
+  return by_cols ? t.t() : t;
+}
+
+using Tensors = std::optional<std::vector<Tensor>>;
+
+// codes and scales, of ways 1 and 2 in this order; ways as dcpk_fp8_quantize has them
+Tensors quantize8(const Tensor& x, int ways, bool e5m2) {
+  if (!rows_of(x) || value_type(x.scalar_type()) < 0) return std::nullopt;
+  c10::DeviceGuard guard(x.device());
+  const long rows = x.size(0), cols = x.size(1);
+  const at::ScalarType type = e5m2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn;
+  std::vector<Tensor> out;
+  void* p[4] = {nullptr, nullptr, nullptr, nullptr};
+  long scale_pitch[2] = {0, 0};
+  for (int w : {0, 1}) {
+    if (!(w ? ways & 2 : ways & 5)) continue;
+    const long br = w || ways == 4 ? kBlock : 1, bc = w ? 1 : kBlock;
+    out.push_back(empty_codes(rows, cols, type, x));
+    out.push_back(empty_scales(rows, cols, br, bc, x));
+    p[2 * w] = out[out.size() - 2].data_ptr();
+    p[2 * w + 1] = out.back().data_ptr();
+    scale_pitch[w] = up(w ? blocks(rows, kBlock) : blocks(cols, kBlock), 4);
+  }
+  check(dcpk_fp8_quantize(value_type(x.scalar_type()), e5m2, ways, x.const_data_ptr(), pitch(x), p[0], up(cols, 16), p[1], scale_pitch[0], p[2],
+                          up(cols, 16), p[3], scale_pitch[1], rows, int(cols), stream()),
+        "fp8_quantize");
+  return out;
+}
+
+bool like(const Tensor& t, const Tensor& x) {
+  return rows_of(t) && t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device();
+}
+bool channels(const Tensor& w, const Tensor& x) {
+  return dense(w) && w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous() && w.scalar_type() == x.scalar_type() && w.device() == x.device();
+}
+bool norm_input(const Tensor& x) {
+  return rows_of(x) && value_type(x.scalar_type()) >= 0 && x.size(1) >= 1 && x.size(1) <= kNormWidth;
+}
+
+// codes, scales, h, rstd
+Tensors norm8(const Tensor& x, const Tensor& w, double eps, const std::optional<Tensor>& residual, bool e5m2) {
+  if (!norm_input(x) || !channels(w, x) || (residual && !like(*residual, x))) return std::nullopt;
+  c10::DeviceGuard guard(x.device());
+  const long rows = x.size(0), width = x.size(1);
+  Tensor codes = empty_codes(rows, width, e5m2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn, x);
+  Tensor scales = empty_scales(rows, width, 1, kBlock, x);
+  Tensor h = residual ? at::empty({rows, width}, x.options()) : x;
+  Tensor rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  check(dcpk_fp8_norm(value_type(x.scalar_type()), e5m2, x.const_data_ptr(), pitch(x), residual ? residual->const_data_ptr() : nullptr,
+                      residual ? pitch(*residual) : 0, w.const_data_ptr(), residual ? h.data_ptr() : nullptr, codes.data_ptr(), up(width, 16),
+                      scales.data_ptr(), up(blocks(width, kBlock), 4), rstd.data_ptr<float>(), rows, int(width), float(eps), stream()),
+        "fp8_norm");
+  return std::vector<Tensor>{codes, scales, h, rstd};
+}
+
+// dx, dw
+Tensors norm8_bwd(const Tensor& h, const Tensor& w, const Tensor& rstd, const Tensor& dy, const std::optional<Tensor>& add, const Tensor& status) {
+  if (!norm_input(h) || !channels(w, h) || !like(dy, h) || (add && !like(*add, h)) || !dense(rstd) || rstd.dim() != 1 ||
+      rstd.size(0) != h.size(0) || !rstd.is_contiguous() || rstd.scalar_type() != at::kFloat || rstd.device() != h.device())
+    return std::nullopt;
+  c10::DeviceGuard guard(h.device());
+  const long rows = h.size(0), width = h.size(1);
+  const auto f32 = h.options().dtype(at::kFloat);
+  Tensor dx = at::empty({rows, width}, h.options()), dw = at::empty({width}, f32);
+  const Tensor part = at::empty({dcpk_fp8_norm_bwd_parts(rows, int(width)), width}, f32);
+  check(dcpk_fp8_norm_bwd(value_type(h.scalar_type()), h.const_data_ptr(), pitch(h), w.const_data_ptr(), rstd.const_data_ptr<float>(),
+                          dy.const_data_ptr(), pitch(dy), add ? add->const_data_ptr() : nullptr, add ? pitch(*add) : 0, dx.data_ptr(),
+                          dw.data_ptr<float>(), part.data_ptr<float>(), rows, int(width), status.data_ptr<int>(), stream()),
+        "fp8_norm_bwd");
+  return std::vector<Tensor>{dx, dw};
+}
+
+// an operand as the product reads it; k_dim: the dimension that is added up
+bool operand(const Tensor& codes, const Tensor& scales, long br, long bc, int k_dim, DcpkFp8Operand* o) {
+  const long b[2] = {br, bc};
+  if (!rows_of(codes) || code_type(codes.scalar_type()) < 0 || !on_16(codes) || !dense(scales) || scales.dim() != 2 ||
+      scales.scalar_type() != at::kFloat8_e8m0fnu || scales.device() != codes.device())
+    return false;
+  for (int d : {0, 1})
+    if ((b[d] != 1 && b[d] != kBlock) || scales.size(d) != blocks(codes.size(d), b[d])) return false;
+  if (b[k_dim] != kBlock || codes.size(0) > 0x7fffffffl || codes.size(1) > 0x7fffffffl) return false;
+  const long p = codes.size(0) > 1 ? codes.stride(0) : up(codes.size(1), 16);
+  if (p % 16) return false;
+  *o = {codes.const_data_ptr(), p, scales.const_data_ptr(), scales.stride(1 - k_dim), scales.stride(k_dim), int(codes.size(1 - k_dim)),
+        k_dim == 0, b[1 - k_dim] == kBlock ? 7 : 0, code_type(codes.scalar_type())};
+  return true;
+}
+
+std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair<long, long> a_block, const Tensor& b, const Tensor& b_scales,
+                              std::pair<long, long> b_block, bool trans_a, bool trans_b, int out_type, const std::optional<Tensor>& add,
+                              const std::optional<Tensor>& out, int form, const Tensor& status) {
+  DcpkFp8Operand q, p;
+  const int ka = trans_a ? 0 : 1, kb = trans_b ? 1 : 0;
+  if (out_type < 0 || out_type > 2 || !operand(a, a_scales, a_block.first, a_block.second, ka, &q) ||
+      !operand(b, b_scales, b_block.first, b_block.second, kb, &p) || a.size(ka) != b.size(kb) || a.size(ka) < 1 || q.rows < 1 || p.rows < 1 ||
+      a.device() != b.device())
+    return std::nullopt;
+  const at::ScalarType type = out_type == 0 ? at::kFloat : out_type == 1 ? at::kHalf : at::kBFloat16;
+  for (const auto* t : {&add, &out})
+    if (*t && (!rows_of(**t) || (*t)->size(0) != q.rows || (*t)->size(1) != p.rows || (*t)->scalar_type() != type || (*t)->device() != a.device()))
+      return std::nullopt;
+  c10::DeviceGuard guard(a.device());
+  Tensor result = out ? *out : at::empty({q.rows, p.rows}, a.options().dtype(type));
+  check(dcpk_fp8_gemm(&q, &p, int(a.size(ka)), result.data_ptr(), pitch(result), add ? add->const_data_ptr() : nullptr, add ? pitch(*add) : 0,
+                      out_type, form, status.data_ptr<int>(), stream()),
+        "fp8_gemm");
+  return result;
+}
+
+using List = std::vector<Tensor>;
+
+// Whether the call was taken, and the gradients' norm where it is limited.
+std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& grads, const std::optional<List>& masters, const List& m,
+                                               const List& v, const Tensor& step, double lr, double beta1, double beta2, double eps,
+                                               double wd, double grad_scale, double clip, const std::optional<List>& m_scales,
+                                               const std::optional<List>& v_scales, unsigned seed, const std::optional<Tensor>& factor,
+                                               const List& status) {
+  const std::tuple<bool, std::optional<Tensor>> no{false, std::nullopt};
+  const size_t n = params.size();
+  if (n == 0 || n > 0x7fffffff || grads.size() != n || m.size() != n || v.size() != n || (masters && masters->size() != n) ||
+      bool(m_scales) != bool(v_scales) || (m_scales && (m_scales->size() != n || v_scales->size() != n)) || status.size() > 2 || !(clip >= 0))
+    return no;
+  const auto device = params[0].device();
+  const int ptype = value_type(params[0].scalar_type()), gtype = value_type(grads[0].scalar_type());
+  const auto state = m_scales ? at::kFloat8_e4m3fn : at::kFloat;
+  const auto plain = [&](const Tensor& t, at::ScalarType type, long size) {
+    return dense(t) && t.device() == device && t.scalar_type() == type && t.numel() == size && t.is_contiguous();
+  };
+  if (ptype < 0 || gtype < 0 || (!masters && ptype != 0) || !plain(step, at::kLong, 1) || (factor && !plain(*factor, at::kFloat, 1))) return no;
+  for (const Tensor& s : status)
+    if (!dense(s) || s.scalar_type() != at::kInt || s.numel() < 1 || s.device() != device) return no;
+  std::vector<void*> p(n), w(n), pm(n), pv(n), sm(n), sv(n);
+  std::vector<const void*> g(n);
+  std::vector<long> sizes(n);
+  for (size_t i = 0; i < n; ++i) {
+    const long size = params[i].numel(), scales = blocks(size, kStateBlock);
+    if (!plain(params[i], params[0].scalar_type(), size) || !plain(grads[i], grads[0].scalar_type(), size) || !plain(m[i], state, size) ||
+        !plain(v[i], state, size) || (masters && !plain((*masters)[i], at::kFloat, size)) ||
+        (m_scales && (!plain((*m_scales)[i], at::kFloat8_e8m0fnu, scales) || !plain((*v_scales)[i], at::kFloat8_e8m0fnu, scales))))
+      return no;
+    sizes[i] = size;
+    p[i] = params[i].data_ptr(), g[i] = grads[i].const_data_ptr(), pm[i] = m[i].data_ptr(), pv[i] = v[i].data_ptr();
+    if (masters) w[i] = (*masters)[i].data_ptr();
+    if (m_scales) sm[i] = (*m_scales)[i].data_ptr(), sv[i] = (*v_scales)[i].data_ptr();
+  }
+  c10::DeviceGuard guard(device);
+  Tensor work = at::empty({dcpk_adamw_multi_work(int(n))}, step.options().dtype(at::kDouble));
+  std::optional<Tensor> norm;
+  if (clip > 0) norm = at::empty({1}, step.options().dtype(at::kFloat));
+  const int* words[2] = {status.size() > 0 ? status[0].const_data_ptr<int>() : nullptr, status.size() > 1 ? status[1].const_data_ptr<int>() : nullptr};
+  check(dcpk_adamw_multi(int(n), p.data(), g.data(), masters ? w.data() : nullptr, pm.data(), pv.data(), m_scales ? sm.data() : nullptr,
+                         m_scales ? sv.data() : nullptr, sizes.data(), ptype, gtype, step.data_ptr<int64_t>(), float(lr), beta1, beta2,
+                         float(eps), float(wd), float(grad_scale), float(clip), factor ? factor->const_data_ptr<float>() : nullptr, seed,
+                         norm ? norm->data_ptr<float>() : nullptr, words[0], words[1], work.data_ptr<double>(), stream()),
+        "adamw_multi");
+  return {true, norm};
+}
+
+}  // namespace
+
+void bind_ops8(py::module_& m) {
+  auto free_gil = py::call_guard<py::gil_scoped_release>();   // a launch may wait for room in the stream's queue
+  m.def("quantize8", &quantize8, free_gil);
+  m.def("norm8", &norm8, free_gil);
+  m.def("norm8_bwd", &norm8_bwd, free_gil);
+  m.def("matmul8", &matmul8, free_gil);
+  m.def("adamw8", &adamw8, free_gil);
+}

@@ -18,6 +18,7 @@
 // are on the GPU, so a replayed graph counts on.
 #include <algorithm>
 
+#include "entries.h"
 #include "fp8_common.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"

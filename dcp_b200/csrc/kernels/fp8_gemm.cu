@@ -24,6 +24,7 @@
 
 #include <algorithm>
 
+#include "entries.h"
 #include "fp8_common.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -543,16 +544,6 @@ static int launch_split(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const 
 }  // namespace dcpk
 
 using namespace dcpk;
-
-// An operand's codes: `rows` x k with k innermost, or (rows_inner) k x rows; `pitch` bytes per row of memory, a multiple of
-// 16 like the base.  scales[(row >> shift) * row_stride + (k / 128) * k_stride].
-struct DcpkFp8Operand {
-  const void* codes;
-  long pitch;
-  const void* scales;
-  long scale_row_stride, scale_k_stride;
-  int rows, rows_inner, shift, code_type;
-};
 
 // out [q.rows, p.rows] = q p^T + add.  form: 0 the rule below, 1 pairs, 2 split (tests and measurements).
 extern "C" int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, int k, void* out, long out_pitch, const void* add,

@@ -12,6 +12,7 @@
 // neighbours.
 #include <algorithm>
 
+#include "entries.h"
 #include "fp8_common.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"

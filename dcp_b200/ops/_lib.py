@@ -54,7 +54,7 @@ def calls_path() -> Path:
 
 
 def calls():
-    """The native host side of single-rank attention calls (``csrc/host/calls.cpp``)."""
+    """The native host side of single-rank attention calls and of the 8-bit operators (``csrc/host``)."""
     load()
     try:
         from .. import _calls

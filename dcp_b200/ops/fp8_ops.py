@@ -18,8 +18,6 @@ their results there and may be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -32,8 +30,7 @@ MAX_NORM_WIDTH = 16384
 _CODES = {E4M3: 0, E5M2: 1}
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _KINDS = {(1, BLOCK): 1, (BLOCK, 1): 2, (BLOCK, BLOCK): 4}
-_c_int, _c_long, _c_float = ctypes.c_int, ctypes.c_long, ctypes.c_float
-_NULL = ctypes.c_void_p(0)
+_WAYS = {1: [(1, BLOCK)], 2: [(BLOCK, 1)], 3: [(1, BLOCK), (BLOCK, 1)], 4: [(BLOCK, BLOCK)]}
 
 
 class BlockScaled(NamedTuple):
@@ -56,22 +53,32 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _on(t: torch.Tensor):
-    """The tensor's device as the current one."""
-    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
-
-
 def _up(n: int, to: int) -> int:
     return -(-n // to) * to
 
 
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A 2-D tensor whose rows are contiguous, of any pitch."""
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    """A 2-D tensor whose rows are contiguous and apart, of any pitch."""
+    return t if (t.stride(1) == 1 or t.shape[1] <= 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+_NATIVE = None
+
+
+def _native():
+    """The native host side (``csrc/host/ops8.cpp``), looked up once."""
+    global _NATIVE
+    if _NATIVE is None:
+        _NATIVE = _lib.calls()
+    return _NATIVE
+
+
+def _taken(got):
+    """What the native call gave for tensors that are known to be right and have been brought into shape."""
+    if got is None:
+        raise RuntimeError("the native call does not take these tensors")
+    _lib.count(1)
+    return got
 
 
 _STATUS = {}
@@ -139,39 +146,22 @@ def _empty_codes(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tens
     return torch.empty(rows, _up(cols, 16), dtype=dtype, device=device)[:, :cols]
 
 
-def _empty_scales(rows: int, cols: int, block: Tuple[int, int], device) -> torch.Tensor:
-    """Scales with those of neighbouring blocks along the contraction next to one another: a (128, 1) tensor's are stored
-    by columns."""
-    nr, nc = -(-rows // block[0]), -(-cols // block[1])
-    if block == (BLOCK, 1):
-        return torch.empty(nc, _up(nr, 4), dtype=torch.uint8, device=device)[:, :nr].t().view(E8M0)
-    return torch.empty(nr, _up(nc, 4), dtype=torch.uint8, device=device)[:, :nc].view(E8M0)
-
-
 def _check_matrix(x: torch.Tensor, what: str) -> None:
     _need(x.dim() == 2, f"{what} has to be a matrix, not {tuple(x.shape)}")
     _need(x.dtype in _TYPES, f"{what} has to be bfloat16, float16 or float32, not {x.dtype}")
 
 
 def _quantize(x: torch.Tensor, ways: int, dtype: torch.dtype):
-    _check_matrix(x, "x")
-    _need(dtype in _CODES, f"codes are float8_e4m3fn or float8_e5m2, not {dtype}")
-    kinds = [k for k, bit in _KINDS.items() if ways & bit]
-    if not x.is_cuda:
-        return [quantize_reference(x, k, dtype) for k in kinds]
-    rows, cols = x.shape
-    with _on(x):
-        x = _rows(x)
-        out = [BlockScaled(_empty_codes(rows, cols, dtype, x.device), _empty_scales(rows, cols, k, x.device), k) for k in kinds]
-        a = next((q for q in out if q.block != (BLOCK, 1)), None)
-        b = next((q for q in out if q.block == (BLOCK, 1)), None)
-        place = lambda q, t, stride: (_NULL, _c_long(0)) if q is None else (_lib.ptr(t(q)), _c_long(stride(q)))  # noqa: E731
-        _lib.check(_lib.load().dcpk_fp8_quantize(
-            _c_int(_TYPES[x.dtype]), _c_int(_CODES[dtype]), _c_int(ways), _lib.ptr(x), _c_long(_pitch(x)),
-            *place(a, lambda q: q.codes, lambda q: _up(cols, 16)), *place(a, lambda q: q.scales, lambda q: _up(q.scales.shape[1], 4)),
-            *place(b, lambda q: q.codes, lambda q: _up(cols, 16)), *place(b, lambda q: q.scales, lambda q: _up(q.scales.shape[0], 4)),
-            _c_long(rows), _c_int(cols), _lib.stream_handle()), "fp8_quantize")
-    return out
+    kinds = _WAYS[ways]
+    got = _native().quantize8(x, ways, dtype == E5M2) if x.is_cuda and dtype in _CODES else None
+    if got is None:
+        _check_matrix(x, "x")
+        _need(dtype in _CODES, f"codes are float8_e4m3fn or float8_e5m2, not {dtype}")
+        if not x.is_cuda:
+            return [quantize_reference(x, k, dtype) for k in kinds]
+        got = _native().quantize8(_rows(x), ways, dtype == E5M2)
+    _taken(got)
+    return [BlockScaled(got[2 * i], got[2 * i + 1], k) for i, k in enumerate(kinds)]
 
 
 def quantize(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK), dtype: torch.dtype = E4M3) -> BlockScaled:
@@ -191,63 +181,45 @@ def rmsnorm_quant(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, residual:
                   dtype: torch.dtype = E4M3):
     """(y, h, rstd): h = x + residual in x's type (x itself without a residual), y = rmsnorm(h) * w as ``BlockScaled`` by rows,
     rounded once; rstd fp32 [rows].  x, residual [rows, width] of any pitch, w [width], all of one type; no autograd."""
-    _check_matrix(x, "x")
-    _need(dtype in _CODES, f"codes are float8_e4m3fn or float8_e5m2, not {dtype}")
-    rows, width = x.shape
-    _need(w.shape == (width,) and w.dtype == x.dtype, f"w has to be {x.dtype} of {width} channels")
-    _need(1 <= width <= MAX_NORM_WIDTH, f"rows of 1 to {MAX_NORM_WIDTH} channels, not {width}")
-    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "the residual has to be like x")
-    _need(all(t.device == x.device for t in (w, residual) if t is not None), "all tensors have to be on x's device")
-    if not x.is_cuda:
-        return rmsnorm_quant_reference(x, w, eps, residual, dtype)
-    with _on(x):
-        x, w = _rows(x), w.contiguous()
-        res = None if residual is None else _rows(residual)
-        h = x if res is None else torch.empty(rows, width, dtype=x.dtype, device=x.device)
-        y = BlockScaled(_empty_codes(rows, width, dtype, x.device), _empty_scales(rows, width, (1, BLOCK), x.device), (1, BLOCK))
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-        _lib.check(_lib.load().dcpk_fp8_norm(
-            _c_int(_TYPES[x.dtype]), _c_int(_CODES[dtype]), _lib.ptr(x), _c_long(_pitch(x)), _NULL if res is None else _lib.ptr(res),
-            _c_long(0 if res is None else _pitch(res)), _lib.ptr(w), _lib.ptr(h), _lib.ptr(y.codes), _c_long(_up(width, 16)),
-            _lib.ptr(y.scales), _c_long(_up(y.scales.shape[1], 4)), _lib.ptr(rstd), _c_long(rows), _c_int(width), _c_float(eps),
-            _lib.stream_handle()), "fp8_norm")
-    return y, h, rstd
+    got = _native().norm8(x, w, eps, residual, dtype == E5M2) if x.is_cuda and dtype in _CODES else None
+    if got is None:
+        _check_matrix(x, "x")
+        _need(dtype in _CODES, f"codes are float8_e4m3fn or float8_e5m2, not {dtype}")
+        width = x.shape[1]
+        _need(w.shape == (width,) and w.dtype == x.dtype, f"w has to be {x.dtype} of {width} channels")
+        _need(1 <= width <= MAX_NORM_WIDTH, f"rows of 1 to {MAX_NORM_WIDTH} channels, not {width}")
+        _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "the residual has to be like x")
+        _need(all(t.device == x.device for t in (w, residual) if t is not None), "all tensors have to be on x's device")
+        if not x.is_cuda:
+            return rmsnorm_quant_reference(x, w, eps, residual, dtype)
+        got = _native().norm8(_rows(x), w.contiguous(), eps, None if residual is None else _rows(residual), dtype == E5M2)
+    codes, scales, h, rstd = _taken(got)
+    return BlockScaled(codes, scales, (1, BLOCK)), (x if residual is None else h), rstd
 
 
 def rmsnorm_quant_bwd(h: torch.Tensor, w: torch.Tensor, rstd: torch.Tensor, dy: torch.Tensor, add: Optional[torch.Tensor] = None):
     """(dx, dw fp32) for what ``rmsnorm_quant`` returned and the gradient ``dy`` of y (of the values the codes stand for);
     ``add``, the gradient of h from elsewhere, is added to dx, which is the gradient of x and of the residual.  Sums in fp32
     and in a fixed order: the same bits in every run."""
-    _check_matrix(h, "h")
-    rows, width = h.shape
-    _need(w.shape == (width,) and w.dtype == h.dtype, f"w has to be {h.dtype} of {width} channels")
-    _need(1 <= width <= MAX_NORM_WIDTH, f"rows of 1 to {MAX_NORM_WIDTH} channels, not {width}")
-    _need(dy.shape == h.shape and dy.dtype == h.dtype, "dy has to be like h")
-    _need(add is None or (add.shape == h.shape and add.dtype == h.dtype), "add has to be like h")
-    _need(rstd.shape == (rows,) and rstd.dtype == torch.float32, f"rstd has to be float32 of {rows} rows")
-    _need(all(t.device == h.device for t in (w, rstd, dy, add) if t is not None), "all tensors have to be on h's device")
-    if not h.is_cuda:
-        return rmsnorm_quant_bwd_reference(h, w, rstd, dy, add)
-    with _on(h):
-        h, w, rstd, dy = _rows(h), w.contiguous(), rstd.contiguous(), _rows(dy)
-        add = None if add is None else _rows(add)
-        lib = _lib.load()
-        dx = torch.empty(rows, width, dtype=h.dtype, device=h.device)
-        dw = torch.empty(width, dtype=torch.float32, device=h.device)
-        part = torch.empty(lib.dcpk_fp8_norm_bwd_parts(_c_long(rows), _c_int(width)), width, dtype=torch.float32, device=h.device)
-        _lib.check(lib.dcpk_fp8_norm_bwd(
-            _c_int(_TYPES[h.dtype]), _lib.ptr(h), _c_long(_pitch(h)), _lib.ptr(w), _lib.ptr(rstd), _lib.ptr(dy), _c_long(_pitch(dy)),
-            _NULL if add is None else _lib.ptr(add), _c_long(0 if add is None else _pitch(add)), _lib.ptr(dx), _lib.ptr(dw),
-            _lib.ptr(part), _c_long(rows), _c_int(width), _lib.ptr(_status(h.device)), _lib.stream_handle()), "fp8_norm_bwd")
+    got = _native().norm8_bwd(h, w, rstd, dy, add, _status(h.device)) if h.is_cuda else None
+    if got is None:
+        _check_matrix(h, "h")
+        rows, width = h.shape
+        _need(w.shape == (width,) and w.dtype == h.dtype, f"w has to be {h.dtype} of {width} channels")
+        _need(1 <= width <= MAX_NORM_WIDTH, f"rows of 1 to {MAX_NORM_WIDTH} channels, not {width}")
+        _need(dy.shape == h.shape and dy.dtype == h.dtype, "dy has to be like h")
+        _need(add is None or (add.shape == h.shape and add.dtype == h.dtype), "add has to be like h")
+        _need(rstd.shape == (rows,) and rstd.dtype == torch.float32, f"rstd has to be float32 of {rows} rows")
+        _need(all(t.device == h.device for t in (w, rstd, dy, add) if t is not None), "all tensors have to be on h's device")
+        if not h.is_cuda:
+            return rmsnorm_quant_bwd_reference(h, w, rstd, dy, add)
+        got = _native().norm8_bwd(_rows(h), w.contiguous(), rstd.contiguous(), _rows(dy), None if add is None else _rows(add),
+                                     _status(h.device))
+    dx, dw = _taken(got)
     return dx, dw
 
 
 # --------------------------------------------------------------------------- products
-class _Operand(ctypes.Structure):
-    _fields_ = [("codes", ctypes.c_void_p), ("pitch", _c_long), ("scales", ctypes.c_void_p), ("scale_row_stride", _c_long),
-                ("scale_k_stride", _c_long), ("rows", _c_int), ("rows_inner", _c_int), ("shift", _c_int), ("code_type", _c_int)]
-
-
 def _check_scaled(q: BlockScaled, what: str) -> None:
     codes, scales, block = q
     _need(codes.dim() == 2 and codes.dtype in _CODES, f"{what}: codes have to be a float8_e4m3fn or float8_e5m2 matrix")
@@ -257,16 +229,12 @@ def _check_scaled(q: BlockScaled, what: str) -> None:
     _need(scales.device == codes.device, f"{what}: codes and scales on two devices")
 
 
-def _operand(q: BlockScaled, k_dim: int) -> Tuple[_Operand, tuple]:
-    """The operand as the kernel takes it and the tensors that have to live until it is launched."""
-    codes, scales, block = q
-    inner = 1 if codes.stride(1) == 1 or codes.shape[1] == 1 else None
-    if inner is None or codes.data_ptr() % 16 or (codes.shape[0] > 1 and (codes.stride(0) % 16 or codes.stride(0) < codes.shape[1])):
+def _on_16(q: BlockScaled) -> BlockScaled:
+    """The operand with codes whose rows begin on 16 bytes, as the makers here lay them out."""
+    codes = _rows(q.codes)
+    if codes.data_ptr() % 16 or (codes.shape[0] > 1 and codes.stride(0) % 16):
         codes = _empty_codes(*codes.shape, codes.dtype, codes.device).copy_(codes)
-    pitch = codes.stride(0) if codes.shape[0] > 1 else _up(codes.shape[1], 16)
-    row_dim = 1 - k_dim
-    return _Operand(codes.data_ptr(), pitch, scales.data_ptr(), scales.stride(row_dim), scales.stride(k_dim), codes.shape[row_dim],
-                    k_dim == 0, 7 if block[row_dim] == BLOCK else 0, _CODES[codes.dtype]), (codes, scales)
+    return q._replace(codes=codes)
 
 
 def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bool = True, out_dtype: torch.dtype = torch.bfloat16,
@@ -278,40 +246,37 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
     both need a scale per 128 values; along the other dimension one per value or per 128.  Codes whose rows begin on 16 bytes
     (as the makers here lay them out) are read where they are, others are copied first.  ``form``: 0 chooses the kernel, 1 and
     2 name it (measurements)."""
-    _check_scaled(a, "a")
-    _check_scaled(b, "b")
-    ka, kb = (0 if trans_a else 1), (1 if trans_b else 0)
-    m, n, k = a.codes.shape[1 - ka], b.codes.shape[1 - kb], a.codes.shape[ka]
-    _need(k == b.codes.shape[kb], f"contraction over {k} values of a and {b.codes.shape[kb]} of b")
-    _need(a.block[ka] == BLOCK and b.block[kb] == BLOCK, "both operands need a scale per 128 values along the contraction")
-    _need(a.codes.device == b.codes.device, "a and b are on two devices")
-    _need(form in (0, 1, 2), "form is 0, 1 or 2")
     if out is not None:
         out_dtype = out.dtype
-        _need(tuple(out.shape) == (m, n) and out.device == a.codes.device, f"out has to be {(m, n)} on a's device")
-        _need(n <= 1 or out.stride(1) == 1, "rows of out have to be contiguous")
-    _need(out_dtype in _TYPES, f"results are bfloat16, float16 or float32, not {out_dtype}")
-    if add is not None:
-        _need(tuple(add.shape) == (m, n) and add.dtype == out_dtype and add.device == a.codes.device,
-              f"add has to be {out_dtype} {(m, n)} on a's device")
-    if not a.codes.is_cuda:
-        got = matmul_reference(a, b, trans_a, trans_b, out_dtype, add)
-        return got if out is None else out.copy_(got)
-    with _on(a.codes):
-        if out is None:
-            out = torch.empty(m, n, dtype=out_dtype, device=a.codes.device)
-        if m == 0 or n == 0:
-            return out
-        if k == 0:
+
+    def call(a, b, add):
+        return _native().matmul8(*a, *b, trans_a, trans_b, _TYPES.get(out_dtype, -1), add, out, form, _status(a.codes.device))
+
+    got = call(a, b, add) if a.codes.is_cuda and form in (0, 1, 2) else None
+    if got is None:
+        _check_scaled(a, "a")
+        _check_scaled(b, "b")
+        ka, kb = (0 if trans_a else 1), (1 if trans_b else 0)
+        m, n, k = a.codes.shape[1 - ka], b.codes.shape[1 - kb], a.codes.shape[ka]
+        _need(k == b.codes.shape[kb], f"contraction over {k} values of a and {b.codes.shape[kb]} of b")
+        _need(a.block[ka] == BLOCK and b.block[kb] == BLOCK, "both operands need a scale per 128 values along the contraction")
+        _need(a.codes.device == b.codes.device, "a and b are on two devices")
+        _need(form in (0, 1, 2), "form is 0, 1 or 2")
+        _need(out_dtype in _TYPES, f"results are bfloat16, float16 or float32, not {out_dtype}")
+        if out is not None:
+            _need(tuple(out.shape) == (m, n) and out.device == a.codes.device, f"out has to be {(m, n)} on a's device")
+            _need(out is _rows(out), "rows of out have to be contiguous")
+        if add is not None:
+            _need(tuple(add.shape) == (m, n) and add.dtype == out_dtype and add.device == a.codes.device,
+                  f"add has to be {out_dtype} {(m, n)} on a's device")
+        if not a.codes.is_cuda:
+            got = matmul_reference(a, b, trans_a, trans_b, out_dtype, add)
+            return got if out is None else out.copy_(got)
+        if m == 0 or n == 0 or k == 0:
+            out = torch.empty(m, n, dtype=out_dtype, device=a.codes.device) if out is None else out
             return out.zero_() if add is None else out.copy_(add)
-        add = None if add is None else _rows(add)
-        qa, keep_a = _operand(a, ka)
-        qb, keep_b = _operand(b, kb)
-        _lib.check(_lib.load().dcpk_fp8_gemm(
-            ctypes.byref(qa), ctypes.byref(qb), _c_int(k), _lib.ptr(out), _c_long(_pitch(out)), _NULL if add is None else _lib.ptr(add),
-            _c_long(0 if add is None else _pitch(add)), _c_int(_TYPES[out_dtype]), _c_int(form), _lib.ptr(_status(out.device)),
-            _lib.stream_handle()), "fp8_gemm")
-    return out
+        got = call(_on_16(a), _on_16(b), None if add is None else _rows(add))
+    return _taken(got) if out is None else (_taken(got), out)[1]
 
 
 # --------------------------------------------------------------------------- autograd

@@ -5,13 +5,12 @@
 """
 from __future__ import annotations
 
-import ctypes
 from typing import List, Optional, Sequence
 
 import torch
 
 from . import _lib
-from .fp8_ops import E4M3, E8M0, _need, _on, _scale_bytes
+from .fp8_ops import E4M3, E8M0, _native, _need, _scale_bytes
 
 STATE_BLOCK = 256       # values that share a scale in an 8-bit moment
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -93,10 +92,6 @@ def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta
     return norm
 
 
-def _pointers(ts: Optional[Sequence[torch.Tensor]]):
-    return None if ts is None else (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
-
-
 def _check_lists(params, grads, masters, m, v, step, m_scales, v_scales):
     n = len(params)
     _need(n > 0, "no parameters")
@@ -133,30 +128,24 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
     of sqrt(v), rounded stochastically by a hash of ``seed``, step, tensor and element: right on average, and the same bits
     for the same inputs.  ``step``: one int64 on the device, counted up by the call, so a captured step can be replayed; all
     other numbers are the call's.  A gradient that is not finite makes its own element NaN, and with ``clip`` all."""
-    _check_lists(params, grads, masters, m, v, step, m_scales, v_scales)
-    _need(clip is None or clip > 0, "clip has to be positive")
-    _need(factor is None or (factor.dtype == torch.float32 and factor.numel() == 1 and factor.device == step.device),
-          "factor has to be one float32 on the parameters' device")
-    _need(len(status) <= 2 and all(s.dtype == torch.int32 and s.device == step.device for s in status), "status: up to two int32 words")
-    if not params[0].is_cuda:
+    def call():
+        return _native().adamw8(params, grads, masters, m, v, step, lr, beta1, beta2, eps, weight_decay, grad_scale, clip or 0.0, m_scales,
+                                   v_scales, seed & 0xFFFFFFFF, factor, status)
+
+    taken, norm = call() if step.is_cuda and (clip is None or clip > 0) else (False, None)
+    if not taken:
+        _check_lists(params, grads, masters, m, v, step, m_scales, v_scales)
+        _need(clip is None or clip > 0, "clip has to be positive")
+        _need(factor is None or (factor.dtype == torch.float32 and factor.numel() == 1 and factor.device == step.device),
+              "factor has to be one float32 on the parameters' device")
+        _need(len(status) <= 2 and all(s.dtype == torch.int32 and s.device == step.device for s in status), "status: up to two int32 words")
+        _need(not step.is_cuda, "the native call does not take these tensors")
         if any(int(s.reshape(-1)[0]) for s in status):
             return None if clip is None else torch.zeros(1)
         return adamw_multi_reference(params, grads, masters, m, v, step, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
                                      weight_decay=weight_decay, grad_scale=grad_scale if factor is None else grad_scale * float(factor),
                                      clip=clip, m_scales=m_scales, v_scales=v_scales, seed=seed)
-    n, lib = len(params), _lib.load()
-    lib.dcpk_adamw_multi_work.restype = ctypes.c_long
-    f, d = ctypes.c_float, ctypes.c_double
-    with _on(step):
-        work = torch.empty(lib.dcpk_adamw_multi_work(ctypes.c_int(n)), dtype=torch.float64, device=step.device)
-        norm = torch.empty(1, dtype=torch.float32, device=step.device) if clip is not None else None
-        sizes = (ctypes.c_long * n)(*[p.numel() for p in params])
-        _lib.check(lib.dcpk_adamw_multi(
-            ctypes.c_int(n), _pointers(params), _pointers(grads), _pointers(masters), _pointers(m), _pointers(v), _pointers(m_scales),
-            _pointers(v_scales), sizes, ctypes.c_int(_TYPES[params[0].dtype]), ctypes.c_int(_TYPES[grads[0].dtype]), _lib.ptr(step), f(lr),
-            d(beta1), d(beta2), f(eps), f(weight_decay), f(grad_scale), f(clip or 0.0), None if factor is None else _lib.ptr(factor),
-            ctypes.c_uint(seed & 0xFFFFFFFF), None if norm is None else _lib.ptr(norm), *[_lib.ptr(s) for s in status], *[None] * (2 - len(status)),
-            _lib.ptr(work), _lib.stream_handle()), "adamw_multi")
+    _lib.count(1)
     return norm
 
 
