@@ -158,8 +158,11 @@ std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair
       return std::nullopt;
   c10::DeviceGuard guard(a.device());
   Tensor result = out ? *out : at::empty({q.rows, p.rows}, a.options().dtype(type));
+  const long bytes = dcpk_fp8_gemm_work(q.rows, p.rows, q.rows_inner, int(a.size(ka)), form);
+  Tensor work;   // of this call alone
+  if (bytes > 0) work = at::empty({bytes}, a.options().dtype(at::kByte));
   check(dcpk_fp8_gemm(&q, &p, int(a.size(ka)), result.data_ptr(), pitch(result), add ? add->const_data_ptr() : nullptr, add ? pitch(*add) : 0,
-                      out_type, form, status.data_ptr<int>(), stream()),
+                      out_type, form, bytes > 0 ? work.data_ptr() : nullptr, status.data_ptr<int>(), stream()),
         "fp8_gemm");
   return result;
 }

@@ -31,7 +31,8 @@ int dcpk_fp8_norm_bwd_parts(long n_rows, int width);
 int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const void* w, const float* rstd, const void* dy, long dy_pitch, const void* add,
                       long add_pitch, void* dx, float* dw, float* part, long n_rows, int width, int* status, void* stream);
 int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, int k, void* out, long out_pitch, const void* add, long add_pitch,
-                  int out_type, int form, int* status, void* stream);
+                  int out_type, int form, void* work, int* status, void* stream);
+long dcpk_fp8_gemm_work(long q_rows, long p_rows, int q_rows_inner, int k, int form);
 long dcpk_adamw_multi_work(int n_tensors);
 int dcpk_adamw_multi(int n_tensors, void* const* params, const void* const* grads, void* const* masters, void* const* ms, void* const* vs,
                      void* const* m_scales, void* const* v_scales, const long* sizes, int param_type, int grad_type, int64_t* step, float lr,

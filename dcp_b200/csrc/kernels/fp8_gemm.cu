@@ -34,7 +34,7 @@
 namespace dcpk {
 
 static constexpr int kGemmThreads = 512;   // TMA producer, UMMA issuer, 2 idle warps; 4 scale warps; 8 epilogue warps
-static constexpr int kGemmStages = 7;
+static constexpr int kGemmStages = 6;
 static constexpr int kTileBytes = 128 * 128;  // 128 rows x 128 values, or 128 values x 128 rows
 static constexpr int kScaleBufs = 4;          // of 512 values of k each
 static constexpr int kGemmPairs = 148 / 2;
@@ -56,6 +56,11 @@ struct GemmArgs {
   int tiles_p, tiles_q;
   uint32_t idesc;
   int* status;
+  // pairs: tiles before `whole` are taken by one pair each, the others by `parts` pairs that have a part of k each and leave
+  // sums in `part_sums`; `tickets` (zeros) count those that are through
+  int whole, parts;
+  float* part_sums;
+  int* tickets;
 };
 
 // Instruction descriptor of kind::mxf8f6f4: [4,6) byte of B's scale word; [7,10) / [10,13) type of A / B (0 e4m3, 1 e5m2);
@@ -133,11 +138,36 @@ __device__ __forceinline__ void store_result(T* to, const T* from, float v) {
 struct __align__(1024) GemmSmem {
   uint8_t p[kGemmStages][kTileBytes];
   uint8_t q[kGemmStages][kTileBytes];
+  uint32_t scales[2][128 + 256];   // words of 512 values of k: of p, of q
   // of the even CTA (bytes and arrivals of both): full, scale_full, acc_empty; the others are signalled in both
   uint64_t full[kGemmStages], empty[kGemmStages], scale_full[kScaleBufs], scale_empty[kScaleBufs], acc_full, acc_empty;
   uint32_t tmem_base;
   int abort_word;
 };
+
+// What a pair works on in its i-th turn: a tile and the blocks [kb0, kb1) of k.  Whole tiles come first; the last few, which
+// would leave most pairs idle, are cut along k (in groups of four blocks, whose scales share a word).
+struct Unit { int tp, tq, kb0, kb1, cut; };   // cut: index among the parts of cut tiles, -1 for a whole one
+__device__ __forceinline__ void tile_at(int i, int tiles_p, int tiles_q, int& tp, int& tq);
+__device__ __forceinline__ bool unit_at(const GemmArgs& a, int u, Unit& unit) {
+  const int n_tiles = a.tiles_p * a.tiles_q;
+  if (u >= a.whole + (n_tiles - a.whole) * a.parts) return false;
+  unit.kb0 = 0;
+  unit.kb1 = a.n_kb;
+  unit.cut = u - a.whole;
+  int tile = u;
+  if (unit.cut < 0) {
+    unit.cut = -1;
+  } else {
+    const int part = unit.cut % a.parts, groups = (a.n_kb + 3) / 4;
+    tile = a.whole + unit.cut / a.parts;
+    unit.kb0 = 4 * (groups * part / a.parts);
+    unit.kb1 = min(4 * (groups * (part + 1) / a.parts), a.n_kb);
+    if (a.parts == 1) unit.cut = -1;
+  }
+  tile_at(tile, a.tiles_p, a.tiles_q, unit.tp, unit.tq);
+  return true;
+}
 
 // Neighbouring tiles in time share operands in L2: eight tiles of q by as many of p as are under way.
 __device__ __forceinline__ void tile_at(int i, int tiles_p, int tiles_q, int& tp, int& tq) {
@@ -173,7 +203,8 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
   grid_wait();
   const uint32_t tmem = sm.tmem_base;
   volatile int* abort_word = &sm.abort_word;
-  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, n_tiles = args.tiles_p * args.tiles_q, n_kb = args.n_kb;
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, n_kb = args.n_kb;
+  Unit unit;
   constexpr int kScaleCol = 256;   // TMEM: results [0, 256), scales of the buffers behind them, 4 columns of p, 8 of q each
   // a CTA that gives up tells the other, which waits for it
   auto wait = [&](uint64_t* bar, int parity) -> bool {
@@ -190,9 +221,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
     const uint32_t addr = tmem + (uint32_t(quad * 32) << 16) + half * 128;
     const uint32_t empty_bar = cluster_addr(smem_u32(&sm.acc_empty), 0);
     int ph = 0;
-    for (int i = pair; i < n_tiles; i += n_pairs, ph ^= 1) {
-      int tp, tq;
-      tile_at(i, args.tiles_p, args.tiles_q, tp, tq);
+    for (int u = pair; unit_at(args, u, unit); u += n_pairs, ph ^= 1) {
       if (!__all_sync(0xffffffffu, wait(&sm.acc_full, ph))) break;
       tc_fence_after();
       uint32_t acc[128];
@@ -202,13 +231,34 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(empty_bar);   // the results are in registers: the next tile's products may come
-      const int p = (tp * 2 + X) * 128 + quad * 32 + lane, q0 = tq * 256 + half * 128;
+      const int p = (unit.tp * 2 + X) * 128 + quad * 32 + lane, q0 = unit.tq * 256 + half * 128, n = args.q.rows - q0;
+      if (unit.cut >= 0) {
+        // A part of k: the sums of this warp's 32 p x 128 q go to memory.  The last of the parts to come adds them all up, in
+        // the order of k: the same bits whichever is last.
+        constexpr int kPart = 128 * 32;   // floats of a warp; 16 warps of a pair
+        const int cut_tile = unit.cut / args.parts, mine = X * 8 + warp - 8;
+        float* to = args.part_sums + (size_t(unit.cut) * 16 + mine) * kPart + lane;
+#pragma unroll
+        for (int c = 0; c < 128; ++c) __stcg(to + c * 32, __uint_as_float(acc[c]));
+        __threadfence();
+        __syncwarp();
+        int last = 0;
+        if (lane == 0) last = atomicAdd(args.tickets + cut_tile * 16 + mine, 1) == args.parts - 1;
+        if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+        __threadfence();
+        const float* from = args.part_sums + (size_t(cut_tile) * args.parts * 16 + mine) * kPart + lane;
+#pragma unroll
+        for (int c = 0; c < 128; ++c) acc[c] = 0;
+#pragma unroll 1
+        for (int part = 0; part < args.parts; ++part, from += 16 * kPart)
+#pragma unroll
+          for (int c = 0; c < 128; ++c) acc[c] = __float_as_uint(__uint_as_float(acc[c]) + __ldcg(from + c * 32));
+      }
       if (p < args.p.rows)
         by_output(args, [&](auto type, auto added) {
           using T = typename decltype(type)::T;
           T* to = static_cast<T*>(args.out) + size_t(q0) * args.out_pitch + p;
           const T* from = static_cast<const T*>(args.add) + size_t(q0) * args.add_pitch + p;
-          const int n = args.q.rows - q0;
 #pragma unroll
           for (int c = 0; c < 128; ++c, to += args.out_pitch, from += args.add_pitch)
             if (c < n) store_result<decltype(added)::value>(to, from, __uint_as_float(acc[c]));
@@ -217,33 +267,51 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
   } else if (warp >= 4) {
     // ------------------------------------------------------------ scales: every warp to its quarter of the lanes
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    const int quad = warp & 3;
+    const int quad = warp & 3, t = threadIdx.x & 127;
     const uint32_t full_bar = cluster_addr(smem_u32(&sm.scale_full[0]), 0);
-    int buf = 0, ph = 1, used = 0;
+    int buf = 0, ph = 1, used = 0, turn = 0;
     bool ok = true;
-    for (int i = pair; i < n_tiles && ok; i += n_pairs) {
-      int tp, tq;
-      tile_at(i, args.tiles_p, args.tiles_q, tp, tq);
-      const int p0 = (tp * 2 + X) * 128 + lane, q0 = tq * 256 + lane;
-      for (int kb = 0; kb < n_kb; kb += 4) {
-        uint32_t wp[4], wq[8];
+    // Each thread brings three of the 384 words, while those before are on their way to TMEM: with scales that are not
+    // neighbours along k (four bytes each) twelve words per thread, one group after the other, a weight gradient over
+    // 16384 tokens took 1130 us.
+    uint32_t next[3];
+    const auto fetch = [&](int kb) {
+      next[0] = scale_word(args.p, (unit.tp * 2 + X) * 128 + t, kb, n_kb);
+      next[1] = scale_word(args.q, unit.tq * 256 + t, kb, n_kb);
+      next[2] = scale_word(args.q, unit.tq * 256 + 128 + t, kb, n_kb);
+    };
+    int u = pair, kb = 0;
+    bool more = unit_at(args, u, unit);
+    if (more) fetch(kb = unit.kb0);
+    while (more) {
+      uint32_t* words = sm.scales[turn];
+      turn ^= 1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wp[j] = scale_word(args.p, p0 + 32 * j, kb, n_kb);
+      for (int j = 0; j < 3; ++j) words[t + 128 * j] = next[j];
+      kb += 4;
+      if (kb >= unit.kb1) {
+        more = unit_at(args, u += n_pairs, unit);
+        kb = unit.kb0;
+      }
+      if (more) fetch(kb);
+      asm volatile("bar.sync 1, 128;" ::: "memory");   // the words of all four warps are there, and those before the last are read
+      uint32_t w[12];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) wq[j] = scale_word(args.q, q0 + 32 * j, kb, n_kb);
-        ok = __all_sync(0xffffffffu, wait(&sm.scale_empty[buf], ph));
-        if (!ok) break;
+      for (int j = 0; j < 12; ++j) w[j] = words[lane + 32 * j];
+      ok = __all_sync(0xffffffffu, wait(&sm.scale_empty[buf], ph));
+      // a warp that gave up goes on to the barriers: the others wait there
+      if (ok) {
         tc_fence_after();
         const uint32_t to = tmem + (uint32_t(quad * 32) << 16) + kScaleCol + buf * 16;
-        tmem_st4(to, wp);
-        tmem_st8(to + 4, wq);
+        tmem_st4(to, w);
+        tmem_st8(to + 4, w + 4);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(full_bar + 8 * buf);
-        used |= 1 << buf;
-        if (++buf == kScaleBufs) { buf = 0; ph ^= 1; }
       }
+      used |= 1 << buf;
+      if (++buf == kScaleBufs) { buf = 0; ph ^= 1; }
     }
     // what the even CTA's issuer signals has all come in before this CTA may retire
     for (int i = 0; i < kScaleBufs && ok; ++i) {
@@ -257,11 +325,9 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
       const uint32_t full_bar = cluster_addr(smem_u32(&sm.full[0]), 0);
       int stage = 0, ph = 1, used = 0;
       bool ok = true;
-      for (int i = pair; i < n_tiles && ok; i += n_pairs) {
-        int tp, tq;
-        tile_at(i, args.tiles_p, args.tiles_q, tp, tq);
-        const int p0 = (tp * 2 + X) * 128, q0 = tq * 256 + X * 128;
-        for (int kb = 0; kb < n_kb; ++kb) {
+      for (int u = pair; ok && unit_at(args, u, unit); u += n_pairs) {
+        const int p0 = (unit.tp * 2 + X) * 128, q0 = unit.tq * 256 + X * 128;
+        for (int kb = unit.kb0; kb < unit.kb1; ++kb) {
           ok = wait(&sm.empty[stage], ph);
           if (!ok) break;
           if (X == 0) mbar_expect_tx(&sm.full[stage], 4 * kTileBytes);
@@ -288,10 +354,10 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
       constexpr uint32_t kPK = kPMn ? 256 : 2, kQK = kQMn ? 256 : 2;   // 32 values of k
       int stage = 0, ph = 0, buf = 0, sph = 0, aph = 1, done = 0;
       bool ok = true;
-      for (int i = pair; i < n_tiles && ok; i += n_pairs) {
+      for (int u = pair; ok && unit_at(args, u, unit); u += n_pairs) {
         ok = wait(&sm.acc_empty, aph);   // the last tile's results are in registers
         aph ^= 1;
-        for (int kb = 0; kb < n_kb && ok; ++kb) {
+        for (int kb = unit.kb0; kb < unit.kb1 && ok; ++kb) {
           if ((kb & 3) == 0) ok = wait(&sm.scale_full[buf], sph);
           ok = ok && wait(&sm.full[stage], ph);
           if (!ok) break;
@@ -300,9 +366,9 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_mx_pair(tmem, desc(p_lo + stage * kStep + k * kPK), desc(q_lo + stage * kStep + k * kQK), idesc, scales, scales + 4,
-                         (kb > 0 || k > 0) ? 1u : 0u);
+                         (kb > unit.kb0 || k > 0) ? 1u : 0u);
           umma_commit_pair(&sm.empty[stage]);
-          if ((kb & 3) == 3 || kb + 1 == n_kb) {
+          if ((kb & 3) == 3 || kb + 1 == unit.kb1) {
             umma_commit_pair(&sm.scale_empty[buf]);
             if (++buf == kScaleBufs) { buf = 0; sph ^= 1; }
           }
@@ -337,6 +403,7 @@ struct __align__(1024) SplitSmem {
     };
     float part[kN][128];   // this CTA's sums, when all products are through
   };
+  uint32_t scales[2][256];
   uint64_t full[split_stages<kN>()], empty[split_stages<kN>()], scale_full[kScaleBufs], scale_empty[kScaleBufs], acc_full;
   uint32_t tmem_base;
   int abort_word;
@@ -425,25 +492,36 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
       for (int spin = 0; spin < 200000 && !mbar_try_wait(&sm.acc_full, 0); ++spin) {}
     }
   } else if (warp >= 4) {
-    const int quad = warp & 3;
-    int buf = 0, ph = 1;
+    const int quad = warp & 3, t = threadIdx.x & 127;
+    int buf = 0, ph = 1, turn = 0;
     bool ok = true;
+    uint32_t next[2];
+    const auto fetch = [&](int kb) {
+      next[0] = scale_word(args.p, p0 + t, kb, args.n_kb);
+      next[1] = t < kN ? scale_word(args.q, q0 + t, kb, args.n_kb) : 0u;
+    };
+    fetch(kb0);
     for (int kb = kb0; kb < kb1; kb += 4) {
-      uint32_t wp[4], wq[4];
+      uint32_t* words = sm.scales[turn];
+      turn ^= 1;
+      words[t] = next[0];
+      words[128 + t] = next[1];
+      if (kb + 4 < kb1) fetch(kb + 4);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) wp[j] = scale_word(args.p, p0 + lane + 32 * j, kb, args.n_kb);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) wq[j] = 32 * j < kN ? scale_word(args.q, q0 + lane + 32 * j, kb, args.n_kb) : 0u;
+      for (int j = 0; j < 8; ++j) w[j] = words[lane + 32 * j];
       ok = __all_sync(0xffffffffu, mbar_wait(&sm.scale_empty[buf], ph, abort_word));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t to = tmem + (uint32_t(quad * 32) << 16) + kScaleCol + buf * 8;
-      tmem_st4(to, wp);
-      tmem_st4(to + 4, wq);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.scale_full[buf]);
+      if (ok) {   // a warp that gave up goes on to the barriers: the others wait there
+        tc_fence_after();
+        const uint32_t to = tmem + (uint32_t(quad * 32) << 16) + kScaleCol + buf * 8;
+        tmem_st4(to, w);
+        tmem_st4(to + 4, w + 4);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.scale_full[buf]);
+      }
       if (++buf == kScaleBufs) { buf = 0; ph ^= 1; }
     }
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.acc_full, 0, abort_word));
@@ -526,8 +604,8 @@ static int launch_pair(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const G
   const int smem = int(sizeof(GemmSmem)) + 1024;
   auto kernel = fp8_gemm_pair_kernel<kPMn, kQMn>;
   if (raise_smem_limit(kernel, smem, g_gemm_smem_raised[kPMn * 2 + kQMn]) != cudaSuccess) return -4;
-  const int tiles = args.tiles_p * args.tiles_q;
-  const cudaError_t rc = launch_overlapped(kernel, dim3(2 * std::min(tiles, kGemmPairs)), kGemmThreads, smem, stream, 1, false, tm_p, tm_q, args);
+  const int units = args.whole + (args.tiles_p * args.tiles_q - args.whole) * args.parts;
+  const cudaError_t rc = launch_overlapped(kernel, dim3(2 * std::min(units, kGemmPairs)), kGemmThreads, smem, stream, 1, false, tm_p, tm_q, args);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
@@ -545,9 +623,45 @@ static int launch_split(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const 
 
 using namespace dcpk;
 
-// out [q.rows, p.rows] = q p^T + add.  form: 0 the rule below, 1 pairs, 2 split (tests and measurements).
+// Which kernel, and how its work is cut.
+struct GemmPlan {
+  bool pairs;
+  int n;                    // q of a tile
+  long tiles_p, tiles_q;
+  int whole, parts;         // pairs: see GemmArgs; split: parts
+  long work() const { return pairs && parts > 1 ? (tiles_p * tiles_q - whole) * (parts * 16l * 128 * 32 * 4 + 16 * 4) : 0; }
+};
+static GemmPlan plan_gemm(long p_rows, long q_rows, bool q_rows_inner, int k, int form) {
+  GemmPlan g;
+  const int groups = ((k + 127) / 128 + 3) / 4;
+  g.tiles_p = (p_rows + 255) / 256;
+  g.tiles_q = (q_rows + 255) / 256;
+  const long pair_tiles = g.tiles_p * g.tiles_q;
+  g.pairs = form == 1 || (form == 0 && q_rows > 128 && pair_tiles >= 48);
+  if (g.pairs) {
+    g.n = 256;
+    const int rest = int(pair_tiles % kGemmPairs);
+    g.parts = rest > 0 ? std::max(1, std::min(kGemmPairs / rest, groups)) : 1;
+    g.whole = int(std::min(g.parts > 1 ? pair_tiles - rest : pair_tiles, 0x7fffffffl));
+    return g;
+  }
+  g.n = q_rows_inner || q_rows > 64 ? 128 : q_rows > 32 ? 64 : q_rows > 16 ? 32 : 16;
+  g.tiles_p = (p_rows + 127) / 128;
+  g.tiles_q = (q_rows + g.n - 1) / g.n;
+  g.whole = 0;
+  g.parts = int(std::max(1l, std::min({148 / (g.tiles_p * g.tiles_q), long(groups), long(kSplitMax)})));
+  return g;
+}
+
+// bytes of scratch a call needs; 0: none
+extern "C" long dcpk_fp8_gemm_work(long q_rows, long p_rows, int q_rows_inner, int k, int form) {
+  return q_rows <= 0 || p_rows <= 0 || k <= 0 ? 0 : plan_gemm(p_rows, q_rows, q_rows_inner, k, form).work();
+}
+
+// out [q.rows, p.rows] = q p^T + add.  form: 0 by rule, 1 pairs, 2 split (tests and measurements).  work: scratch of
+// dcpk_fp8_gemm_work() bytes.
 extern "C" int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, int k, void* out, long out_pitch, const void* add,
-                             long add_pitch, int out_type, int form, int* status, void* stream) {
+                             long add_pitch, int out_type, int form, void* work, int* status, void* stream) {
   if (q->rows <= 0 || p->rows <= 0) return 0;
   if (k <= 0 || out_type < 0 || out_type > 2) return -3;
   GemmArgs args;
@@ -567,10 +681,16 @@ extern "C" int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, i
   args.add_pitch = add_pitch;
   args.out_type = out_type;
   args.status = status;
-  const long pair_tiles = long((p->rows + 255) / 256) * ((q->rows + 255) / 256);
-  const bool pairs = form == 1 || (form == 0 && q->rows > 128 && pair_tiles >= 48);
-  const bool small = !pairs && !q->rows_inner;
-  const int n = pairs ? 256 : small && q->rows <= 16 ? 16 : small && q->rows <= 32 ? 32 : small && q->rows <= 64 ? 64 : 128;
+  const GemmPlan plan = plan_gemm(p->rows, q->rows, q->rows_inner, k, form);
+  const bool pairs = plan.pairs;
+  const int n = plan.n;
+  if (plan.tiles_p * plan.tiles_q * kSplitMax > 0x7fffffffl) return -3;
+  args.tiles_p = int(plan.tiles_p);
+  args.tiles_q = int(plan.tiles_q);
+  args.whole = plan.whole;
+  args.parts = plan.parts;
+  args.part_sums = nullptr;
+  args.tickets = nullptr;
   const auto map = [&](CUtensorMap* m, const DcpkFp8Operand& o, int box) {
     return o.rows_inner ? encode_codes_map(m, o.codes, k, o.rows, o.pitch, 128) : encode_codes_map(m, o.codes, o.rows, k, o.pitch, box);
   };
@@ -579,20 +699,19 @@ extern "C" int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, i
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int mode = p->rows_inner * 2 + q->rows_inner;
   if (pairs) {
-    if (pair_tiles > 0x7fffffffl) return -3;
-    args.tiles_p = (p->rows + 255) / 256;
-    args.tiles_q = (q->rows + 255) / 256;
+    if (plan.work() > 0) {
+      const size_t tickets = size_t(plan.tiles_p * plan.tiles_q - plan.whole) * 16 * sizeof(int);
+      if (!work) return -3;
+      args.part_sums = static_cast<float*>(work);
+      args.tickets = reinterpret_cast<int*>(static_cast<char*>(work) + plan.work() - tickets);
+      if (cudaMemsetAsync(args.tickets, 0, tickets, s) != cudaSuccess) return -5;
+    }
     args.idesc = make_idesc_mx(256, 256, p->code_type, q->code_type, p->rows_inner, q->rows_inner);
     return mode == 0 ? launch_pair<false, false>(tm_p, tm_q, args, s) : mode == 1 ? launch_pair<false, true>(tm_p, tm_q, args, s)
          : mode == 2 ? launch_pair<true, false>(tm_p, tm_q, args, s) : launch_pair<true, true>(tm_p, tm_q, args, s);
   }
-  args.tiles_p = (p->rows + 127) / 128;
-  args.tiles_q = (q->rows + n - 1) / n;
   args.idesc = make_idesc_mx(128, n, p->code_type, q->code_type, p->rows_inner, q->rows_inner);
-  const long tiles = long(args.tiles_p) * args.tiles_q;
-  if (tiles * kSplitMax > 0x7fffffffl) return -3;
-  const int groups = (args.n_kb + 3) / 4;
-  const int splits = int(std::max(1l, std::min({148 / tiles, long(groups), long(kSplitMax)})));
+  const int splits = plan.parts;
 #define DCPK_SPLIT(N, PM, QM, SLOT) launch_split<N, PM, QM>(tm_p, tm_q, args, splits, SLOT, s)
   if (q->rows_inner) return p->rows_inner ? DCPK_SPLIT(128, true, true, 4) : DCPK_SPLIT(128, false, true, 5);
   if (p->rows_inner)
