@@ -392,7 +392,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
 static constexpr int kSplitThreads = 256;   // TMA producer, UMMA issuer, 2 idle warps; 4 warps for scales, then results
 static constexpr int kSplitMax = 8;
 
-template <int kN> constexpr int split_stages() { return kN <= 32 ? 8 : 6; }
+template <int kN> constexpr int split_stages() { return kN <= 16 ? 11 : kN <= 32 ? 10 : kN <= 64 ? 8 : 6; }
 
 template <int kN>
 struct __align__(1024) SplitSmem {
@@ -442,8 +442,7 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
   constexpr int kScaleCol = 128;
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
   const int tp = tile % args.tiles_p, tq = tile / args.tiles_p;
-  // parts of k in whole groups of four blocks, so that a scale word belongs to one CTA
-  const int groups = (args.n_kb + 3) / 4, kb0 = 4 * (groups * rank / splits), kb1 = min(4 * (groups * (rank + 1) / splits), args.n_kb);
+  const int kb0 = args.n_kb * rank / splits, kb1 = args.n_kb * (rank + 1) / splits;   // a scale word may belong to two parts
   const int p0 = tp * 128, q0 = tq * kN;
 
   if (warp == 0) {
@@ -471,7 +470,7 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
       int stage = 0, ph = 0, buf = 0, sph = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if ((kb & 3) == 0) ok = mbar_wait(&sm.scale_full[buf], sph, abort_word);
+        if ((kb & 3) == 0 || kb == kb0) ok = mbar_wait(&sm.scale_full[buf], sph, abort_word);
         ok = ok && mbar_wait(&sm.full[stage], ph, abort_word);
         if (!ok) break;
         tc_fence_after();
@@ -500,8 +499,8 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
       next[0] = scale_word(args.p, p0 + t, kb, args.n_kb);
       next[1] = t < kN ? scale_word(args.q, q0 + t, kb, args.n_kb) : 0u;
     };
-    fetch(kb0);
-    for (int kb = kb0; kb < kb1; kb += 4) {
+    fetch(kb0 & ~3);
+    for (int kb = kb0 & ~3; kb < kb1; kb += 4) {
       uint32_t* words = sm.scales[turn];
       turn ^= 1;
       words[t] = next[0];
@@ -554,24 +553,27 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
   if (splits > 1) {
     __syncwarp();
     cluster_sync();
-    // every CTA adds up its share of the columns, in the order of k
-    if (warp >= 4 && !sm.abort_word) {
-      const int row = threadIdx.x & 127, p = p0 + row, n = min(kN, args.q.rows - q0);
-      const uint32_t at = smem_u32(&sm.part[0][row]);
+    // every CTA adds up its share of the columns, in the order of k: a warp has a column, a lane four neighbours of it
+    if (!sm.abort_word) {
+      const int n = min(kN, args.q.rows - q0), stop = n * (rank + 1) / splits, p = p0 + 4 * lane;
+      const uint32_t at = smem_u32(&sm.part[0][4 * lane]);
       by_output(args, [&](auto type, auto added) {
         using T = typename decltype(type)::T;
-        for (int c = n * rank / splits; c < n * (rank + 1) / splits; ++c) {
-          float v[kSplitMax];
+#pragma unroll 2
+        for (int c = n * rank / splits + warp; c < stop; c += kSplitThreads / 32) {
+          float4 v[kSplitMax];
 #pragma unroll
           for (int r = 0; r < kSplitMax; ++r)
-            if (r < splits) v[r] = __uint_as_float(ld_cluster_u32(at + c * 512, r));
-          float sum = v[0];
+            if (r < splits) v[r] = ld_cluster_f4(at + c * 512, r);
 #pragma unroll
           for (int r = 1; r < kSplitMax; ++r)
-            if (r < splits) sum += v[r];
-          if (p < args.p.rows)
-            store_result<decltype(added)::value>(static_cast<T*>(args.out) + size_t(q0 + c) * args.out_pitch + p,
-                                                 static_cast<const T*>(args.add) + size_t(q0 + c) * args.add_pitch + p, sum);
+            if (r < splits) { v[0].x += v[r].x; v[0].y += v[r].y; v[0].z += v[r].z; v[0].w += v[r].w; }
+          T* to = static_cast<T*>(args.out) + size_t(q0 + c) * args.out_pitch + p;
+          const T* from = static_cast<const T*>(args.add) + size_t(q0 + c) * args.add_pitch + p;
+          const float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (p + j < args.p.rows) store_result<decltype(added)::value>(to + j, from + j, f[j]);
         }
       });
     }
@@ -614,7 +616,7 @@ static int launch_split(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const 
   const int smem = int(sizeof(SplitSmem<kN>)) + 1024;
   auto kernel = fp8_gemm_split_kernel<kN, kPMn, kQMn>;
   if (raise_smem_limit(kernel, smem, g_gemm_smem_raised[slot]) != cudaSuccess) return -4;
-  const cudaError_t rc = launch_overlapped(kernel, dim3(args.tiles_p * args.tiles_q * splits), kSplitThreads, smem, stream, splits, false,
+  const cudaError_t rc = launch_overlapped(kernel, dim3(args.tiles_p * args.tiles_q * splits), kSplitThreads, smem, stream, splits, true,
                                            tm_p, tm_q, args, splits);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
@@ -649,7 +651,13 @@ static GemmPlan plan_gemm(long p_rows, long q_rows, bool q_rows_inner, int k, in
   g.tiles_p = (p_rows + 127) / 128;
   g.tiles_q = (q_rows + g.n - 1) / g.n;
   g.whole = 0;
-  g.parts = int(std::max(1l, std::min({148 / (g.tiles_p * g.tiles_q), long(groups), long(kSplitMax)})));
+  // as many parts as still are all under way at once: clusters of so many CTAs that fit the GPU's processors (one CTA per SM; by
+  // cudaOccupancyMaxActiveClusters).  A second round costs more than the shorter sums give: 17 x 6144 x 4096 in clusters of
+  // six, 48 of them, 16.5 us, in clusters of two 11.
+  constexpr int kFit[kSplitMax + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+  g.parts = 1;
+  for (int parts = 2; parts <= std::min(kSplitMax, (k + 127) / 128); ++parts)
+    if (g.tiles_p * g.tiles_q <= kFit[parts]) g.parts = parts;
   return g;
 }
 
