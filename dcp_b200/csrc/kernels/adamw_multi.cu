@@ -93,7 +93,7 @@ __device__ __forceinline__ void store_near(float* p, const float (&f)[8]) {
   st_global_v8(p, r);
 }
 template <typename T>
-__device__ __forceinline__ void store_near(T* p, const float (&f)[8]) { store8(p, f); }
+__device__ __forceinline__ void store_near(T* p, const float (&f)[8]) { store_raw(p, narrow<T>(f)); }
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, long e0, int lane, long n, bool vec, float (&f)[8]) {
@@ -155,11 +155,6 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, long e0, int lane, long
     for (int j = 0; j < 8; ++j)
       if (e0 + j * 32 + lane < n) p[e0 + j * 32 + lane] = uint8_t((j < 4 ? r.x : r.y) >> (8 * (j & 3)));
   }
-}
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {   // NaN if one is
-  float d;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 // Square root by one step of Newton's iteration with the residual of a fused product: to nearest but for one value in a
 // million, without sqrtf's branch for the ends of the range.  Zero for zero; below 2^-126 too small.

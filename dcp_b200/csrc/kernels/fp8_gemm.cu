@@ -607,7 +607,7 @@ static int launch_pair(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const G
   auto kernel = fp8_gemm_pair_kernel<kPMn, kQMn>;
   if (raise_smem_limit(kernel, smem, g_gemm_smem_raised[kPMn * 2 + kQMn]) != cudaSuccess) return -4;
   const int units = args.whole + (args.tiles_p * args.tiles_q - args.whole) * args.parts;
-  const cudaError_t rc = launch_overlapped(kernel, dim3(2 * std::min(units, kGemmPairs)), kGemmThreads, smem, stream, 1, false, tm_p, tm_q, args);
+  const cudaError_t rc = launch_overlapped(kernel, dim3(2 * std::min(units, kGemmPairs)), kGemmThreads, smem, stream, 1, args.tickets == nullptr, tm_p, tm_q, args);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 

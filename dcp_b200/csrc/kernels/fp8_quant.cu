@@ -7,9 +7,9 @@
 //  fp8_quantize    codes of a matrix with a scale per 1 x 128, 128 x 1 or 128 x 128 block, or both of the first two from one
 //                  pass: a CTA holds a tile of 128 x 128 in registers
 //
-// A thread has eight neighbouring channels in 16-byte accesses where rows begin on 16 bytes and hold a multiple of eight
-// values; otherwise every sixteenth channel of a block of 128, so that the 16 threads of a block still read and write
-// neighbours.
+// A thread has eight neighbouring channels (see fp8_common.cuh for rows that do not begin on 16 bytes), sixteen threads a
+// block of 128.  Packed arithmetic where there is some: with one instruction per value the norm of bf16 rows was bound by
+// issuing (27 instructions per value; 16384 x 4096 with a residual 89 us, fp32 rows of twice the bytes 135).
 #include <algorithm>
 
 #include "entries.h"
@@ -22,67 +22,9 @@ namespace dcpk {
 
 static constexpr int kBlock = 128;
 
-__device__ __forceinline__ int column(bool aligned, int chunk, int j) {
-  return aligned ? chunk * 8 + j : (chunk >> 4) * kBlock + j * 16 + (chunk & 15);
-}
-template <bool kAligned, typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int chunk, int width, float (&f)[8]) {
-  if (kAligned) {
-    if (chunk * 8 < width) {
-      Raw8<T> raw;
-      load_raw(raw, row + chunk * 8);
-      widen(raw, f);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = column(false, chunk, j);
-      f[j] = c < width ? to_float(row[c]) : 0.f;
-    }
-  }
-}
-template <typename T, bool kAligned>
-__device__ __forceinline__ void load_packed(const T* row, int chunk, int width, Raw8<T>& r) {
-  if (kAligned) {
-    if (chunk * 8 < width) load_raw(r, row + chunk * 8);
-    else r = Raw8<T>{};
-  } else {
-    T v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = column(false, chunk, j);
-      v[j] = c < width ? row[c] : from_float<T>(0.f);
-    }
-    r = *reinterpret_cast<const Raw8<T>*>(v);
-  }
-}
-template <bool kAligned, typename T>
-__device__ __forceinline__ void store_chunk(T* row, int chunk, int width, const float (&f)[8]) {
-  if (kAligned) {
-    if (chunk * 8 < width) store8(row + chunk * 8, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = column(false, chunk, j);
-      if (c < width) row[c] = from_float<T>(f[j]);
-    }
-  }
-}
-// rows of codes begin on 16 bytes in any case
-template <bool kAligned>
+// rows of codes begin on 16 bytes and have room for whole chunks
 __device__ __forceinline__ void store_codes(uint8_t* row, int chunk, int width, const uint2& codes) {
-  if (kAligned) {
-    if (chunk * 8 < width) *reinterpret_cast<uint2*>(row + chunk * 8) = codes;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = column(false, chunk, j);
-      if (c < width) row[c] = uint8_t((j < 4 ? codes.x : codes.y) >> (8 * (j & 3)));
-    }
-  }
+  if (chunk * 8 < width) *reinterpret_cast<uint2*>(row + chunk * 8) = codes;
 }
 __device__ __forceinline__ uint32_t max_of_16(uint32_t m) {
 #pragma unroll
@@ -114,44 +56,47 @@ fp8_norm_kernel(const T* __restrict__ x, long x_pitch, const T* __restrict__ res
   __shared__ float scratch[kNormThreads / 32];
   constexpr int kTop = kCode == kCodeE4m3 ? 8 : 15;
   const long row = blockIdx.x;
-  float v[kVecs][8];
-  float ss = 0.f;
+  Raw8<T> v[kVecs];
   grid_wait();
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) load_chunk<kAligned>(x + row * x_pitch, threadIdx.x + i * blockDim.x, width, v[i]);
   if (residual) {
+    // the sum goes on in x's type: what the norm sees is what the next layer adds to
+    Raw8<T> r[kVecs];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) load_chunk<kAligned>(residual + row * residual_pitch, threadIdx.x + i * blockDim.x, width, r[i]);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      float r[8];
-      const int chunk = threadIdx.x + i * blockDim.x;
-      load_chunk<kAligned>(residual + row * residual_pitch, chunk, width, r);
-      // the sum goes on in x's type: what the norm sees is what the next layer adds to
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = to_float(from_float<T>(v[i][j] + r[j]));
-      store_chunk<kAligned>(h + row * width, chunk, width, v[i]);
+      v[i] = add_raw(v[i], r[i]);
+      store_chunk<kAligned>(h + row * width, threadIdx.x + i * blockDim.x, width, v[i]);
     }
   }
   grid_let_next();
+  uint64_t ss2[2] = {0ull, 0ull};
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i)
+  for (int i = 0; i < kVecs; ++i) {
+    uint64_t f[4];
+    widen(v[i], f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
-  ss = row_sum(ss, scratch, blockDim.x >> 5);
-  const float r = rsqrtf(ss / width + eps);
+    for (int j = 0; j < 4; ++j) ss2[j & 1] = fma_f32x2(f[j], f[j], ss2[j & 1]);
+  }
+  float lo, hi;
+  unpack_f32x2(add_f32x2(ss2[0], ss2[1]), lo, hi);
+  const float r = rsqrtf(row_sum(lo + hi, scratch, blockDim.x >> 5) / width + eps);
   if (threadIdx.x == 0) rstd[row] = r;
+  const uint64_t r2 = pack_f32x2(r, r);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int chunk = threadIdx.x + i * blockDim.x;
-    float g[8];
-    uint32_t amax = 0;
-    load_chunk<kAligned>(w, chunk, width, g);
+    Raw8<T> wr;
+    uint64_t f[4], g[4];
+    load_chunk<kAligned>(w, chunk, width, wr);
+    widen(v[i], f);
+    widen(wr, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[i][j] = v[i][j] * r * g[j];
-      amax = amax_bits(amax, v[i][j]);
-    }
-    const int byte = scale_byte<kTop>(max_of_16(amax));
-    store_codes<kAligned>(codes + row * code_pitch, chunk, width, to_codes8<kCode>(v[i], scale_inverse(byte)));
+    for (int j = 0; j < 4; ++j) f[j] = mul_f32x2(mul_f32x2(f[j], r2), g[j]);
+    const int byte = scale_byte<kTop>(max_of_16(amax_bits(f)));
+    store_codes(codes + row * code_pitch, chunk, width, to_codes8<kCode>(f, scale_inverse(byte)));
     if ((chunk & 15) == 0 && chunk * 8 < width) scales[row * scale_pitch + (chunk >> 4)] = uint8_t(byte);
   }
 }
@@ -173,7 +118,7 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
   extern __shared__ __align__(128) uint8_t ring[];
   constexpr bool kAligned = kRing;
   const uint32_t row_bytes = uint32_t(width) * sizeof(T), stage_bytes = row_bytes * (kAdd ? 3 : 2);
-  float dw[kVecs][8];
+  uint64_t dw[kVecs][4];
   Raw8<T> wv[kVecs];
   if (kRing) {
     if (threadIdx.x == 0) {
@@ -196,15 +141,16 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
     for (int i = 0; i < stages; ++i) fetch(blockIdx.x + long(i) * gridDim.x, i);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    load_packed<T, kAligned>(w, threadIdx.x + i * blockDim.x, width, wv[i]);
+    load_chunk<kAligned>(w, threadIdx.x + i * blockDim.x, width, wv[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) dw[i][j] = 0ull;
   }
   int turn = 0, stage = 0, parity = 0;
   bool ok = true;
   for (long row = blockIdx.x; row < n_rows; row += gridDim.x, turn ^= 1) {
     const float r = rstd[row];
-    float xh[kVecs][8], g[kVecs][8];
+    const uint64_t r2 = pack_f32x2(r, r);
+    uint64_t xh[kVecs][4], g[kVecs][4];
     const T *hr = h + row * h_pitch, *gr = dy + row * dy_pitch, *ar = add + row * add_pitch;
     if (kRing) {
       ok = ok && mbar_wait(&full[stage], parity, &abort_word);
@@ -212,46 +158,63 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
       gr = hr + width;
       ar = gr + width;
     }
-    float dot = 0.f;
+    uint64_t dot2[2] = {0ull, 0ull};
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int chunk = threadIdx.x + i * blockDim.x;
-      float wf[8];
-      load_chunk<kAligned>(hr, chunk, width, xh[i]);
-      load_chunk<kAligned>(gr, chunk, width, g[i]);
+      Raw8<T> raw;
+      uint64_t wf[4];
+      load_chunk<kAligned>(hr, chunk, width, raw);
+      widen(raw, xh[i]);
+      load_chunk<kAligned>(gr, chunk, width, raw);
+      widen(raw, g[i]);
       widen(wv[i], wf);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        xh[i][j] *= r;
-        dw[i][j] += g[i][j] * xh[i][j];
-        g[i][j] *= wf[j];
-        dot += g[i][j] * xh[i][j];
+      for (int j = 0; j < 4; ++j) {
+        xh[i][j] = mul_f32x2(xh[i][j], r2);
+        dw[i][j] = fma_f32x2(g[i][j], xh[i][j], dw[i][j]);
+        g[i][j] = mul_f32x2(g[i][j], wf[j]);
+        dot2[j & 1] = fma_f32x2(g[i][j], xh[i][j], dot2[j & 1]);
       }
     }
-    dot = row_sum(dot, scratch[turn], blockDim.x >> 5) / width;   // alternating scratch: one barrier per row
+    float lo, hi;
+    unpack_f32x2(add_f32x2(dot2[0], dot2[1]), lo, hi);
+    const float dot = row_sum(lo + hi, scratch[turn], blockDim.x >> 5) / width;   // alternating scratch: one barrier per row
     if (kRing) {
       // all are through with the row before: its stage is free
       const int before = stage == 0 ? stages - 1 : stage - 1;
       if (threadIdx.x == 0 && row != blockIdx.x) fetch(row + long(stages - 1) * gridDim.x, before);
       if (++stage == stages) { stage = 0; parity ^= 1; }
     }
+    const uint64_t minus = pack_f32x2(-dot, -dot);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int chunk = threadIdx.x + i * blockDim.x;
-      float a[8];
-      if (kAdd) load_chunk<kAligned>(ar, chunk, width, a);
+      uint64_t a[4] = {0ull, 0ull, 0ull, 0ull};
+      if (kAdd) {
+        Raw8<T> raw;
+        load_chunk<kAligned>(ar, chunk, width, raw);
+        widen(raw, a);
+      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[i][j] = r * (g[i][j] - xh[i][j] * dot) + (kAdd ? a[j] : 0.f);
-      store_chunk<kAligned>(dx + row * width, chunk, width, g[i]);
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t t = fma_f32x2(xh[i][j], minus, g[i][j]);
+        g[i][j] = kAdd ? fma_f32x2(t, r2, a[j]) : mul_f32x2(t, r2);
+      }
+      store_chunk<kAligned>(dx + row * width, chunk, width, narrow<T>(g[i]));
     }
   }
   grid_let_next();
 #pragma unroll
   for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = column(kAligned, threadIdx.x + i * blockDim.x, j);
-      if (c < width) part[size_t(blockIdx.x) * width + c] = dw[i][j];
+    for (int j = 0; j < 4; ++j) {
+      const int c = (threadIdx.x + i * blockDim.x) * 8 + 2 * j;
+      float lo, hi;
+      unpack_f32x2(dw[i][j], lo, hi);
+      float* to = part + size_t(blockIdx.x) * width + c;
+      if (c < width) to[0] = lo;
+      if (c + 1 < width) to[1] = hi;
     }
   if (kRing && !ok) {   // copies under way get a millisecond to land
     atomicExch(status, kStatusBarrierTimeout);
@@ -287,16 +250,14 @@ struct QuantizeOut {
 
 // Eight values as they lie in memory and their magnitudes, two to a word in 16-bit types: magnitudes order like their bits
 // there too, so one instruction masks two and one compares two.
-template <typename T> struct Magnitudes { uint32_t m[4]; };
-template <> struct Magnitudes<float> { uint32_t m[8]; };
+template <typename T> struct Magnitudes { uint32_t m[kWordsOf<T>]; };
 
 template <typename T>
 __device__ __forceinline__ Magnitudes<T> magnitudes(const Raw8<T>& r) {
   constexpr uint32_t kMask = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
   Magnitudes<T> m;
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
 #pragma unroll
-  for (int i = 0; i < int(sizeof(m) / 4); ++i) m.m[i] = w[i] & kMask;
+  for (int i = 0; i < kWordsOf<T>; ++i) m.m[i] = r.w[i] & kMask;
   return m;
 }
 template <typename T>
@@ -332,7 +293,7 @@ fp8_quantize_kernel(const T* __restrict__ x, long pitch, QuantizeOut by_rows, Qu
     const T* p = x + row0 * pitch;
 #pragma unroll
     for (int i = 0; i < 8; ++i, p += 16 * pitch) {
-      if (16 * i < rows_left) load_packed<T, kAligned>(p, chunk, width, v[i]);
+      if (16 * i < rows_left) load_chunk<kAligned>(p, chunk, width, v[i]);
       else v[i] = Raw8<T>{};
     }
   }
@@ -355,7 +316,7 @@ fp8_quantize_kernel(const T* __restrict__ x, long pitch, QuantizeOut by_rows, Qu
 #pragma unroll
       for (int i = 0; i < 16; ++i) amax = larger<T>(amax, column_max[i][t + 16 * (j / kPer)]);
       if (sizeof(T) == 2) amax = j & 1 ? amax >> 16 : amax & 0xffffu;
-      const int byte = scale_byte<kTop>(as_float_bits<T>(amax)), c = tile_x * kBlock + column(kAligned, t, j);
+      const int byte = scale_byte<kTop>(as_float_bits<T>(amax)), c = tile_x * kBlock + t * 8 + j;
       if (c < width) by_cols.scales[c * by_cols.scale_pitch + tile_y] = uint8_t(byte);
       column_inv[t + 16 * j] = scale_inverse(byte);
     }
@@ -387,9 +348,9 @@ fp8_quantize_kernel(const T* __restrict__ x, long pitch, QuantizeOut by_rows, Qu
       for (int h = 0; h < 2; ++h, to += 16 * by_rows.pitch, scale += 16 * by_rows.scale_pitch) {
         if (16 * (i + h) >= rows_left) continue;
         const int byte = scale_byte<kTop>(as_float_bits<T>(m[h]));
-        float f[8];
+        uint64_t f[4];
         widen(v[i + h], f);
-        store_codes<kAligned>(to, chunk, width, to_codes8<kCode>(f, scale_inverse(byte)));
+        store_codes(to, chunk, width, to_codes8<kCode>(f, scale_inverse(byte)));
         if (tx == 0) *scale = uint8_t(byte);
       }
     }
@@ -415,26 +376,24 @@ fp8_quantize_kernel(const T* __restrict__ x, long pitch, QuantizeOut by_rows, Qu
 #pragma unroll
     for (int i = 0; i < 8; ++i, to += 16 * by_rows.pitch) {
       if (16 * i >= rows_left) continue;
-      float f[8];
+      uint64_t f[4];
       widen(v[i], f);
-      store_codes<kAligned>(to, chunk, width, to_codes8<kCode>(f, inv));
+      store_codes(to, chunk, width, to_codes8<kCode>(f, inv));
     }
     if (threadIdx.x == 0) by_rows.scales[tile_y * by_rows.scale_pitch + tile_x] = uint8_t(byte);
   }
   if (kWays & kCols) {
     __syncthreads();
-    float inv[8];
+    uint64_t inv[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) inv[j] = column_inv[tx + 16 * j];
+    for (int j = 0; j < 4; ++j) inv[j] = pack_f32x2(column_inv[tx + 32 * j], column_inv[tx + 32 * j + 16]);
     uint8_t* to = by_cols.codes + row0 * by_cols.pitch;
 #pragma unroll
     for (int i = 0; i < 8; ++i, to += 16 * by_cols.pitch) {
       if (16 * i >= rows_left) continue;
-      float f[8];
+      uint64_t f[4];
       widen(v[i], f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= inv[j];
-      store_codes<kAligned>(to, chunk, width, to_codes8<kCode>(f, 1.f));
+      store_codes(to, chunk, width, to_codes8<kCode>(f, inv));
     }
   }
 }
@@ -471,7 +430,7 @@ extern "C" int dcpk_fp8_norm(int type, int code, const void* x, long x_pitch, co
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     const auto launch = [&](auto kernel) {
       const cudaError_t rc = launch_overlapped(
-          kernel, dim3(unsigned(n_rows)), threads_for(width, vecs), 0, static_cast<cudaStream_t>(stream), 1, false, static_cast<const T*>(x),
+          kernel, dim3(unsigned(n_rows)), threads_for(width, vecs), 0, static_cast<cudaStream_t>(stream), 1, true, static_cast<const T*>(x),
           x_pitch, static_cast<const T*>(residual), residual_pitch, static_cast<const T*>(w), static_cast<T*>(h), static_cast<uint8_t*>(codes),
           code_pitch, static_cast<uint8_t*>(scales), scale_pitch, rstd, width, eps);
       return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
@@ -517,7 +476,7 @@ extern "C" int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const vo
     const auto launch = [&](auto kernel, int slot) {
       const int smem = ring ? stages * stage_bytes : 0;
       if (smem > 48 * 1024 - 512 && raise_smem_limit(kernel, kRingBytes, g_ring_raised[slot]) != cudaSuccess) return -4;
-      const cudaError_t rc = launch_overlapped(kernel, dim3(ctas), threads_for(width, vecs), smem, s, 1, false, static_cast<const T*>(h), h_pitch,
+      const cudaError_t rc = launch_overlapped(kernel, dim3(ctas), threads_for(width, vecs), smem, s, 1, true, static_cast<const T*>(h), h_pitch,
                                                static_cast<const T*>(w), rstd, static_cast<const T*>(dy), dy_pitch, static_cast<const T*>(add),
                                                add_pitch, static_cast<T*>(dx), part, int(n_rows), width, stages, status);
       return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
@@ -552,7 +511,7 @@ extern "C" int dcpk_fp8_quantize(int type, int code, int ways, const void* x, lo
   return by_type(type, [&](auto* t) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     const auto launch = [&](auto kernel) {
-      const cudaError_t rc = launch_overlapped(kernel, dim3(unsigned(tiles)), 256, 0, static_cast<cudaStream_t>(stream), 1, false,
+      const cudaError_t rc = launch_overlapped(kernel, dim3(unsigned(tiles)), 256, 0, static_cast<cudaStream_t>(stream), 1, true,
                                                static_cast<const T*>(x), pitch, a, b, int(n_rows), width, int(tiles_x));
       return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
     };
