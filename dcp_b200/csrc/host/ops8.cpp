@@ -119,7 +119,7 @@ Tensors norm8_bwd(const Tensor& h, const Tensor& w, const Tensor& rstd, const Te
   const long rows = h.size(0), width = h.size(1);
   const auto f32 = h.options().dtype(at::kFloat);
   Tensor dx = at::empty({rows, width}, h.options()), dw = at::empty({width}, f32);
-  const Tensor part = at::empty({dcpk_fp8_norm_bwd_parts(rows, int(width)), width}, f32);
+  const Tensor part = at::empty({dcpk_fp8_norm_bwd_parts(value_type(h.scalar_type()), rows, int(width), add.has_value()), width}, f32);
   check(dcpk_fp8_norm_bwd(value_type(h.scalar_type()), h.const_data_ptr(), pitch(h), w.const_data_ptr(), rstd.const_data_ptr<float>(),
                           dy.const_data_ptr(), pitch(dy), add ? add->const_data_ptr() : nullptr, add ? pitch(*add) : 0, dx.data_ptr(),
                           dw.data_ptr<float>(), part.data_ptr<float>(), rows, int(width), status.data_ptr<int>(), stream()),

@@ -27,7 +27,7 @@ int dcpk_fp8_quantize(int type, int code, int ways, const void* x, long pitch, v
                       void* codes_b, long pitch_b, void* scales_b, long scale_pitch_b, long n_rows, int width, void* stream);
 int dcpk_fp8_norm(int type, int code, const void* x, long x_pitch, const void* residual, long residual_pitch, const void* w, void* h, void* codes,
                   long code_pitch, void* scales, long scale_pitch, float* rstd, long n_rows, int width, float eps, void* stream);
-int dcpk_fp8_norm_bwd_parts(long n_rows, int width);
+int dcpk_fp8_norm_bwd_parts(int type, long n_rows, int width, int add);
 int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const void* w, const float* rstd, const void* dy, long dy_pitch, const void* add,
                       long add_pitch, void* dx, float* dw, float* part, long n_rows, int width, int* status, void* stream);
 int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, int k, void* out, long out_pitch, const void* add, long add_pitch,

@@ -186,7 +186,8 @@ __device__ __forceinline__ void shift_words(uint32_t (&w)[kWords], uint32_t byte
     for (int i = 0; i + 1 < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
 }
 // Values 8 chunk .. 8 chunk + 7 of a row of `width`, zeros behind its end.  Unaligned ones come in the aligned pieces of 16
-// bytes that hold some of them, of which neighbouring threads share one: one and a quarter accesses instead of eight.
+// bytes that hold some of them (so none lies outside the memory they were allocated in, which begins and ends on more than
+// 16), of which neighbouring threads share one: two accesses instead of eight.
 template <bool kAligned, typename T>
 __device__ __forceinline__ void load_chunk(const T* row, int chunk, int width, Raw8<T>& r) {
   const int n = width - chunk * 8;

@@ -31,16 +31,17 @@ __device__ __forceinline__ uint32_t max_of_16(uint32_t m) {
   for (int s = 8; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
   return m;
 }
-__device__ __forceinline__ float row_sum(float v, float* scratch, int warps) {
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = lane < warps ? scratch[lane] : 0.f;
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
   return v;
+}
+__device__ __forceinline__ float row_sum(float v, float* scratch, int warps) {
+  v = lanes_sum(v);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return lanes_sum(lane < warps ? scratch[lane] : 0.f);
 }
 
 static constexpr int kNormThreads = 512;
@@ -48,27 +49,31 @@ static constexpr int kNormWidth = 16384;   // four chunks of eight channels per 
 static constexpr int kMaxStages = 8;       // rows under way in the backward pass
 static constexpr int kRingBytes = 200 * 1024;   // of an SM's shared memory, for all its CTAs
 
-template <typename T, int kVecs, bool kAligned, int kCode>
+// kWarps: a row per warp, eight to a CTA, where a row's chunks are few: no barrier, and a CTA per row of 512 channels is bound by
+// the CTAs' coming and going (65536 rows with a residual 70 us).
+template <typename T, int kVecs, bool kAligned, int kCode, bool kWarps>
 __global__ void __launch_bounds__(kNormThreads)
 fp8_norm_kernel(const T* __restrict__ x, long x_pitch, const T* __restrict__ residual, long residual_pitch, const T* __restrict__ w,
                 T* __restrict__ h, uint8_t* __restrict__ codes, long code_pitch, uint8_t* __restrict__ scales, long scale_pitch,
-                float* __restrict__ rstd, int width, float eps) {
+                float* __restrict__ rstd, int n_rows, int width, float eps) {
   __shared__ float scratch[kNormThreads / 32];
   constexpr int kTop = kCode == kCodeE4m3 ? 8 : 15;
-  const long row = blockIdx.x;
+  const long row = kWarps ? long(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (kWarps && row >= n_rows) return;
+  const int first = kWarps ? threadIdx.x & 31 : threadIdx.x, step = kWarps ? 32 : blockDim.x;
   Raw8<T> v[kVecs];
   grid_wait();
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) load_chunk<kAligned>(x + row * x_pitch, threadIdx.x + i * blockDim.x, width, v[i]);
+  for (int i = 0; i < kVecs; ++i) load_chunk<kAligned>(x + row * x_pitch, first + i * step, width, v[i]);
   if (residual) {
     // the sum goes on in x's type: what the norm sees is what the next layer adds to
     Raw8<T> r[kVecs];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) load_chunk<kAligned>(residual + row * residual_pitch, threadIdx.x + i * blockDim.x, width, r[i]);
+    for (int i = 0; i < kVecs; ++i) load_chunk<kAligned>(residual + row * residual_pitch, first + i * step, width, r[i]);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       v[i] = add_raw(v[i], r[i]);
-      store_chunk<kAligned>(h + row * width, threadIdx.x + i * blockDim.x, width, v[i]);
+      store_chunk<kAligned>(h + row * width, first + i * step, width, v[i]);
     }
   }
   grid_let_next();
@@ -82,12 +87,12 @@ fp8_norm_kernel(const T* __restrict__ x, long x_pitch, const T* __restrict__ res
   }
   float lo, hi;
   unpack_f32x2(add_f32x2(ss2[0], ss2[1]), lo, hi);
-  const float r = rsqrtf(row_sum(lo + hi, scratch, blockDim.x >> 5) / width + eps);
-  if (threadIdx.x == 0) rstd[row] = r;
+  const float r = rsqrtf((kWarps ? lanes_sum(lo + hi) : row_sum(lo + hi, scratch, blockDim.x >> 5)) / width + eps);
+  if (first == 0) rstd[row] = r;
   const uint64_t r2 = pack_f32x2(r, r);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int chunk = threadIdx.x + i * blockDim.x;
+    const int chunk = first + i * step;
     Raw8<T> wr;
     uint64_t f[4], g[4];
     load_chunk<kAligned>(w, chunk, width, wr);
@@ -104,10 +109,10 @@ fp8_norm_kernel(const T* __restrict__ x, long x_pitch, const T* __restrict__ res
 // Persistent CTAs: each walks rows blockIdx.x, + gridDim.x, ... and keeps its part of dW in registers; the parts go to
 // `part` [gridDim.x, width], which a second kernel adds up in order: the same bits in every run.
 //
-// kRing (rows on 16 bytes): the rows of h, dy and add come by bulk copies into a ring of `stages` rows in shared memory, so
+// kRing: the rows of h, dy and add come by bulk copies into a ring of `stages` rows in shared memory, so
 // that what is under way does not depend on the registers; the barrier inside the row's sum is also what frees the stage.
 // With plain loads at the beginning of a row 5003 rows of 5120 took 62 us (2.9 TB/s).
-template <typename T, int kVecs, bool kRing, bool kAdd>
+template <typename T, int kVecs, bool kAligned, bool kRing, bool kAdd>
 __global__ void __launch_bounds__(kVecs == 1 ? 1024 : kVecs == 2 ? 768 : 512)   // 64, 80 and 128 registers
 fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__ w, const float* __restrict__ rstd, const T* __restrict__ dy,
                     long dy_pitch, const T* __restrict__ add, long add_pitch, T* __restrict__ dx, float* __restrict__ part, int n_rows,
@@ -116,8 +121,10 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
   __shared__ uint64_t full[kMaxStages];
   __shared__ int abort_word;
   extern __shared__ __align__(128) uint8_t ring[];
-  constexpr bool kAligned = kRing;
-  const uint32_t row_bytes = uint32_t(width) * sizeof(T), stage_bytes = row_bytes * (kAdd ? 3 : 2);
+  // a row in the ring: the aligned pieces of 16 bytes that hold some of it, from its offset in the first on
+  const uint32_t row_bytes = uint32_t(width) * sizeof(T), slot_bytes = kAligned ? row_bytes : (row_bytes + 45) & ~15u,
+                 stage_bytes = slot_bytes * (kAdd ? 3 : 2);
+  const auto past = [](const T* p) { return uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u; };
   uint64_t dw[kVecs][4];
   Raw8<T> wv[kVecs];
   if (kRing) {
@@ -131,11 +138,14 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
   grid_wait();
   const auto fetch = [&](long row, int stage) {   // by one thread
     if (row >= n_rows) return;
-    uint8_t* to = ring + size_t(stage) * stage_bytes;
-    mbar_expect_tx(&full[stage], stage_bytes);
-    bulk_load(to, h + row * h_pitch, row_bytes, &full[stage]);
-    bulk_load(to + row_bytes, dy + row * dy_pitch, row_bytes, &full[stage]);
-    if (kAdd) bulk_load(to + 2 * row_bytes, add + row * add_pitch, row_bytes, &full[stage]);
+    const T* from[3] = {h + row * h_pitch, dy + row * dy_pitch, add + row * add_pitch};
+    uint32_t bytes[3], total = 0;
+#pragma unroll
+    for (int i = 0; i < (kAdd ? 3 : 2); ++i) total += bytes[i] = kAligned ? row_bytes : (past(from[i]) + row_bytes + 15) & ~15u;
+    mbar_expect_tx(&full[stage], total);
+#pragma unroll
+    for (int i = 0; i < (kAdd ? 3 : 2); ++i)
+      bulk_load(ring + size_t(stage) * stage_bytes + i * slot_bytes, reinterpret_cast<const uint8_t*>(from[i]) - past(from[i]), bytes[i], &full[stage]);
   };
   if (kRing && threadIdx.x == 0)
     for (int i = 0; i < stages; ++i) fetch(blockIdx.x + long(i) * gridDim.x, i);
@@ -154,9 +164,10 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
     const T *hr = h + row * h_pitch, *gr = dy + row * dy_pitch, *ar = add + row * add_pitch;
     if (kRing) {
       ok = ok && mbar_wait(&full[stage], parity, &abort_word);
-      hr = reinterpret_cast<const T*>(ring + size_t(stage) * stage_bytes);
-      gr = hr + width;
-      ar = gr + width;
+      const uint8_t* at = ring + size_t(stage) * stage_bytes;
+      hr = reinterpret_cast<const T*>(at + past(hr));
+      gr = reinterpret_cast<const T*>(at + slot_bytes + past(gr));
+      ar = reinterpret_cast<const T*>(at + 2 * slot_bytes + past(ar));
     }
     uint64_t dot2[2] = {0ull, 0ull};
 #pragma unroll
@@ -422,23 +433,33 @@ extern "C" int dcpk_fp8_norm(int type, int code, const void* x, long x_pitch, co
   if (width <= 0 || width > kNormWidth || n_rows > 0x7fffffffl || (code != kCodeE4m3 && code != kCodeE5m2)) return -3;
   const bool aligned = width % 8 == 0 && x_pitch % 8 == 0 && on_16(x) && on_16(w) && (!residual || (residual_pitch % 8 == 0 && on_16(residual) && on_16(h))) &&
                        code_pitch % 16 == 0 && on_16(codes);
-  // few rows: as many threads per row as it takes, for the shortest chain
+  // Rows of up to 1024 channels: a warp each (up to 256 where they do not begin on 16 bytes: 16384 x 1001 45 us against 38).  Few longer rows: as many threads per row as it takes, for the shortest chain.
+  const bool warps = width <= (aligned ? 1024 : 256);
   int vecs = n_rows <= 148 * 2 ? 1 : 4;
   while (vecs > 1 && threads_for(width, vecs) < 64) vecs >>= 1;
   while (threads_for(width, vecs) > kNormThreads) vecs <<= 1;
+  if (warps) {
+    vecs = 1;
+    while (threads_for(width, vecs) > 32) vecs <<= 1;
+  }
+  const unsigned ctas = unsigned(warps ? (n_rows + 7) / 8 : n_rows), threads = warps ? 256 : threads_for(width, vecs);
   return by_type(type, [&](auto* t) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     const auto launch = [&](auto kernel) {
       const cudaError_t rc = launch_overlapped(
-          kernel, dim3(unsigned(n_rows)), threads_for(width, vecs), 0, static_cast<cudaStream_t>(stream), 1, true, static_cast<const T*>(x),
+          kernel, dim3(ctas), threads, 0, static_cast<cudaStream_t>(stream), 1, true, static_cast<const T*>(x),
           x_pitch, static_cast<const T*>(residual), residual_pitch, static_cast<const T*>(w), static_cast<T*>(h), static_cast<uint8_t*>(codes),
-          code_pitch, static_cast<uint8_t*>(scales), scale_pitch, rstd, width, eps);
+          code_pitch, static_cast<uint8_t*>(scales), scale_pitch, rstd, int(n_rows), width, eps);
       return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
     };
     const auto sized = [&](auto al, auto c) {
       constexpr bool A = decltype(al)::value;
       constexpr int C = decltype(c)::value;
-      return vecs == 1 ? launch(fp8_norm_kernel<T, 1, A, C>) : vecs == 2 ? launch(fp8_norm_kernel<T, 2, A, C>) : launch(fp8_norm_kernel<T, 4, A, C>);
+      if (warps)
+        return vecs == 1 ? launch(fp8_norm_kernel<T, 1, A, C, true>) : vecs == 2 ? launch(fp8_norm_kernel<T, 2, A, C, true>)
+                                                                                : launch(fp8_norm_kernel<T, 4, A, C, true>);
+      return vecs == 1 ? launch(fp8_norm_kernel<T, 1, A, C, false>) : vecs == 2 ? launch(fp8_norm_kernel<T, 2, A, C, false>)
+                                                                               : launch(fp8_norm_kernel<T, 4, A, C, false>);
     };
     const auto coded = [&](auto al) {
       return code == kCodeE4m3 ? sized(al, std::integral_constant<int, kCodeE4m3>()) : sized(al, std::integral_constant<int, kCodeE5m2>());
@@ -447,14 +468,19 @@ extern "C" int dcpk_fp8_norm(int type, int code, const void* x, long x_pitch, co
   });
 }
 
-// CTAs of the backward pass, which is also how many rows of `width` floats `part` has.  As many threads to an SM as the
-// registers allow at two chunks each.
-static int norm_bwd_per_sm(int width) { return std::max(1, std::min(8, 768 / threads_for(width, 2))); }
-extern "C" int dcpk_fp8_norm_bwd_parts(long n_rows, int width) {
-  return int(std::max(1l, std::min(n_rows, 148l * norm_bwd_per_sm(width))));
+// CTAs of the backward pass to an SM: as many threads as the registers allow at two chunks each, with three rows under way per
+// CTA (16384 x 4096 in fp32 with three CTAs and no room for a ring 224 us, with one 152; bf16 with three CTAs of two rows 85, with
+// two of four 80).  Two rows where they do not begin on 16 bytes, which takes more threads' work (fp32 one CTA 374 us, two 228).
+static int norm_bwd_per_sm(int type, int width, bool add) {
+  const int row = width * (type == kTypeF32 ? 4 : 2) + 45, rows = (width % 8 ? 2 : 3) * (add ? 3 : 2);
+  return std::max(1, std::min({8, 768 / threads_for(width, 2), kRingBytes / (rows * row)}));
+}
+// CTAs in all, which is also how many rows of `width` floats `part` has
+extern "C" int dcpk_fp8_norm_bwd_parts(int type, long n_rows, int width, int add) {
+  return int(std::max(1l, std::min(n_rows, 148l * norm_bwd_per_sm(type, width, add))));
 }
 
-static std::atomic<uint64_t> g_ring_raised[18];
+static std::atomic<uint64_t> g_ring_raised[36];
 
 // dx [n_rows, width]; dw fp32 [width], written; add: null, or what is added to dx
 extern "C" int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const void* w, const float* rstd, const void* dy, long dy_pitch,
@@ -465,14 +491,14 @@ extern "C" int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const vo
   if (n_rows == 0) return cudaMemsetAsync(dw, 0, size_t(width) * 4, s) == cudaSuccess ? 0 : -5;
   const bool aligned = width % 8 == 0 && h_pitch % 8 == 0 && dy_pitch % 8 == 0 && on_16(h) && on_16(w) && on_16(dy) && on_16(dx) &&
                        (!add || (add_pitch % 8 == 0 && on_16(add)));
-  const int ctas = dcpk_fp8_norm_bwd_parts(n_rows, width);
+  const int ctas = dcpk_fp8_norm_bwd_parts(type, n_rows, width, add != nullptr);
   int vecs = threads_for(width, 2) <= 256 && threads_for(width, 1) <= 128 ? 1 : 2;
   while (threads_for(width, vecs) > kNormThreads) vecs <<= 1;
   const int rc = by_type(type, [&](auto* t) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-    const int stage_bytes = width * int(sizeof(T)) * (add ? 3 : 2);
-    const int stages = std::min(kMaxStages, kRingBytes / norm_bwd_per_sm(width) / stage_bytes);
-    const bool ring = aligned && stages >= 2;
+    const int row_bytes = width * int(sizeof(T)), stage_bytes = (aligned ? row_bytes : (row_bytes + 45) & ~15) * (add ? 3 : 2);
+    const int stages = std::min(kMaxStages, kRingBytes / norm_bwd_per_sm(type, width, add != nullptr) / stage_bytes);
+    const bool ring = stages >= 2;   // not for long rows of fp32
     const auto launch = [&](auto kernel, int slot) {
       const int smem = ring ? stages * stage_bytes : 0;
       if (smem > 48 * 1024 - 512 && raise_smem_limit(kernel, kRingBytes, g_ring_raised[slot]) != cudaSuccess) return -4;
@@ -481,14 +507,14 @@ extern "C" int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const vo
                                                add_pitch, static_cast<T*>(dx), part, int(n_rows), width, stages, status);
       return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
     };
-    const auto sized = [&](auto al, auto ad) {
-      constexpr bool A = decltype(al)::value, D = decltype(ad)::value;
-      constexpr int base = (std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 6 : 12) + D * 3;
-      return vecs == 1 ? launch(fp8_norm_bwd_kernel<T, 1, A, D>, base) : vecs == 2 ? launch(fp8_norm_bwd_kernel<T, 2, A, D>, base + 1)
-                                                                                  : launch(fp8_norm_bwd_kernel<T, 4, A, D>, base + 2);
+    const auto sized = [&](auto al, auto ri, auto ad) {
+      constexpr bool A = decltype(al)::value, R = decltype(ri)::value, D = decltype(ad)::value;
+      constexpr int base = (std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 12 : 24) + (A * 2 + D) * 3;
+      return vecs == 1 ? launch(fp8_norm_bwd_kernel<T, 1, A, R, D>, base) : vecs == 2 ? launch(fp8_norm_bwd_kernel<T, 2, A, R, D>, base + 1)
+                                                                                     : launch(fp8_norm_bwd_kernel<T, 4, A, R, D>, base + 2);
     };
-    const auto added = [&](auto al) { return add ? sized(al, std::true_type()) : sized(al, std::false_type()); };
-    return ring ? added(std::true_type()) : added(std::false_type());
+    const auto added = [&](auto al, auto ri) { return add ? sized(al, ri, std::true_type()) : sized(al, ri, std::false_type()); };
+    return !ring ? added(std::false_type(), std::false_type()) : aligned ? added(std::true_type(), std::true_type()) : added(std::false_type(), std::true_type());
   });
   if (rc) return rc;
   const cudaError_t rc2 = launch_overlapped(fp8_norm_dw_kernel, dim3((width + 31) / 32), 256, 0, s, 1, true, static_cast<const float*>(part), dw, ctas, width);
