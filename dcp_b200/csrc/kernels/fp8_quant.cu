@@ -233,22 +233,20 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
   }
 }
 
-// 32 columns per CTA, eight threads of a column take every eighth of the parts
-__global__ void __launch_bounds__(256) fp8_norm_dw_kernel(const float* __restrict__ part, float* __restrict__ dw, int n, int width) {
-  __shared__ float sums[8][32];
+// 32 columns per CTA, 32 threads of a column take every 32nd of the parts
+__global__ void __launch_bounds__(1024) fp8_norm_dw_kernel(const float* __restrict__ part, float* __restrict__ dw, int n, int width) {
+  __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
   grid_wait();
   if (c < width)
 #pragma unroll 8
-    for (int i = group; i < n; i += 8) s += part[size_t(i) * width + c];
+    for (int i = group; i < n; i += 32) s += part[size_t(i) * width + c];
   sums[group][lane] = s;
   __syncthreads();
-  if (group == 0 && c < width) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += sums[i][lane];
-    dw[c] = s;
-  }
+  s = lanes_sum(sums[lane][group]);   // a warp per column
+  const int mine = blockIdx.x * 32 + group;
+  if (lane == 0 && mine < width) dw[mine] = s;
 }
 
 enum : int { kRows = 1, kCols = 2, kBlocks = 4 };
@@ -288,7 +286,7 @@ template <> __device__ __forceinline__ uint32_t as_float_bits<__half>(uint32_t m
 // Bound by HBM where rows begin on 16 bytes.  The tile stays packed, so that the registers of four CTAs (two in fp32) fit an
 // SM and their loads, maxima and stores overlap.
 template <typename T, int kWays, bool kAligned, int kCode>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4)
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : kWays == 3 ? 3 : 4)
 fp8_quantize_kernel(const T* __restrict__ x, long pitch, QuantizeOut by_rows, QuantizeOut by_cols, int n_rows, int width, int tiles_x) {
   constexpr int kTop = kCode == kCodeE4m3 ? 8 : 15;
   constexpr int kWords = sizeof(Magnitudes<T>) / 4, kPer = 8 / kWords;   // values to a word
@@ -517,7 +515,7 @@ extern "C" int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const vo
     return !ring ? added(std::false_type(), std::false_type()) : aligned ? added(std::true_type(), std::true_type()) : added(std::false_type(), std::true_type());
   });
   if (rc) return rc;
-  const cudaError_t rc2 = launch_overlapped(fp8_norm_dw_kernel, dim3((width + 31) / 32), 256, 0, s, 1, true, static_cast<const float*>(part), dw, ctas, width);
+  const cudaError_t rc2 = launch_overlapped(fp8_norm_dw_kernel, dim3((width + 31) / 32), 1024, 0, s, 1, true, static_cast<const float*>(part), dw, ctas, width);
   return rc2 == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
