@@ -38,6 +38,8 @@ static constexpr int kGemmStages = 6;
 static constexpr int kTileBytes = 128 * 128;  // 128 rows x 128 values, or 128 values x 128 rows
 static constexpr int kScaleBufs = 4;          // of 512 values of k each
 static constexpr int kGemmPairs = 148 / 2;
+static constexpr int kPairParts = 8;          // of k at most, where a tile is cut
+static constexpr int kPart = 32 * 128;        // sums of a warp
 
 struct GemmOperand {
   const uint8_t* scales;
@@ -57,10 +59,9 @@ struct GemmArgs {
   uint32_t idesc;
   int* status;
   // pairs: tiles before `whole` are taken by one pair each, the others by `parts` pairs that have a part of k each and leave
-  // sums in `part_sums`; `tickets` (zeros) count those that are through
+  // sums in `part_sums`, 16 warps of kPart floats each
   int whole, parts;
   float* part_sums;
-  int* tickets;
 };
 
 // Instruction descriptor of kind::mxf8f6f4: [4,6) byte of B's scale word; [7,10) / [10,13) type of A / B (0 e4m3, 1 e5m2);
@@ -215,8 +216,8 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
 
   if (warp >= 8) {
     // ------------------------------------------------------------ epilogue: lane = p, 128 of the tile's q
-    // registers: 256 x 184 + 256 x 64 = 63488 of the 65536 the block is launched with
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    // registers: 256 x 192 + 256 x 64 = 65536, what the block is launched with
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int quad = warp & 3, half = (warp - 8) >> 2;
     const uint32_t addr = tmem + (uint32_t(quad * 32) << 16) + half * 128;
     const uint32_t empty_bar = cluster_addr(smem_u32(&sm.acc_empty), 0);
@@ -232,27 +233,13 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(empty_bar);   // the results are in registers: the next tile's products may come
       const int p = (unit.tp * 2 + X) * 128 + quad * 32 + lane, q0 = unit.tq * 256 + half * 128, n = args.q.rows - q0;
-      if (unit.cut >= 0) {
-        // A part of k: the sums of this warp's 32 p x 128 q go to memory.  The last of the parts to come adds them all up, in
-        // the order of k: the same bits whichever is last.
-        constexpr int kPart = 128 * 32;   // floats of a warp; 16 warps of a pair
-        const int cut_tile = unit.cut / args.parts, mine = X * 8 + warp - 8;
-        float* to = args.part_sums + (size_t(unit.cut) * 16 + mine) * kPart + lane;
+      if (unit.cut >= 0) {   // a part of k: the sums of this warp's 32 p x 128 q go to memory, four q of a lane to a piece
+        float4* to = reinterpret_cast<float4*>(args.part_sums + (size_t(unit.cut) * 16 + X * 8 + warp - 8) * kPart) + lane;
 #pragma unroll
-        for (int c = 0; c < 128; ++c) __stcg(to + c * 32, __uint_as_float(acc[c]));
-        __threadfence();
-        __syncwarp();
-        int last = 0;
-        if (lane == 0) last = atomicAdd(args.tickets + cut_tile * 16 + mine, 1) == args.parts - 1;
-        if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-        __threadfence();
-        const float* from = args.part_sums + (size_t(cut_tile) * args.parts * 16 + mine) * kPart + lane;
-#pragma unroll
-        for (int c = 0; c < 128; ++c) acc[c] = 0;
-#pragma unroll 1
-        for (int part = 0; part < args.parts; ++part, from += 16 * kPart)
-#pragma unroll
-          for (int c = 0; c < 128; ++c) acc[c] = __float_as_uint(__uint_as_float(acc[c]) + __ldcg(from + c * 32));
+        for (int c = 0; c < 32; ++c)
+          to[c * 32] = make_float4(__uint_as_float(acc[4 * c]), __uint_as_float(acc[4 * c + 1]), __uint_as_float(acc[4 * c + 2]),
+                                   __uint_as_float(acc[4 * c + 3]));
+        continue;
       }
       if (p < args.p.rows)
         by_output(args, [&](auto type, auto added) {
@@ -386,6 +373,35 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
   cluster_sync();
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
   if (threadIdx.x == 0 && sm.abort_word) atomicExch(args.status, kStatusBarrierTimeout);
+}
+
+// Adds up the parts of cut tiles in the order of k: a thread has four q of one p.  A kernel of its own over the whole GPU takes
+// 3 us; the last of a tile's pairs to be through, which has the parts in reach of one SM, took 2.4 us for each of them.
+__global__ void __launch_bounds__(256) fp8_gemm_join_kernel(const __grid_constant__ GemmArgs args) {
+  const int lane = threadIdx.x & 31, piece = (blockIdx.x * 256 + threadIdx.x) >> 5, c = piece & 31, mine = (piece >> 5) & 15, tile = piece >> 9;
+  int tp, tq;
+  tile_at(args.whole + tile, args.tiles_p, args.tiles_q, tp, tq);
+  const int half = (mine >> 2) & 1, p = (tp * 2 + (mine >> 3)) * 128 + (mine & 3) * 32 + lane, q = tq * 256 + half * 128 + c * 4;
+  grid_wait();
+  const float4* from = reinterpret_cast<const float4*>(args.part_sums + (size_t(tile) * args.parts * 16 + mine) * kPart) + c * 32 + lane;
+  float4 v[kPairParts];
+#pragma unroll
+  for (int r = 0; r < kPairParts; ++r)
+    if (r < args.parts) v[r] = from[size_t(r) * 16 * (kPart / 4)];
+  grid_let_next();
+#pragma unroll
+  for (int r = 1; r < kPairParts; ++r)
+    if (r < args.parts) { v[0].x += v[r].x; v[0].y += v[r].y; v[0].z += v[r].z; v[0].w += v[r].w; }
+  if (p >= args.p.rows) return;
+  const float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+  by_output(args, [&](auto type, auto added) {
+    using T = typename decltype(type)::T;
+    T* to = static_cast<T*>(args.out) + size_t(q) * args.out_pitch + p;
+    const T* add = static_cast<const T*>(args.add) + size_t(q) * args.add_pitch + p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j, to += args.out_pitch, add += args.add_pitch)
+      if (q + j < args.q.rows) store_result<decltype(added)::value>(to, add, f[j]);
+  });
 }
 
 // ------------------------------------------------------------------ small outputs
@@ -607,7 +623,11 @@ static int launch_pair(const CUtensorMap& tm_p, const CUtensorMap& tm_q, const G
   auto kernel = fp8_gemm_pair_kernel<kPMn, kQMn>;
   if (raise_smem_limit(kernel, smem, g_gemm_smem_raised[kPMn * 2 + kQMn]) != cudaSuccess) return -4;
   const int units = args.whole + (args.tiles_p * args.tiles_q - args.whole) * args.parts;
-  const cudaError_t rc = launch_overlapped(kernel, dim3(2 * std::min(units, kGemmPairs)), kGemmThreads, smem, stream, 1, args.tickets == nullptr, tm_p, tm_q, args);
+  const cudaError_t rc = launch_overlapped(kernel, dim3(2 * std::min(units, kGemmPairs)), kGemmThreads, smem, stream, 1, true, tm_p, tm_q, args);
+  if (rc == cudaSuccess && args.parts > 1) {
+    const cudaError_t join = launch_overlapped(fp8_gemm_join_kernel, dim3((args.tiles_p * args.tiles_q - args.whole) * 64), 256, 0, stream, 1, true, args);
+    if (join != cudaSuccess) return -5;
+  }
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
@@ -631,7 +651,7 @@ struct GemmPlan {
   int n;                    // q of a tile
   long tiles_p, tiles_q;
   int whole, parts;         // pairs: see GemmArgs; split: parts
-  long work() const { return pairs && parts > 1 ? (tiles_p * tiles_q - whole) * (parts * 16l * 128 * 32 * 4 + 16 * 4) : 0; }
+  long work() const { return pairs && parts > 1 ? (tiles_p * tiles_q - whole) * parts * 16l * kPart * 4 : 0; }
 };
 static GemmPlan plan_gemm(long p_rows, long q_rows, bool q_rows_inner, int k, int form) {
   GemmPlan g;
@@ -639,11 +659,14 @@ static GemmPlan plan_gemm(long p_rows, long q_rows, bool q_rows_inner, int k, in
   g.tiles_p = (p_rows + 255) / 256;
   g.tiles_q = (q_rows + 255) / 256;
   const long pair_tiles = g.tiles_p * g.tiles_q;
-  g.pairs = form == 1 || (form == 0 && q_rows > 128 && pair_tiles >= 48);
+  // Pairs where their tiles give two thirds of them work, or fewer tiles long sums, which are cut; us with pairs / split:
+  // 2048 x 1536 x 1024 (48 tiles) 9.5 / 12.4, 200 x 28672 x 4096 (112) 32 / 49, 1024 x 2048 x 4096 (32) 18.4 / 13.5, 512 x 4096 x
+  // 14336 (32) 32.5 / 34.8, 1536 x 1024 x 16384 (24) 28 / 37, 512 x 1024 x 4096 (8) 14.3 / 10.5.
+  g.pairs = form == 1 || (form == 0 && q_rows > 128 && (pair_tiles >= 48 || pair_tiles * ((k + 127) / 128) >= 2304));
   if (g.pairs) {
     g.n = 256;
     const int rest = int(pair_tiles % kGemmPairs);
-    g.parts = rest > 0 ? std::max(1, std::min(kGemmPairs / rest, groups)) : 1;
+    g.parts = rest > 0 ? std::max(1, std::min({kGemmPairs / rest, groups, kPairParts})) : 1;
     g.whole = int(std::min(g.parts > 1 ? pair_tiles - rest : pair_tiles, 0x7fffffffl));
     return g;
   }
@@ -652,8 +675,8 @@ static GemmPlan plan_gemm(long p_rows, long q_rows, bool q_rows_inner, int k, in
   g.tiles_q = (q_rows + g.n - 1) / g.n;
   g.whole = 0;
   // as many parts as still are all under way at once: clusters of so many CTAs that fit the GPU's processors (one CTA per SM; by
-  // cudaOccupancyMaxActiveClusters).  A second round costs more than the shorter sums give: 17 x 6144 x 4096 in clusters of
-  // six, 48 of them, 16.5 us, in clusters of two 11.
+  // cudaOccupancyMaxActiveClusters).  A second round costs more than the shorter sums give: 17 x 6144 x 4096 in 48 clusters of
+  // six 16 us, of two 12 (operands from HBM, as all of these).
   constexpr int kFit[kSplitMax + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
   g.parts = 1;
   for (int parts = 2; parts <= std::min(kSplitMax, (k + 127) / 128); ++parts)
@@ -698,7 +721,6 @@ extern "C" int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, i
   args.whole = plan.whole;
   args.parts = plan.parts;
   args.part_sums = nullptr;
-  args.tickets = nullptr;
   const auto map = [&](CUtensorMap* m, const DcpkFp8Operand& o, int box) {
     return o.rows_inner ? encode_codes_map(m, o.codes, k, o.rows, o.pitch, 128) : encode_codes_map(m, o.codes, o.rows, k, o.pitch, box);
   };
@@ -707,13 +729,8 @@ extern "C" int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, i
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int mode = p->rows_inner * 2 + q->rows_inner;
   if (pairs) {
-    if (plan.work() > 0) {
-      const size_t tickets = size_t(plan.tiles_p * plan.tiles_q - plan.whole) * 16 * sizeof(int);
-      if (!work) return -3;
-      args.part_sums = static_cast<float*>(work);
-      args.tickets = reinterpret_cast<int*>(static_cast<char*>(work) + plan.work() - tickets);
-      if (cudaMemsetAsync(args.tickets, 0, tickets, s) != cudaSuccess) return -5;
-    }
+    if (plan.work() > 0 && !work) return -3;
+    args.part_sums = static_cast<float*>(work);
     args.idesc = make_idesc_mx(256, 256, p->code_type, q->code_type, p->rows_inner, q->rows_inner);
     return mode == 0 ? launch_pair<false, false>(tm_p, tm_q, args, s) : mode == 1 ? launch_pair<false, true>(tm_p, tm_q, args, s)
          : mode == 2 ? launch_pair<true, false>(tm_p, tm_q, args, s) : launch_pair<true, true>(tm_p, tm_q, args, s);
