@@ -10,6 +10,7 @@
 #include <pybind11/stl.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -178,7 +179,8 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
   const std::tuple<bool, std::optional<Tensor>> no{false, std::nullopt};
   const size_t n = params.size();
   if (n == 0 || n > 0x7fffffff || grads.size() != n || m.size() != n || v.size() != n || (masters && masters->size() != n) ||
-      bool(m_scales) != bool(v_scales) || (m_scales && (m_scales->size() != n || v_scales->size() != n)) || status.size() > 2 || !(clip >= 0))
+      bool(m_scales) != bool(v_scales) || (m_scales && (m_scales->size() != n || v_scales->size() != n)) || status.size() > 2 || !(clip >= 0) ||
+      (clip > 0 && factor))
     return no;
   const auto device = params[0].device();
   const int ptype = value_type(params[0].scalar_type()), gtype = value_type(grads[0].scalar_type());
@@ -203,6 +205,13 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
     if (masters) w[i] = (*masters)[i].data_ptr();
     if (m_scales) sm[i] = (*m_scales)[i].data_ptr(), sv[i] = (*v_scales)[i].data_ptr();
   }
+  // a tensor given twice would be written by two blocks at once
+  std::vector<const void*> written;
+  for (const auto* list : {&p, &w, &pm, &pv, &sm, &sv})
+    for (size_t i = 0; i < n; ++i)
+      if ((*list)[i] && sizes[i] > 0 && !(list == &w && !masters)) written.push_back((*list)[i]);
+  std::sort(written.begin(), written.end());
+  if (std::adjacent_find(written.begin(), written.end()) != written.end()) return no;
   c10::DeviceGuard guard(device);
   Tensor work = at::empty({dcpk_adamw_multi_work(int(n))}, step.options().dtype(at::kDouble));
   std::optional<Tensor> norm;

@@ -14,7 +14,8 @@ A product's scales have to run along the contraction in blocks of 128, so
 
 ``linear`` and ``norm_linear`` are these three as autograd functions.  On a CUDA tensor the kernels always run (a missing
 library raises); CPU tensors take the plain forms.  All calls run on the current stream of their tensors' device, allocate
-their results there and may be captured into a CUDA graph.
+their results there and may be captured into a CUDA graph once a call has been made on the device.  (As with torch's own
+functions, a backward pass is captured together with its forward pass, not while an eager graph of the same leaves lives.)
 """
 from __future__ import annotations
 
@@ -85,8 +86,11 @@ _STATUS = {}
 
 
 def _status(device: torch.device) -> torch.Tensor:
+    """The device's status word, which bounded waits report to; shared by all calls and graphs, written on failure only."""
     if device.index not in _STATUS:
-        _STATUS[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("call one of the 8-bit operators on this device before capturing a graph with them")
+        _STATUS.setdefault(device.index, torch.zeros(1, dtype=torch.int32, device=device))
     return _STATUS[device.index]
 
 

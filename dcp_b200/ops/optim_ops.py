@@ -92,6 +92,15 @@ def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta
     return norm
 
 
+def _check_written(*lists) -> None:
+    seen = set()
+    for ts in lists:
+        for t in ts or ():
+            if t.numel() > 0:
+                _need(t.data_ptr() not in seen, "a tensor that the step writes is given twice")
+                seen.add(t.data_ptr())
+
+
 def _check_lists(params, grads, masters, m, v, step, m_scales, v_scales):
     n = len(params)
     _need(n > 0, "no parameters")
@@ -135,7 +144,9 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
     taken, norm = call() if step.is_cuda and (clip is None or clip > 0) else (False, None)
     if not taken:
         _check_lists(params, grads, masters, m, v, step, m_scales, v_scales)
+        _check_written(params, masters, m, v, m_scales, v_scales)
         _need(clip is None or clip > 0, "clip has to be positive")
+        _need(clip is None or factor is None, "either clip, or a factor from elsewhere")
         _need(factor is None or (factor.dtype == torch.float32 and factor.numel() == 1 and factor.device == step.device),
               "factor has to be one float32 on the parameters' device")
         _need(len(status) <= 2 and all(s.dtype == torch.int32 and s.device == step.device for s in status), "status: up to two int32 words")

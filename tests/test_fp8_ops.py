@@ -242,6 +242,9 @@ def test_refusals_of_adamw():
                        (dict(grads=[st["grads"][0], st["grads"][1].float()]), "tensor 1"),
                        (dict(params=[p.double() for p in st["params"]]), "parameters and gradients"),
                        (dict(clip=0.0), "positive"), (dict(factor=torch.zeros(2)), "factor"),
+                       (dict(clip=1.0, factor=torch.ones(1)), "either clip"), (dict(params=[st["params"][1], st["params"][1]][:1] * 2,
+                        grads=[st["grads"][1]] * 2, masters=[st["masters"][1]] * 2, m=[st["m"][1]] * 2, v=[st["v"][1]] * 2,
+                        m_scales=[st["m_scales"][1]] * 2, v_scales=[st["v_scales"][1]] * 2), "given twice"),
                        (dict(status=[torch.zeros(1)]), "status")]:
         with pytest.raises(ValueError, match=words):
             O.adamw_multi(**ok(**bad))

@@ -478,6 +478,49 @@ def test_adamw_is_replayed_and_repeats_to_the_bit(dev):
         assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(st[k], eager[k])), k
 
 
+def test_adamw_refuses_a_tensor_given_twice(dev):
+    st = _adam_state([300, 300], 8, torch.bfloat16, torch.bfloat16, dev)
+    for k in ("params", "m", "v_scales"):
+        bad = _copy(st)
+        bad[k][1] = bad[k][0]
+        with pytest.raises(ValueError, match="given twice"):
+            O.adamw_multi(**bad, **HYPER)
+    with pytest.raises(ValueError, match="either clip"):
+        O.adamw_multi(**st, **HYPER, clip=1.0, factor=torch.ones(1, device=dev))
+    with pytest.raises(ValueError, match="tensor 1"):
+        O.adamw_multi(**{**st, "grads": [st["grads"][0], st["grads"][1][::2]]}, **HYPER)
+
+
+def test_refusals_on_the_gpu(dev):
+    x, w = torch.zeros(4, 256, device=dev), torch.zeros(8, 256, device=dev)
+    q, wq = F.quantize(x), F.quantize(w, (128, 128))
+    for call, words in [
+            (lambda: F.quantize(x[0]), "matrix"), (lambda: F.quantize(x.double()), "bfloat16"),
+            (lambda: F.rmsnorm_quant(x, w[0].cpu()), "device"), (lambda: F.rmsnorm_quant(x, w[0, :255]), "w has to be"),
+            (lambda: F.rmsnorm_quant(x, w[0], 1e-5, x.bfloat16()), "residual"),
+            (lambda: F.rmsnorm_quant_bwd(x, w[0], torch.zeros(4, device=dev), x[:2]), "dy"),
+            (lambda: F.matmul(q, wq._replace(codes=wq.codes.cpu(), scales=wq.scales.cpu())), "two devices"),
+            (lambda: F.matmul(q, wq, out=torch.zeros(8, 4, device=dev).t()), "contiguous"),
+            (lambda: F.matmul(q, wq, out=torch.zeros(1, 8, device=dev).expand(4, 8)), "contiguous"),
+            (lambda: F.matmul(q, wq, add=torch.zeros(4, 8, device=dev)), "add has to be"),
+            (lambda: F.matmul(q._replace(scales=q.scales[:, :1]), wq), "scales"), (lambda: F.matmul(q, wq, form=7), "form")]:
+        with pytest.raises(ValueError, match=words):
+            call()
+    # a broadcast addition is taken, row by row
+    got = F.matmul(q, wq, add=torch.ones(1, 8, device=dev, dtype=torch.bfloat16).expand(4, 8))
+    assert torch.equal(got, torch.ones(4, 8, device=dev, dtype=torch.bfloat16))
+    assert torch.equal(F.matmul(F.quantize(x[:0]), wq), torch.zeros(0, 8, device=dev, dtype=torch.bfloat16))
+    assert torch.equal(F.matmul(F.quantize(x[:, :0]), F.quantize(w[:, :0], (128, 128))), torch.zeros(4, 8, device=dev, dtype=torch.bfloat16))
+
+
+def test_a_graph_needs_one_call_before(dev, monkeypatch):
+    q, wq = F.quantize(torch.zeros(4, 256, device=dev)), F.quantize(torch.zeros(8, 256, device=dev), (128, 128))
+    monkeypatch.setattr(F, "_STATUS", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        F.matmul(q, wq)
+
+
 def test_adamw_status_and_factor(dev):
     st = _adam_state([300, 4096], 8, torch.bfloat16, torch.bfloat16, dev)
     ref, before = _copy(st), _copy(st)
