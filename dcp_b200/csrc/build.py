@@ -134,7 +134,7 @@ def build_calls(force: bool = False) -> Path:
     _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, *["-I%s" % i for i in inc], *map(str, srcs),
           "-o", str(out), "-L%s" % PKG, "-l:" + kernels_lib_path().name, "-Wl,-rpath,$ORIGIN", "-L%s" % (pt / "lib"),
-          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-ldl"])
+          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10", "-ldl"])
     stamp.write_text(digest)
     return out
 

@@ -5,6 +5,7 @@
 // whatever device they are; for anything else it returns nothing before it allocates or launches anything, and the caller
 // says what is wrong or brings the tensors into shape and asks again.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/stl.h>
@@ -44,19 +45,27 @@ bool rows_of(const Tensor& t) {
 long pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 bool on_16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 
-// codes whose rows begin on 16 bytes
-Tensor empty_codes(long rows, long cols, at::ScalarType type, const Tensor& like) {
-  const Tensor t = at::empty({rows, up(cols, 16)}, like.options().dtype(type));
-  return t.size(1) == cols ? t : t.narrow(1, 0, cols);
+// The GIL is given up for a call, which may wait for room in the stream's queue; pybind's own guard takes 1.5 us.
+struct WithoutGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+
+// A matrix of its own memory, straight from the allocator (a call through the dispatcher takes 0.8 us, and as much again for a
+// view of the result)
+Tensor empty_matrix(long rows, long cols, long pitch, at::ScalarType type, const Tensor& like, bool by_cols = false) {
+  Tensor t = at::detail::empty_cuda({rows * pitch}, type, like.device(), std::nullopt);
+  const int64_t sizes[2] = {by_cols ? cols : rows, by_cols ? rows : cols}, strides[2] = {by_cols ? 1 : pitch, by_cols ? pitch : 1};
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef(sizes, 2), at::IntArrayRef(strides, 2));
+  return t;
 }
-// scales of neighbouring blocks along the contraction lie next to one another: by_cols, those of 128 x 1 blocks, by columns
+Tensor empty_vector(long n, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda({n}, type, like.device(), std::nullopt); }
+// codes whose rows begin on 16 bytes
+Tensor empty_codes(long rows, long cols, at::ScalarType type, const Tensor& like) { return empty_matrix(rows, cols, up(cols, 16), type, like); }
+// scales of neighbouring blocks along the contraction lie next to one another: those of 128 x 1 blocks by columns
 Tensor empty_scales(long rows, long cols, long br, long bc, const Tensor& like) {
   const long nr = blocks(rows, br), nc = blocks(cols, bc);
-  const bool by_cols = bc == 1;
-  const long inner = by_cols ? nr : nc;
-  Tensor t = at::empty({by_cols ? nc : nr, up(inner, 4)}, like.options().dtype(at::kFloat8_e8m0fnu));
-  if (t.size(1) != inner) t = t.narrow(1, 0, inner);
-  return by_cols ? t.t() : t;
+  return bc == 1 ? empty_matrix(nc, nr, up(nr, 4), at::kFloat8_e8m0fnu, like, true) : empty_matrix(nr, nc, up(nc, 4), at::kFloat8_e8m0fnu, like);
 }
 
 using Tensors = std::optional<std::vector<Tensor>>;
@@ -102,8 +111,8 @@ Tensors norm8(const Tensor& x, const Tensor& w, double eps, const std::optional<
   const long rows = x.size(0), width = x.size(1);
   Tensor codes = empty_codes(rows, width, e5m2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn, x);
   Tensor scales = empty_scales(rows, width, 1, kBlock, x);
-  Tensor h = residual ? at::empty({rows, width}, x.options()) : x;
-  Tensor rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  Tensor h = residual ? empty_matrix(rows, width, width, x.scalar_type(), x) : x;
+  Tensor rstd = empty_vector(rows, at::kFloat, x);
   check(dcpk_fp8_norm(value_type(x.scalar_type()), e5m2, x.const_data_ptr(), pitch(x), residual ? residual->const_data_ptr() : nullptr,
                       residual ? pitch(*residual) : 0, w.const_data_ptr(), residual ? h.data_ptr() : nullptr, codes.data_ptr(), up(width, 16),
                       scales.data_ptr(), up(blocks(width, kBlock), 4), rstd.data_ptr<float>(), rows, int(width), float(eps), stream()),
@@ -118,9 +127,8 @@ Tensors norm8_bwd(const Tensor& h, const Tensor& w, const Tensor& rstd, const Te
     return std::nullopt;
   c10::DeviceGuard guard(h.device());
   const long rows = h.size(0), width = h.size(1);
-  const auto f32 = h.options().dtype(at::kFloat);
-  Tensor dx = at::empty({rows, width}, h.options()), dw = at::empty({width}, f32);
-  const Tensor part = at::empty({dcpk_fp8_norm_bwd_parts(value_type(h.scalar_type()), rows, int(width), add.has_value()), width}, f32);
+  Tensor dx = empty_matrix(rows, width, width, h.scalar_type(), h), dw = empty_vector(width, at::kFloat, h);
+  const Tensor part = empty_vector(dcpk_fp8_norm_bwd_parts(value_type(h.scalar_type()), rows, int(width), add.has_value()) * width, at::kFloat, h);
   check(dcpk_fp8_norm_bwd(value_type(h.scalar_type()), h.const_data_ptr(), pitch(h), w.const_data_ptr(), rstd.const_data_ptr<float>(),
                           dy.const_data_ptr(), pitch(dy), add ? add->const_data_ptr() : nullptr, add ? pitch(*add) : 0, dx.data_ptr(),
                           dw.data_ptr<float>(), part.data_ptr<float>(), rows, int(width), status.data_ptr<int>(), stream()),
@@ -158,10 +166,10 @@ std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair
     if (*t && (!rows_of(**t) || (*t)->size(0) != q.rows || (*t)->size(1) != p.rows || (*t)->scalar_type() != type || (*t)->device() != a.device()))
       return std::nullopt;
   c10::DeviceGuard guard(a.device());
-  Tensor result = out ? *out : at::empty({q.rows, p.rows}, a.options().dtype(type));
+  Tensor result = out ? *out : empty_matrix(q.rows, p.rows, p.rows, type, a);
   const long bytes = dcpk_fp8_gemm_work(q.rows, p.rows, q.rows_inner, int(a.size(ka)), form);
   Tensor work;   // of this call alone
-  if (bytes > 0) work = at::empty({bytes}, a.options().dtype(at::kByte));
+  if (bytes > 0) work = empty_vector(bytes, at::kByte, a);
   check(dcpk_fp8_gemm(&q, &p, int(a.size(ka)), result.data_ptr(), pitch(result), add ? add->const_data_ptr() : nullptr, add ? pitch(*add) : 0,
                       out_type, form, bytes > 0 ? work.data_ptr() : nullptr, status.data_ptr<int>(), stream()),
         "fp8_gemm");
@@ -213,9 +221,9 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
   std::sort(written.begin(), written.end());
   if (std::adjacent_find(written.begin(), written.end()) != written.end()) return no;
   c10::DeviceGuard guard(device);
-  Tensor work = at::empty({dcpk_adamw_multi_work(int(n))}, step.options().dtype(at::kDouble));
+  Tensor work = empty_vector(dcpk_adamw_multi_work(int(n)), at::kDouble, step);
   std::optional<Tensor> norm;
-  if (clip > 0) norm = at::empty({1}, step.options().dtype(at::kFloat));
+  if (clip > 0) norm = empty_vector(1, at::kFloat, step);
   const int* words[2] = {status.size() > 0 ? status[0].const_data_ptr<int>() : nullptr, status.size() > 1 ? status[1].const_data_ptr<int>() : nullptr};
   check(dcpk_adamw_multi(int(n), p.data(), g.data(), masters ? w.data() : nullptr, pm.data(), pv.data(), m_scales ? sm.data() : nullptr,
                          m_scales ? sv.data() : nullptr, sizes.data(), ptype, gtype, step.data_ptr<int64_t>(), float(lr), beta1, beta2,
@@ -228,7 +236,7 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
 }  // namespace
 
 void bind_ops8(py::module_& m) {
-  auto free_gil = py::call_guard<py::gil_scoped_release>();   // a launch may wait for room in the stream's queue
+  const py::call_guard<WithoutGil> free_gil;
   m.def("quantize8", &quantize8, free_gil);
   m.def("norm8", &norm8, free_gil);
   m.def("norm8_bwd", &norm8_bwd, free_gil);
