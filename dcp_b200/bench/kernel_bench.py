@@ -4,6 +4,7 @@ larger than L2 or an L2 flush between iterations), with achieved fractions of th
     python -m dcp_b200.bench.kernel_bench attn_fwd --tokens 8192 --kv 8192 --hq 32 --hkv 8 --mask causal
     python -m dcp_b200.bench.kernel_bench attn_bwd ...
     python -m dcp_b200.bench.kernel_bench ops
+    python -m dcp_b200.bench.kernel_bench ops8
     python -m torch.distributed.run --nproc-per-node 2 ... -m dcp_b200.bench.kernel_bench nvlink
 
 Counterpart of the reference's benchmark/ops/{benchmark_fused_memcpy,benchmark_fused_update,
@@ -213,6 +214,55 @@ def bench_ops(args):
         report("fused_rs_adamw_ag", time_fn(lambda: opt.step(1.0), args.iters, 3, flush), n * (2 + 12 + 12 + 2))
 
 
+def bench_ops8(args):
+    """Operators of training in 8 bits at a Llama-3-8B layer's sizes: milliseconds and GB/s of algorithmic bytes, or TFLOP/s,
+    with the fraction of the measured copy bandwidth or of the measured bf16 rate (the tensor cores' 8-bit rate is twice that)."""
+    from ..ops import fp8_ops, optim_ops
+    dev = torch.device("cuda")
+    hbm, tf, src = measured_peaks()
+    T, H, F = args.tokens, 4096, 14336
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device=dev)
+    want = lambda name: args.only is None or args.only == name  # noqa: E731
+    rand = lambda *shape: torch.randn(*shape, device=dev).bfloat16()  # noqa: E731
+
+    def report(name, fn, nbytes=0, flops=0):
+        ms = time_fn(fn, args.iters, 3, flush)
+        rate = {"TFLOP/s": round(flops / ms / 1e9, 1), f"of_{src}_bf16_peak": round(flops / ms / 1e9 / tf, 3)} if flops else \
+            {"GB/s": round(nbytes / ms / 1e6, 1), f"frac_of_{src}_hbm": round(nbytes / ms / 1e6 / hbm, 3)}
+        print(json.dumps({"op": name, "ms": round(ms, 4), **rate}))
+
+    x, res, w = rand(T, H), rand(T, H), rand(H)
+    if want("rmsnorm_quant"):
+        report("rmsnorm_quant", lambda: fp8_ops.rmsnorm_quant(x, w, 1e-5, res), T * H * 7)
+    if want("rmsnorm_quant_bwd"):
+        rstd = torch.rand(T, device=dev) + 0.5
+        report("rmsnorm_quant_bwd", lambda: fp8_ops.rmsnorm_quant_bwd(x, w, rstd, res, x), T * H * 8)
+    if want("quantize_rows"):
+        report("quantize_rows", lambda: fp8_ops.quantize(x), T * H * 3)
+    if want("quantize_both"):
+        report("quantize_both", lambda: fp8_ops.quantize_both(x), T * H * 4)
+    if any(want(f"matmul_{k}") for k in ("forward", "dgrad", "wgrad")):
+        (xr, xc), (gr, gc) = fp8_ops.quantize_both(x), fp8_ops.quantize_both(rand(T, 2 * F))
+        wq = fp8_ops.quantize(rand(2 * F, H), (128, 128))
+        flops = 2 * T * H * 2 * F
+        if want("matmul_forward"):
+            report("matmul_forward", lambda: fp8_ops.matmul(xr, wq), flops=flops)
+        if want("matmul_dgrad"):
+            report("matmul_dgrad", lambda: fp8_ops.matmul(gr, wq, trans_b=False), flops=flops)
+        if want("matmul_wgrad"):
+            report("matmul_wgrad", lambda: fp8_ops.matmul(gc, xc, trans_a=True, trans_b=False), flops=flops)
+    for bits, per in ((32, 28), (8, 16)):
+        if want(f"adamw_{bits}"):
+            n = args.opt_elems // 4
+            params = [rand(n // 4) for _ in range(4)]
+            opt = optim_ops.MultiTensorAdamW(params, state_bits=bits)
+            for p in params:
+                p.grad = rand(p.numel())
+            report(f"adamw_{bits}", opt.step, n * per)
+            del params, opt
+    fp8_ops.check_status()
+
+
 def bench_nvlink(args):
     """Two or more ranks (torch.distributed.run): bandwidth of the in-kernel communication primitives
     over NVLink, CUDA-event timed, max over ranks: peer -> local copy jobs (the operand fetch),
@@ -267,9 +317,9 @@ def bench_nvlink(args):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("kind", choices=["attn_fwd", "attn_bwd", "ops", "nvlink"])
-    ap.add_argument("--only", default=None, help="ops: build and run just this op (small working set for a profiler)")
-    ap.add_argument("--opt-elems", type=int, default=256 << 20, help="ops: parameters of the optimizer-kernel benchmark")
+    ap.add_argument("kind", choices=["attn_fwd", "attn_bwd", "ops", "ops8", "nvlink"])
+    ap.add_argument("--only", default=None, help="ops, ops8: build and run just this op (small working set for a profiler)")
+    ap.add_argument("--opt-elems", type=int, default=256 << 20, help="ops, ops8: parameters of the optimizer-kernel benchmark")
     ap.add_argument("--tokens", type=int, default=8192)
     ap.add_argument("--kv", type=int, default=8192)
     ap.add_argument("--hq", type=int, default=32)
@@ -285,6 +335,8 @@ def main():
         bench_nvlink(args)
     elif args.kind == "ops":
         bench_ops(args)
+    elif args.kind == "ops8":
+        bench_ops8(args)
     else:
         bench_attention(args.kind, args)
 

@@ -2,8 +2,11 @@
 //
 //   m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      w -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + wd w)
 //
-// with g the gradient times grad_scale and the clipping coefficient min(1, clip / (norm + 1e-6)).  Bound by HBM: 28 bytes per
-// parameter with moments in 32 bits (bf16 parameter and gradient, fp32 master), 16 with moments in 8.
+// with g the gradient times grad_scale and the clipping coefficient min(1, clip / (norm + 1e-6)).  28 bytes per parameter with
+// moments in 32 bits (bf16 parameter and gradient, fp32 master), 16 with moments in 8, and 2 more for the norm.  218M parameters
+// in 32 bits: norm 68 us (6.4 TB/s), update 967 (6.3 TB/s), bound by HBM.  In 8 bits: update 627 us (5.5 TB/s), bound by issuing 76
+// instructions per parameter (78 % of the slots): hash 9, rounding and packing of two codes 15, the moments 11, root and
+// quotient 13, addresses and conversions.
 //
 // Moments in 8 bits: m and sqrt(v) as e4m3 with a power-of-two scale per 256 values (fp8_common.cuh).  The root, because it
 // is what the update divides by and because it halves v's range of exponents.  A moving average does not survive rounding to
