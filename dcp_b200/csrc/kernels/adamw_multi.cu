@@ -229,7 +229,7 @@ __device__ __forceinline__ uint2 encode8(float amax, const float (&f)[8], const 
 // run of chunks, so that it looks for its tensor once and has four loads per thread under way (a chunk at a time from a
 // grid of CTAs: 436 MB in 144 us).
 template <typename G>
-__global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_constant__ AdamList list, float grad_scale, double* __restrict__ parts) {
+__global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_constant__ AdamList list, float grad_scale, double* parts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
   float sq[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   grid_wait();
@@ -285,10 +285,10 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
 }
 
 // step counter, bias corrections, clipping coefficient: one CTA
-__global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* __restrict__ parts, int n_parts, int64_t* __restrict__ step, double beta1,
-                                                            double beta2, float grad_scale, float clip, const float* __restrict__ factor,
-                                                            uint32_t seed, float* __restrict__ norm, const int* __restrict__ status_a,
-                                                            const int* __restrict__ status_b, AdamShared* __restrict__ shared) {
+__global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* parts, int n_parts, int64_t* step, double beta1,
+                                                            double beta2, float grad_scale, float clip, const float* factor,
+                                                            uint32_t seed, float* norm, const int* status_a,
+                                                            const int* status_b, AdamShared* shared) {
   __shared__ double sums[8];
   grid_wait();
   grid_let_next();
@@ -330,7 +330,7 @@ struct Block8 {   // a lane's part of a block with moments in 8 bits
 // for 218M parameters in 8 bits).
 template <typename P, typename G, bool kMaster, bool kEight>
 __global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 5) adamw_multi_kernel(const __grid_constant__ AdamList list, const AdamScalars s,
-                                                                                   const AdamShared* __restrict__ shared) {
+                                                                                   const AdamShared* shared) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
   grid_wait();
   if (shared->skip) return;

@@ -5,6 +5,10 @@
 // 57344), so the exponent comes from the exponent field of max|x| and one comparison of its mantissa, without a
 // logarithm.  A block with a value that is not finite gets the byte 255, which stands for NaN: all of it reads back as
 // NaN.  Zeros get the byte 0.
+//
+// The kernels are launched while the one before them ends (launch.cuh) and read what it writes, after grid_wait().  So no pointer
+// to global memory is __restrict__ and nothing goes through __ldg: the compiler takes such loads for loads of constants, which
+// it may move in front of the wait.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

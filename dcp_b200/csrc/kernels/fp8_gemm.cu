@@ -118,7 +118,7 @@ __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
 // scales of a row (the last one's where it is past the end: those results are not stored) of blocks kb .. kb + 3
 __device__ __forceinline__ uint32_t scale_word(const GemmOperand& o, int row, int kb, int n_kb) {
   const uint8_t* p = o.scales + long(min(row, o.rows - 1) >> o.shift) * o.row_stride + long(kb) * o.k_stride;
-  if (o.words && kb + 4 <= n_kb) return __ldg(reinterpret_cast<const uint32_t*>(p));
+  if (o.words && kb + 4 <= n_kb) return *reinterpret_cast<const uint32_t*>(p);
   uint32_t v = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -139,11 +139,16 @@ __device__ __forceinline__ void by_output(const GemmArgs& a, F f) {
   else if (a.out_type == kTypeF16) a.add ? f(OutType<kTypeF16>(), std::true_type()) : f(OutType<kTypeF16>(), std::false_type());
   else a.add ? f(OutType<kTypeF32>(), std::true_type()) : f(OutType<kTypeF32>(), std::false_type());
 }
-// one result, rounded once; `from` is read where something is added
-template <bool kAdd, typename T>
-__device__ __forceinline__ void store_result(T* to, const T* from, float v) {
-  if (kAdd) v += to_float(*from);
-  *to = from_float<T>(v);
+// `kN` results that lie a pitch apart, the first n of them, rounded once; what they are added to is read first, so that its
+// loads are under way together (it may be the output itself)
+template <bool kAdd, int kN, typename T>
+__device__ __forceinline__ void store_results(const GemmArgs& a, T* to, const T* from, const uint32_t (&v)[kN], int n) {
+  float sum[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i, from += a.add_pitch) sum[i] = __uint_as_float(v[i]) + (kAdd && i < n ? to_float(*from) : 0.f);
+#pragma unroll
+  for (int i = 0; i < kN; ++i, to += a.out_pitch)
+    if (i < n) *to = from_float<T>(sum[i]);
 }
 
 struct __align__(1024) GemmSmem {
@@ -257,8 +262,8 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_cons
           T* to = static_cast<T*>(args.out) + size_t(q0) * args.out_pitch + p;
           const T* from = static_cast<const T*>(args.add) + size_t(q0) * args.add_pitch + p;
 #pragma unroll
-          for (int c = 0; c < 128; ++c, to += args.out_pitch, from += args.add_pitch)
-            if (c < n) store_result<decltype(added)::value>(to, from, __uint_as_float(acc[c]));
+          for (int c = 0; c < 128; c += 16, to += 16 * args.out_pitch, from += 16 * args.add_pitch)
+            store_results<decltype(added)::value>(args, to, from, *reinterpret_cast<const uint32_t(*)[16]>(acc + c), n - c);
         });
     }
   } else if (warp >= 4) {
@@ -403,14 +408,11 @@ __global__ void __launch_bounds__(256) fp8_gemm_join_kernel(const __grid_constan
   for (int r = 1; r < kPairParts; ++r)
     if (r < args.parts) { v[0].x += v[r].x; v[0].y += v[r].y; v[0].z += v[r].z; v[0].w += v[r].w; }
   if (p >= args.p.rows) return;
-  const float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+  const uint32_t sum[4] = {__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[0].z), __float_as_uint(v[0].w)};
   by_output(args, [&](auto type, auto added) {
     using T = typename decltype(type)::T;
-    T* to = static_cast<T*>(args.out) + size_t(q) * args.out_pitch + p;
-    const T* add = static_cast<const T*>(args.add) + size_t(q) * args.add_pitch + p;
-#pragma unroll
-    for (int j = 0; j < 4; ++j, to += args.out_pitch, add += args.add_pitch)
-      if (q + j < args.q.rows) store_result<decltype(added)::value>(to, add, f[j]);
+    store_results<decltype(added)::value>(args, static_cast<T*>(args.out) + size_t(q) * args.out_pitch + p,
+                                          static_cast<const T*>(args.add) + size_t(q) * args.add_pitch + p, sum, args.q.rows - q);
   });
 }
 
@@ -566,10 +568,7 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
             using T = typename decltype(type)::T;
             T* to = static_cast<T*>(args.out) + size_t(q0 + c0) * args.out_pitch + p;
             const T* from = static_cast<const T*>(args.add) + size_t(q0 + c0) * args.add_pitch + p;
-            const int n = args.q.rows - q0 - c0;
-#pragma unroll
-            for (int c = 0; c < 16; ++c, to += args.out_pitch, from += args.add_pitch)
-              if (c < n) store_result<decltype(added)::value>(to, from, __uint_as_float(acc[c]));
+            store_results<decltype(added)::value>(args, to, from, acc, args.q.rows - q0 - c0);
           });
         }
       }
@@ -596,10 +595,13 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_con
             if (r < splits) { v[0].x += v[r].x; v[0].y += v[r].y; v[0].z += v[r].z; v[0].w += v[r].w; }
           T* to = static_cast<T*>(args.out) + size_t(q0 + c) * args.out_pitch + p;
           const T* from = static_cast<const T*>(args.add) + size_t(q0 + c) * args.add_pitch + p;
-          const float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+          float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (p + j < args.p.rows) store_result<decltype(added)::value>(to + j, from + j, f[j]);
+            if (decltype(added)::value && p + j < args.p.rows) f[j] += to_float(from[j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (p + j < args.p.rows) to[j] = from_float<T>(f[j]);
         }
       });
     }

@@ -56,9 +56,9 @@ static constexpr int kRingBytes = 200 * 1024;   // of an SM's shared memory, for
 // the CTAs' coming and going (65536 rows with a residual 70 us).
 template <typename T, int kVecs, bool kAligned, int kCode, bool kWarps>
 __global__ void __launch_bounds__(kNormThreads)
-fp8_norm_kernel(const T* __restrict__ x, long x_pitch, const T* __restrict__ residual, long residual_pitch, const T* __restrict__ w,
-                T* __restrict__ h, uint8_t* __restrict__ codes, long code_pitch, uint8_t* __restrict__ scales, long scale_pitch,
-                float* __restrict__ rstd, int n_rows, int width, float eps) {
+fp8_norm_kernel(const T* x, long x_pitch, const T* residual, long residual_pitch, const T* w,
+                T* h, uint8_t* codes, long code_pitch, uint8_t* scales, long scale_pitch,
+                float* rstd, int n_rows, int width, float eps) {
   __shared__ float scratch[kNormThreads / 32];
   constexpr int kTop = kCode == kCodeE4m3 ? 8 : 15;
   const long row = kWarps ? long(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -117,9 +117,9 @@ fp8_norm_kernel(const T* __restrict__ x, long x_pitch, const T* __restrict__ res
 // With plain loads at the beginning of a row 5003 rows of 5120 took 62 us (2.9 TB/s).
 template <typename T, int kVecs, bool kAligned, bool kRing, bool kAdd>
 __global__ void __launch_bounds__(kVecs == 1 ? 1024 : kVecs == 2 ? 768 : 512)   // 64, 80 and 128 registers
-fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__ w, const float* __restrict__ rstd, const T* __restrict__ dy,
-                    long dy_pitch, const T* __restrict__ add, long add_pitch, T* __restrict__ dx, float* __restrict__ part, int n_rows,
-                    int width, int stages, int* __restrict__ status) {
+fp8_norm_bwd_kernel(const T* h, long h_pitch, const T* w, const float* rstd, const T* dy,
+                    long dy_pitch, const T* add, long add_pitch, T* dx, float* part, int n_rows,
+                    int width, int stages, int* status) {
   __shared__ float scratch[2][kNormThreads / 32];
   __shared__ uint64_t full[kMaxStages];
   __shared__ int abort_word;
@@ -237,7 +237,7 @@ fp8_norm_bwd_kernel(const T* __restrict__ h, long h_pitch, const T* __restrict__
 }
 
 // 32 columns per CTA, 32 threads of a column take every 32nd of the parts
-__global__ void __launch_bounds__(1024) fp8_norm_dw_kernel(const float* __restrict__ part, float* __restrict__ dw, int n, int width) {
+__global__ void __launch_bounds__(1024) fp8_norm_dw_kernel(const float* part, float* dw, int n, int width) {
   __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
@@ -290,7 +290,7 @@ template <> __device__ __forceinline__ uint32_t as_float_bits<__half>(uint32_t m
 // SM and their loads, maxima and stores overlap.
 template <typename T, int kWays, bool kAligned, int kCode>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : kWays == 3 ? 3 : 4)
-fp8_quantize_kernel(const T* __restrict__ x, long pitch, QuantizeOut by_rows, QuantizeOut by_cols, int n_rows, int width, int tiles_x) {
+fp8_quantize_kernel(const T* x, long pitch, QuantizeOut by_rows, QuantizeOut by_cols, int n_rows, int width, int tiles_x) {
   constexpr int kTop = kCode == kCodeE4m3 ? 8 : 15;
   constexpr int kWords = sizeof(Magnitudes<T>) / 4, kPer = 8 / kWords;   // values to a word
   __shared__ uint32_t column_max[(kWays & kCols) ? 16 : 1][kBlock / kPer + 4];
