@@ -152,6 +152,16 @@ bool operand(const Tensor& codes, const Tensor& scales, long br, long bc, int k_
   return true;
 }
 
+// Two matrices of one shape and type are one, or share no element: a thread reads what it adds to just before it writes there,
+// but not before others write.
+bool one_or_apart(const Tensor& a, const Tensor& b) {
+  const long m = a.size(0), n = a.size(1), size = long(a.element_size()), pa = pitch(a), pb = pitch(b);
+  const long d = long(reinterpret_cast<intptr_t>(b.const_data_ptr()) - reinterpret_cast<intptr_t>(a.const_data_ptr()));
+  if ((d == 0 && pa == pb) || d >= ((m - 1) * pa + n) * size || -d >= ((m - 1) * pb + n) * size) return true;
+  const long at = (d % (pa * size) + pa * size) % (pa * size);   // of b's rows within a's pitch
+  return pa == pb && at >= n * size && at <= (pa - n) * size;    // columns beside one another
+}
+
 std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair<long, long> a_block, const Tensor& b, const Tensor& b_scales,
                               std::pair<long, long> b_block, bool trans_a, bool trans_b, int out_type, const std::optional<Tensor>& add,
                               const std::optional<Tensor>& out, int form, const Tensor& status) {
@@ -165,6 +175,7 @@ std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair
   for (const auto* t : {&add, &out})
     if (*t && (!rows_of(**t) || (*t)->size(0) != q.rows || (*t)->size(1) != p.rows || (*t)->scalar_type() != type || (*t)->device() != a.device()))
       return std::nullopt;
+  if (add && out && !one_or_apart(*add, *out)) return std::nullopt;
   c10::DeviceGuard guard(a.device());
   Tensor result = out ? *out : empty_matrix(q.rows, p.rows, p.rows, type, a);
   const long bytes = dcpk_fp8_gemm_work(q.rows, p.rows, q.rows_inner, int(a.size(ka)), form);

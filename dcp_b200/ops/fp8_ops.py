@@ -241,10 +241,25 @@ def _on_16(q: BlockScaled) -> BlockScaled:
     return q._replace(codes=codes)
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two matrices of one shape and type whose rows are contiguous share no element; interleaved columns of one are apart."""
+    (m, n), size = a.shape, a.element_size()
+    if m == 0 or n == 0:
+        return True
+    (pa, pb), d = (t.stride(0) if m > 1 else n for t in (a, b)), b.data_ptr() - a.data_ptr()
+    if d >= ((m - 1) * pa + n) * size or -d >= ((m - 1) * pb + n) * size:
+        return True
+    return pa == pb and n * size <= d % (pa * size) <= (pa - n) * size
+
+
+def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and (a.shape[0] <= 1 or a.stride(0) == b.stride(0))
+
+
 def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bool = True, out_dtype: torch.dtype = torch.bfloat16,
            add: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, form: int = 0) -> torch.Tensor:
     """op(a) op(b) of the values the codes stand for, summed in fp32 and rounded once; ``add`` (of the output's type and shape,
-    rows contiguous) is added before the rounding and may be ``out`` itself.
+    rows contiguous) is added before the rounding; it may be ``out`` itself, and shares nothing with it otherwise.
 
     a: [M, K], or [K, M] with ``trans_a``; b: [N, K], or [K, N] without ``trans_b`` -> [M, N] in bf16, fp16 or fp32.  Along K
     both need a scale per 128 values; along the other dimension one per value or per 128.  Codes whose rows begin on 16 bytes
@@ -273,6 +288,9 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
         if add is not None:
             _need(tuple(add.shape) == (m, n) and add.dtype == out_dtype and add.device == a.codes.device,
                   f"add has to be {out_dtype} {(m, n)} on a's device")
+            if out is not None:
+                rows = _rows(add)   # a copy where its rows are not contiguous
+                _need(_same_place(rows, out) or _apart(rows, out), "add has to be out itself or lie apart from it")
         if not a.codes.is_cuda:
             got = matmul_reference(a, b, trans_a, trans_b, out_dtype, add)
             return got if out is None else out.copy_(got)

@@ -259,3 +259,24 @@ def test_a_status_word_stops_the_step():
     before = [p.clone() for p in st["params"]]
     O.adamw_multi(**st, **HYPER, status=[torch.zeros(1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)])
     assert all(torch.equal(a, b) for a, b in zip(before, st["params"])) and int(st["step"]) == 4
+
+
+def test_what_a_product_is_added_to_is_the_output_or_lies_apart():
+    torch.manual_seed(0)
+    a, b = F.quantize(torch.randn(5, 130)), F.quantize(torch.randn(7, 130), (128, 128))
+    buf = torch.randn(40 * 20)
+    at = lambda start, pitch: buf[start:].as_strided((5, 7), (pitch, 1), buf.storage_offset() + start)  # noqa: E731
+    for out, add, ok in ((at(0, 20), at(0, 20), True), (at(0, 20), at(7, 20), True), (at(7, 20), at(0, 20), True), (at(0, 20), at(13, 20), True),
+                         (at(0, 20), at(6, 20), False), (at(0, 20), at(14, 20), False), (at(0, 20), at(20, 20), False), (at(0, 20), at(0, 7), False),
+                         (at(0, 7), at(34, 7), False), (at(0, 7), at(35, 7), True), (at(35, 7), at(0, 7), True), (at(1, 7), at(0, 7), False),
+                         (at(0, 20), at(27, 20), True), (at(0, 8), at(40, 9), True), (at(0, 9), at(3, 8), False)):
+        used = [{t.storage_offset() + i * t.stride(0) + j for i in range(5) for j in range(7)} for t in (out, add)]
+        same = (out.storage_offset(), out.stride()) == (add.storage_offset(), add.stride())
+        if out.stride() == add.stride():   # of one pitch the rule is exact
+            assert ok == (same or not used[0] & used[1])
+        if ok:
+            want = F.matmul(a, b, out_dtype=torch.float32, add=add.clone())
+            assert torch.equal(F.matmul(a, b, add=add, out=out), want)
+        else:
+            with pytest.raises(ValueError, match="lie apart"):
+                F.matmul(a, b, add=add, out=out)

@@ -673,3 +673,21 @@ def test_training_steps_in_8_bits(dev, tmp_path):
     finally:
         eng.close()
         other.close()
+
+
+@pytest.mark.parametrize("form", [1, 2])
+def test_what_a_product_is_added_to_on_the_gpu(dev, form):
+    """Beside the output in one matrix, the output itself, or refused."""
+    m, n, k = 130, 200, 300
+    a, b = F.quantize(_values(m, k, torch.bfloat16, dev)), F.quantize(_values(n, k, torch.bfloat16, dev, 1), (128, 128))
+    buf = torch.randn(m + 2, 2 * n + 3, device=dev)
+    beside = buf[:m, n + 1:2 * n + 1]
+    for out, add in ((buf[:m, :n], beside), (beside, buf[:m, :n]), (buf[:m, :n], buf[:m, :n])):
+        want = F.matmul(a, b, out_dtype=torch.float32, add=add.clone(), form=form)
+        kept = buf.clone()
+        assert torch.equal(F.matmul(a, b, add=add, out=out, form=form), want)
+        out.copy_(kept[:m, :n] if out.data_ptr() == buf.data_ptr() else kept[:m, n + 1:2 * n + 1])
+        assert torch.equal(buf, kept)
+    for out, add in ((buf[:m, :n], buf[1:m + 1, :n]), (buf[:m, :n], buf[:m, 1:n + 1]), (buf[:m, 3:n + 3], buf[2:m + 2, :n])):
+        with pytest.raises(ValueError, match="lie apart"):
+            F.matmul(a, b, add=add, out=out, form=form)
