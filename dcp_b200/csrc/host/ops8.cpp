@@ -199,7 +199,7 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
   const size_t n = params.size();
   if (n == 0 || n > 0x7fffffff || grads.size() != n || m.size() != n || v.size() != n || (masters && masters->size() != n) ||
       bool(m_scales) != bool(v_scales) || (m_scales && (m_scales->size() != n || v_scales->size() != n)) || status.size() > 2 || !(clip >= 0) ||
-      (clip > 0 && factor))
+      (clip > 0 && factor) || !(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1))
     return no;
   const auto device = params[0].device();
   const int ptype = value_type(params[0].scalar_type()), gtype = value_type(grads[0].scalar_type());
@@ -224,13 +224,22 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
     if (masters) w[i] = (*masters)[i].data_ptr();
     if (m_scales) sm[i] = (*m_scales)[i].data_ptr(), sv[i] = (*v_scales)[i].data_ptr();
   }
-  // a tensor given twice would be written by two blocks at once
-  std::vector<const void*> written;
-  for (const auto* list : {&p, &w, &pm, &pv, &sm, &sv})
-    for (size_t i = 0; i < n; ++i)
-      if ((*list)[i] && sizes[i] > 0 && !(list == &w && !masters)) written.push_back((*list)[i]);
+  // memory given twice would be written by two blocks at once
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  written.reserve(6 * n);
+  const auto writes = [&](const std::vector<void*>& list, size_t i, long bytes) {
+    const uintptr_t start = reinterpret_cast<uintptr_t>(list[i]);
+    if (start && bytes > 0) written.emplace_back(start, start + uintptr_t(bytes));
+  };
+  const long of_param = long(params[0].element_size()), of_state = m_scales ? 1 : 4;
+  for (size_t i = 0; i < n; ++i) {
+    writes(p, i, sizes[i] * of_param), writes(w, i, sizes[i] * 4);
+    writes(pm, i, sizes[i] * of_state), writes(pv, i, sizes[i] * of_state);
+    writes(sm, i, blocks(sizes[i], kStateBlock)), writes(sv, i, blocks(sizes[i], kStateBlock));
+  }
   std::sort(written.begin(), written.end());
-  if (std::adjacent_find(written.begin(), written.end()) != written.end()) return no;
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i - 1].second > written[i].first) return no;
   c10::DeviceGuard guard(device);
   Tensor work = empty_vector(dcpk_adamw_multi_work(int(n)), at::kDouble, step);
   std::optional<Tensor> norm;

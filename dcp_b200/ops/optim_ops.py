@@ -93,12 +93,8 @@ def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta
 
 
 def _check_written(*lists) -> None:
-    seen = set()
-    for ts in lists:
-        for t in ts or ():
-            if t.numel() > 0:
-                _need(t.data_ptr() not in seen, "a tensor that the step writes is given twice")
-                seen.add(t.data_ptr())
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for ts in lists for t in ts or () if t.numel() > 0)
+    _need(all(end <= start for (_, end), (start, _) in zip(spans, spans[1:])), "memory that the step writes is given twice")
 
 
 def _check_lists(params, grads, masters, m, v, step, m_scales, v_scales):
@@ -145,6 +141,7 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
     if not taken:
         _check_lists(params, grads, masters, m, v, step, m_scales, v_scales)
         _check_written(params, masters, m, v, m_scales, v_scales)
+        _need(0 <= beta1 < 1 and 0 <= beta2 < 1, f"betas from 0 to below 1, not {beta1} and {beta2}")
         _need(clip is None or clip > 0, "clip has to be positive")
         _need(clip is None or factor is None, "either clip, or a factor from elsewhere")
         _need(factor is None or (factor.dtype == torch.float32 and factor.numel() == 1 and factor.device == step.device),

@@ -280,3 +280,24 @@ def test_what_a_product_is_added_to_is_the_output_or_lies_apart():
         else:
             with pytest.raises(ValueError, match="lie apart"):
                 F.matmul(a, b, add=add, out=out)
+
+
+@pytest.mark.parametrize("key", ["params", "masters", "m", "v", "m_scales", "v_scales"])
+def test_adamw_refuses_memory_that_overlaps(key):
+    """Also where it does not begin at one address; parts of one buffer beside one another are taken."""
+    st = _state([300, 300], 8, torch.bfloat16, torch.bfloat16)
+    for skip, ok in ((st[key][0].numel(), True), (st[key][0].numel() - 1, False), (1, False)):
+        n = st[key][0].numel()
+        flat = torch.zeros(2 * n, dtype=torch.uint8).view(st[key][0].dtype) if st[key][0].element_size() == 1 else torch.zeros(2 * n, dtype=st[key][0].dtype)
+        call = lambda: O.adamw_multi(**{**st, **HYPER, key: [flat[skip:skip + n], flat[:n]]})  # noqa: B023, E731
+        if ok:
+            call()
+        else:
+            with pytest.raises(ValueError, match="given twice"):
+                call()
+
+
+@pytest.mark.parametrize("bad", [dict(beta1=1.0), dict(beta2=1.0), dict(beta1=-0.1), dict(beta2=float("nan"))])
+def test_adamw_refuses_betas_that_it_would_divide_by_zero_with(bad):
+    with pytest.raises(ValueError, match="betas"):
+        O.adamw_multi(**{**_state([5], 8, torch.bfloat16, torch.bfloat16), **HYPER, **bad})

@@ -691,3 +691,21 @@ def test_what_a_product_is_added_to_on_the_gpu(dev, form):
     for out, add in ((buf[:m, :n], buf[1:m + 1, :n]), (buf[:m, :n], buf[:m, 1:n + 1]), (buf[:m, 3:n + 3], buf[2:m + 2, :n])):
         with pytest.raises(ValueError, match="lie apart"):
             F.matmul(a, b, add=add, out=out, form=form)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_refuses_overlapping_memory_and_betas_on_the_gpu(dev, bits):
+    st = _adam_state([300, 300], bits, torch.bfloat16, torch.bfloat16, dev)
+    kept = _copy(st)
+    for key in ("params", "masters", "m", "v") + (("m_scales", "v_scales") if bits == 8 else ()):
+        n, size = st[key][0].numel(), st[key][0].element_size()
+        flat = torch.zeros(2 * n * size, dtype=torch.uint8, device=dev).view(st[key][0].dtype)
+        for skip in (n - 1, 1):
+            if skip < n:
+                with pytest.raises(ValueError, match="given twice"):
+                    O.adamw_multi(**{**st, **HYPER, key: [flat[skip:skip + n], flat[:n]]})
+        O.adamw_multi(**{**_copy(st), **HYPER, key: [flat[n:], flat[:n]]})   # beside one another
+    for bad in (dict(beta1=1.0), dict(beta2=1.0), dict(beta1=float("nan"))):
+        with pytest.raises(ValueError, match="betas"):
+            O.adamw_multi(**{**st, **HYPER, **bad})
+    assert int(st["step"]) == int(kept["step"]) and all(torch.equal(_bits(a), _bits(b)) for a, b in zip(st["params"], kept["params"]))
