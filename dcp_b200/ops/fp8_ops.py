@@ -12,16 +12,18 @@ A product's scales have to run along the contraction in blocks of 128, so
 * ``dx = dy w``     takes dy by rows and the same codes of w:               ``matmul(dy, w, trans_b=False)``
 * ``dw = dy^T x``   takes both by tokens (128 x 1):                         ``matmul(dy, x, trans_a=True, trans_b=False)``
 
-``linear`` and ``norm_linear`` are these three as autograd functions.  On a CUDA tensor the kernels always run (a missing
-library raises); CPU tensors take the plain forms.  All calls run on the current stream of their tensors' device, allocate
-their results there and may be captured into a CUDA graph once a call has been made on the device.  (As with torch's own
-functions, a backward pass is captured together with its forward pass, not while an eager graph of the same leaves lives.)
+``linear`` and ``norm_linear`` are these three as autograd functions (of a first derivative; a second is refused).  On a
+CUDA tensor the kernels always run (a missing library raises); CPU tensors take the plain forms.  All calls run on the
+current stream of their tensors' device, allocate their results there and may be captured into a CUDA graph once a call has
+been made on the device.  (As with torch's own functions, a backward pass is captured together with its forward pass, not
+while an eager graph of the same leaves lives.)
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -322,6 +324,7 @@ class _Linear(torch.autograd.Function):
         return matmul(quantize(x2), wq, out_dtype=x.dtype).view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x2, codes, scales = ctx.saved_tensors
         dx, dw = _grad_products(dy.reshape(-1, dy.shape[-1]), x2, BlockScaled(codes, scales, (BLOCK, BLOCK)), *ctx.needs_input_grad)
@@ -348,6 +351,7 @@ class _NormLinear(torch.autograd.Function):
         return out, (h.view(x.shape) if residual is not None else x.view(x.shape))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dh):
         if dout is None:   # only h was used
             return dh, None, None, None, dh if ctx.with_residual else None

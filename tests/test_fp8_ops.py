@@ -301,3 +301,12 @@ def test_adamw_refuses_memory_that_overlaps(key):
 def test_adamw_refuses_betas_that_it_would_divide_by_zero_with(bad):
     with pytest.raises(ValueError, match="betas"):
         O.adamw_multi(**{**_state([5], 8, torch.bfloat16, torch.bfloat16), **HYPER, **bad})
+
+
+def test_a_second_derivative_is_refused():
+    torch.manual_seed(0)
+    x, w, nw = (torch.randn(s, requires_grad=True) for s in ((4, 130), (6, 130), (130,)))
+    for y in (F.linear(x, w), F.norm_linear(x, nw, w)[0]):
+        dx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.sum().backward()
