@@ -1,7 +1,7 @@
 // Makers of 8-bit codes (see fp8_common.cuh), all bound by HBM in bf16 and fp32 rows on 16 bytes: 16384 x 4096 bf16 with a
 // residual 72 us (6.6 TB/s; copying runs at 6.55), its backward with an addition 81 (6.7), by rows 31 (6.4), by blocks 30
-// (6.7); both ways at once 51 (5.3: 80 registers leave three CTAs to an SM, and it issues 15 instructions per value).  Rows that
-// do not begin on 16 bytes run at 2 to 3 TB/s.
+// (6.7); both ways at once 48 (5.6: 80 registers leave three CTAs to an SM, and it issues 15 instructions per value).  Rows that
+// do not begin on 16 bytes run at 2.7 to 3.6 TB/s, in fp32 at 2.8 to 4.8.
 //
 //  fp8_norm        h = x + residual, rounded to x's type; y = h * rsqrt(mean(h^2) + eps) * w as codes with a scale per 128
 //                  channels.  One CTA per row, the row in registers: x and the residual are read once, h and the codes written
@@ -434,7 +434,8 @@ extern "C" int dcpk_fp8_norm(int type, int code, const void* x, long x_pitch, co
   if (width <= 0 || width > kNormWidth || n_rows > 0x7fffffffl || (code != kCodeE4m3 && code != kCodeE5m2)) return -3;
   const bool aligned = width % 8 == 0 && x_pitch % 8 == 0 && on_16(x) && on_16(w) && (!residual || (residual_pitch % 8 == 0 && on_16(residual) && on_16(h))) &&
                        code_pitch % 16 == 0 && on_16(codes);
-  // Rows of up to 1024 channels: a warp each (up to 256 where they do not begin on 16 bytes: 16384 x 1001 45 us against 38).  Few longer rows: as many threads per row as it takes, for the shortest chain.
+  // Rows of up to 1024 channels: a warp each (up to 256 where they do not begin on 16 bytes: 16384 x 1001 45 us against 38).  Few
+  // longer rows: as many threads per row as it takes, for the shortest chain.
   const bool warps = width <= (aligned ? 1024 : 256);
   int vecs = n_rows <= 148 * 2 ? 1 : 4;
   while (vecs > 1 && threads_for(width, vecs) < 64) vecs >>= 1;
