@@ -136,18 +136,16 @@ Tensors norm8_bwd(const Tensor& h, const Tensor& w, const Tensor& rstd, const Te
   return std::vector<Tensor>{dx, dw};
 }
 
-// an operand as the product reads it; k_dim: the dimension that is added up
+// an operand; k_dim: the dimension that is added up.  The product reads it where it is if its rows begin on 16 bytes
 bool operand(const Tensor& codes, const Tensor& scales, long br, long bc, int k_dim, DcpkFp8Operand* o) {
   const long b[2] = {br, bc};
-  if (!rows_of(codes) || code_type(codes.scalar_type()) < 0 || !on_16(codes) || !dense(scales) || scales.dim() != 2 ||
+  if (!rows_of(codes) || code_type(codes.scalar_type()) < 0 || !dense(scales) || scales.dim() != 2 ||
       scales.scalar_type() != at::kFloat8_e8m0fnu || scales.device() != codes.device())
     return false;
   for (int d : {0, 1})
     if ((b[d] != 1 && b[d] != kBlock) || scales.size(d) != blocks(codes.size(d), b[d])) return false;
   if (b[k_dim] != kBlock || codes.size(0) > 0x7fffffffl || codes.size(1) > 0x7fffffffl) return false;
-  const long p = codes.size(0) > 1 ? codes.stride(0) : up(codes.size(1), 16);
-  if (p % 16) return false;
-  *o = {codes.const_data_ptr(), p, scales.const_data_ptr(), scales.stride(1 - k_dim), scales.stride(k_dim), int(codes.size(1 - k_dim)),
+  *o = {codes.const_data_ptr(), codes.size(0) > 1 ? codes.stride(0) : up(codes.size(1), 16), scales.const_data_ptr(), scales.stride(1 - k_dim), scales.stride(k_dim), int(codes.size(1 - k_dim)),
         k_dim == 0, b[1 - k_dim] == kBlock ? 7 : 0, code_type(codes.scalar_type())};
   return true;
 }
@@ -178,6 +176,24 @@ std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair
   if (add && out && !one_or_apart(*add, *out)) return std::nullopt;
   c10::DeviceGuard guard(a.device());
   Tensor result = out ? *out : empty_matrix(q.rows, p.rows, p.rows, type, a);
+  Tensor laid[2];   // operands whose rows do not begin on 16 bytes
+  const Tensor* codes[2] = {&a, &b};
+  DcpkFp8Operand* operands[2] = {&q, &p};
+  struct { const void* from; long pitch; void* to; int rows, width; } jobs[2] = {};
+  int n_jobs = 0;
+  for (int i : {0, 1}) {
+    DcpkFp8Operand& o = *operands[i];
+    if (o.pitch % 16 == 0 && on_16(*codes[i])) continue;
+    const int rows = int(codes[i]->size(0)), width = int(codes[i]->size(1));
+    laid[i] = empty_codes(rows, width, codes[i]->scalar_type(), a);
+    jobs[n_jobs++] = {o.codes, o.pitch, laid[i].data_ptr(), rows, width};
+    o.codes = laid[i].const_data_ptr();
+    o.pitch = up(width, 16);
+  }
+  if (n_jobs)
+    check(dcpk_fp8_align(jobs[0].from, jobs[0].pitch, jobs[0].to, jobs[0].rows, jobs[0].width, jobs[1].from, jobs[1].pitch, jobs[1].to, jobs[1].rows,
+                         jobs[1].width, stream()),
+          "fp8_align");
   const long bytes = dcpk_fp8_gemm_work(q.rows, p.rows, q.rows_inner, int(a.size(ka)), form);
   Tensor work;   // of this call alone
   if (bytes > 0) work = empty_vector(bytes, at::kByte, a);

@@ -30,6 +30,8 @@ int dcpk_fp8_norm(int type, int code, const void* x, long x_pitch, const void* r
 int dcpk_fp8_norm_bwd_parts(int type, long n_rows, int width, int add);
 int dcpk_fp8_norm_bwd(int type, const void* h, long h_pitch, const void* w, const float* rstd, const void* dy, long dy_pitch, const void* add,
                       long add_pitch, void* dx, float* dw, float* part, long n_rows, int width, int* status, void* stream);
+int dcpk_fp8_align(const void* from_a, long pitch_a, void* to_a, int rows_a, int width_a, const void* from_b, long pitch_b, void* to_b, int rows_b,
+                   int width_b, void* stream);
 int dcpk_fp8_gemm(const DcpkFp8Operand* q, const DcpkFp8Operand* p, int k, void* out, long out_pitch, const void* add, long add_pitch,
                   int out_type, int form, void* work, int* status, void* stream);
 long dcpk_fp8_gemm_work(long q_rows, long p_rows, int q_rows_inner, int k, int form);

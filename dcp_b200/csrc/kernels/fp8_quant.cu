@@ -410,6 +410,50 @@ fp8_quantize_kernel(const T* x, long pitch, QuantizeOut by_rows, QuantizeOut by_
   }
 }
 
+// Codes of other layouts into rows that begin on 16 bytes, as products read them: both operands of one in a launch.  A thread makes
+// chunks of 16 from the aligned pieces that hold some of them, four rows at a time.  A product of 200 x 300 x 391 takes 12 us so and
+// 9 with codes that begin on 16 bytes (43 with the layout by a call per operand), 16384 x 4096 x 14337 1092 and 881.
+struct AlignJob {
+  const uint8_t* from;
+  uint8_t* to;
+  long pitch;
+  int n_rows, width;
+};
+struct AlignJobs { AlignJob job[2]; };
+
+static constexpr int kAlignRows = 32;   // of a CTA: 8 warps, four rows each
+
+__global__ void __launch_bounds__(256) fp8_align_kernel(const __grid_constant__ AlignJobs jobs) {
+  const AlignJob& j = jobs.job[blockIdx.z];
+  const int chunk = blockIdx.x * 32 + (threadIdx.x & 31), at = chunk * 16;
+  const long to_pitch = (j.width + 15l) & ~15l;
+  grid_wait();
+  grid_let_next();
+  if (chunk > (j.width - 1) >> 4) return;
+  for (long row0 = long(blockIdx.y) * kAlignRows + (threadIdx.x >> 5); row0 < j.n_rows; row0 += long(gridDim.y) * kAlignRows) {
+    uint32_t w[4][8], past[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long row = min(row0 + 8 * i, j.n_rows - 1l);
+      const uint8_t *begin = j.from + row * j.pitch + at, *end = begin + (j.width - at);
+      past[i] = uint32_t(reinterpret_cast<uintptr_t>(begin)) & 15u;
+      const uint4* piece = reinterpret_cast<const uint4*>(begin - past[i]);
+      const uint4 a = piece[0], b = reinterpret_cast<const uint8_t*>(piece + 1) < end ? piece[1] : make_uint4(0, 0, 0, 0);
+      w[i][0] = a.x; w[i][1] = a.y; w[i][2] = a.z; w[i][3] = a.w;
+      w[i][4] = b.x; w[i][5] = b.y; w[i][6] = b.z; w[i][7] = b.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      shift_words(w[i], past[i]);
+      if (past[i] & 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[i][k] = __funnelshift_r(w[i][k], w[i][k + 1], 8);
+      if (row0 + 8 * i < j.n_rows)
+        *reinterpret_cast<uint4*>(j.to + (row0 + 8 * i) * to_pitch + at) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+    }
+  }
+}
+
 template <typename F>
 static int by_type(int type, F f) {
   return type == kTypeBf16 ? f(static_cast<const __nv_bfloat16*>(nullptr)) : type == kTypeF16 ? f(static_cast<const __half*>(nullptr))
@@ -554,4 +598,16 @@ extern "C" int dcpk_fp8_quantize(int type, int code, int ways, const void* x, lo
     };
     return aligned ? way(std::true_type()) : way(std::false_type());
   });
+}
+
+// The codes of up to two matrices into rows of whole 16 bytes (to_b null: one matrix)
+extern "C" int dcpk_fp8_align(const void* from_a, long pitch_a, void* to_a, int rows_a, int width_a, const void* from_b, long pitch_b, void* to_b,
+                              int rows_b, int width_b, void* stream) {
+  if (rows_a <= 0 || width_a <= 0 || (to_b && (rows_b <= 0 || width_b <= 0)) || !on_16(to_a) || !on_16(to_b)) return -3;
+  AlignJobs jobs = {{{static_cast<const uint8_t*>(from_a), static_cast<uint8_t*>(to_a), pitch_a, rows_a, width_a},
+                     {static_cast<const uint8_t*>(from_b), static_cast<uint8_t*>(to_b), pitch_b, to_b ? rows_b : 0, to_b ? width_b : 0}}};
+  const int rows = std::max(rows_a, jobs.job[1].n_rows), width = std::max(width_a, jobs.job[1].width);
+  const dim3 grid((width - 1) / 512 + 1, std::min((rows - 1) / kAlignRows + 1, 65535), to_b ? 2 : 1);
+  const cudaError_t rc = launch_overlapped(fp8_align_kernel, grid, 256, 0, static_cast<cudaStream_t>(stream), 1, true, jobs);
+  return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -5;
 }

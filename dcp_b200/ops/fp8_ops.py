@@ -147,11 +147,6 @@ def matmul_reference(a, b, trans_a=False, trans_b=True, out_dtype=torch.bfloat16
 
 
 # --------------------------------------------------------------------------- codes
-def _empty_codes(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
-    """Codes whose rows begin on 16 bytes, as the products read them."""
-    return torch.empty(rows, _up(cols, 16), dtype=dtype, device=device)[:, :cols]
-
-
 def _check_matrix(x: torch.Tensor, what: str) -> None:
     _need(x.dim() == 2, f"{what} has to be a matrix, not {tuple(x.shape)}")
     _need(x.dtype in _TYPES, f"{what} has to be bfloat16, float16 or float32, not {x.dtype}")
@@ -235,14 +230,6 @@ def _check_scaled(q: BlockScaled, what: str) -> None:
     _need(scales.device == codes.device, f"{what}: codes and scales on two devices")
 
 
-def _on_16(q: BlockScaled) -> BlockScaled:
-    """The operand with codes whose rows begin on 16 bytes, as the makers here lay them out."""
-    codes = _rows(q.codes)
-    if codes.data_ptr() % 16 or (codes.shape[0] > 1 and codes.stride(0) % 16):
-        codes = _empty_codes(*codes.shape, codes.dtype, codes.device).copy_(codes)
-    return q._replace(codes=codes)
-
-
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Two matrices of one shape and type whose rows are contiguous share no element; interleaved columns of one are apart."""
     (m, n), size = a.shape, a.element_size()
@@ -265,7 +252,7 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
 
     a: [M, K], or [K, M] with ``trans_a``; b: [N, K], or [K, N] without ``trans_b`` -> [M, N] in bf16, fp16 or fp32.  Along K
     both need a scale per 128 values; along the other dimension one per value or per 128.  Codes whose rows begin on 16 bytes
-    (as the makers here lay them out) are read where they are, others are copied first.  ``form``: 0 chooses the kernel, 1 and
+    (as the makers here lay them out) are read where they are, others are laid out in each call first.  ``form``: 0 chooses the kernel, 1 and
     2 name it (measurements)."""
     if out is not None:
         out_dtype = out.dtype
@@ -299,7 +286,7 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
         if m == 0 or n == 0 or k == 0:
             out = torch.empty(m, n, dtype=out_dtype, device=a.codes.device) if out is None else out
             return out.zero_() if add is None else out.copy_(add)
-        got = call(_on_16(a), _on_16(b), None if add is None else _rows(add))
+        got = call(a._replace(codes=_rows(a.codes)), b._replace(codes=_rows(b.codes)), None if add is None else _rows(add))
     return _taken(got) if out is None else (_taken(got), out)[1]
 
 

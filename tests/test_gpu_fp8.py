@@ -709,3 +709,53 @@ def test_adamw_refuses_overlapping_memory_and_betas_on_the_gpu(dev, bits):
         with pytest.raises(ValueError, match="betas"):
             O.adamw_multi(**{**st, **HYPER, **bad})
     assert int(st["step"]) == int(kept["step"]) and all(torch.equal(_bits(a), _bits(b)) for a, b in zip(st["params"], kept["params"]))
+
+
+def _laid(q, offset, pitch):
+    """The operand with its codes `offset` bytes behind an aligned address, rows `pitch` bytes apart."""
+    rows, cols = q.codes.shape
+    pitch = max(pitch, cols)
+    buf = torch.full((offset + rows * pitch + 64,), 0x7F, dtype=torch.uint8, device=q.codes.device)   # NaN all around
+    codes = buf[offset:].as_strided((rows, cols), (pitch, 1), offset)
+    codes.copy_(q.codes.contiguous().view(torch.uint8))
+    return q._replace(codes=codes.view(q.codes.dtype))
+
+
+@pytest.mark.parametrize("how", ["forward", "dgrad", "wgrad"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 65, 17), (33, 130, 129), (130, 257, 1001), (513, 64, 15), (300, 1030, 511)])
+def test_products_of_codes_that_do_not_begin_on_16_bytes(dev, how, m, n, k):
+    a, b = _values(*((k, m) if how == "wgrad" else (m, k)), torch.bfloat16, dev), _values(*((n, k) if how == "forward" else (k, n)), torch.bfloat16, dev, 1)
+    qa = F.quantize(a, (128, 1) if how == "wgrad" else (1, 128))
+    qb = F.quantize(b, (128, 1) if how == "wgrad" else (128, 128), E5M2)
+    call = lambda a, b: F.matmul(a, b, trans_a=how == "wgrad", trans_b=how == "forward")  # noqa: E731
+    want = call(qa, qb)
+    assert not torch.isnan(want).any()
+    for offset, extra in ((0, 0), (1, 0), (8, 3), (15, 16), (16, 1), (6, 2)):
+        pa, pb = qa.codes.shape[1] + extra, qb.codes.shape[1] + extra
+        for x, y in ((_laid(qa, offset, pa), _laid(qb, 16 - offset, pb)), (qa, _laid(qb, offset, pb)), (_laid(qa, offset, pa), qb)):
+            assert torch.equal(call(x, y), want), (offset, extra)
+    for x, y in ((qa._replace(codes=qa.codes.t().contiguous().t()), qb), (qa, qb._replace(codes=qb.codes.t().contiguous().t()))):   # by columns
+        assert torch.equal(call(x, y), want)
+
+
+def test_codes_laid_out_inside_a_graph_and_beside_another_stream(dev):
+    m, n, k = 200, 300, 391
+    qa, qb = (F.quantize(_values(r, k, torch.bfloat16, dev, r), b) for r, b in ((m, (1, 128)), (n, (128, 128))))
+    x, y = _laid(qa, 3, k), _laid(qb, 5, k)
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros(m, n, dtype=torch.bfloat16, device=dev)
+    want = F.matmul(qa, qb)
+    with torch.cuda.graph(graph):
+        F.matmul(x, y, out=out)
+    other = F.quantize(_values(m, k, torch.bfloat16, dev, 9))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = F.matmul(_laid(other, 1, k), y)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(beside, F.matmul(other, qb))
+    x.codes.view(torch.uint8).copy_(other.codes.contiguous().view(torch.uint8))   # a replay lays out what is there then
+    x.scales.view(torch.uint8).copy_(other.scales.view(torch.uint8))
+    graph.replay()
+    assert torch.equal(out, F.matmul(other, qb))
