@@ -26,6 +26,7 @@ using at::Tensor;
 namespace {
 
 constexpr long kBlock = 128, kStateBlock = 256, kNormWidth = 16384;
+constexpr long kMaxRows = 0x7fffffff, kMaxBlocked = kMaxRows - (kBlock - 1);   // the kernels count in ints, in whole blocks along a block
 
 void check(int rc, const char* what) {
   if (rc != 0) throw std::runtime_error(std::string(what) + " failed with code " + std::to_string(rc));
@@ -72,7 +73,7 @@ using Tensors = std::optional<std::vector<Tensor>>;
 
 // codes and scales, of ways 1 and 2 in this order; ways as dcpk_fp8_quantize has them
 Tensors quantize8(const Tensor& x, int ways, bool e5m2) {
-  if (!rows_of(x) || value_type(x.scalar_type()) < 0) return std::nullopt;
+  if (!rows_of(x) || value_type(x.scalar_type()) < 0 || x.size(0) > kMaxRows || x.size(1) > kMaxBlocked) return std::nullopt;
   c10::DeviceGuard guard(x.device());
   const long rows = x.size(0), cols = x.size(1);
   const at::ScalarType type = e5m2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn;
@@ -144,7 +145,7 @@ bool operand(const Tensor& codes, const Tensor& scales, long br, long bc, int k_
     return false;
   for (int d : {0, 1})
     if ((b[d] != 1 && b[d] != kBlock) || scales.size(d) != blocks(codes.size(d), b[d])) return false;
-  if (b[k_dim] != kBlock || codes.size(0) > 0x7fffffffl || codes.size(1) > 0x7fffffffl) return false;
+  if (b[k_dim] != kBlock || codes.size(k_dim) > kMaxBlocked || codes.size(1 - k_dim) > kMaxRows) return false;
   *o = {codes.const_data_ptr(), codes.size(0) > 1 ? codes.stride(0) : up(codes.size(1), 16), scales.const_data_ptr(), scales.stride(1 - k_dim), scales.stride(k_dim), int(codes.size(1 - k_dim)),
         k_dim == 0, b[1 - k_dim] == kBlock ? 7 : 0, code_type(codes.scalar_type())};
   return true;

@@ -30,6 +30,8 @@ from . import _lib
 BLOCK = 128
 E4M3, E5M2, E8M0 = torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e8m0fnu
 MAX_NORM_WIDTH = 16384
+MAX_ROWS = 2 ** 31 - 1
+MAX_BLOCKED = MAX_ROWS - (BLOCK - 1)    # columns of a quantizer, and what a product adds up: whole blocks are counted in 32 bits
 _CODES = {E4M3: 0, E5M2: 1}
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _KINDS = {(1, BLOCK): 1, (BLOCK, 1): 2, (BLOCK, BLOCK): 4}
@@ -158,6 +160,7 @@ def _quantize(x: torch.Tensor, ways: int, dtype: torch.dtype):
     if got is None:
         _check_matrix(x, "x")
         _need(dtype in _CODES, f"codes are float8_e4m3fn or float8_e5m2, not {dtype}")
+        _need(x.shape[0] <= MAX_ROWS and x.shape[1] <= MAX_BLOCKED, f"up to {MAX_ROWS} rows of {MAX_BLOCKED} columns, not {tuple(x.shape)}")
         if not x.is_cuda:
             return [quantize_reference(x, k, dtype) for k in kinds]
         got = _native().quantize8(_rows(x), ways, dtype == E5M2)
@@ -166,7 +169,8 @@ def _quantize(x: torch.Tensor, ways: int, dtype: torch.dtype):
 
 
 def quantize(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK), dtype: torch.dtype = E4M3) -> BlockScaled:
-    """Codes of a matrix (bf16, fp16 or fp32, any pitch) with a scale per block: (1, 128), (128, 1) or (128, 128)."""
+    """Codes of a matrix (bf16, fp16 or fp32, any pitch) with a scale per block: (1, 128), (128, 1) or (128, 128).  Up to 2^31 - 128
+    columns: a longer flat buffer is viewed as several rows."""
     _need(tuple(block) in _KINDS, f"blocks are (1, 128), (128, 1) or (128, 128), not {block}")
     return _quantize(x, _KINDS[tuple(block)], dtype)[0]
 
@@ -267,6 +271,7 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
         ka, kb = (0 if trans_a else 1), (1 if trans_b else 0)
         m, n, k = a.codes.shape[1 - ka], b.codes.shape[1 - kb], a.codes.shape[ka]
         _need(k == b.codes.shape[kb], f"contraction over {k} values of a and {b.codes.shape[kb]} of b")
+        _need(k <= MAX_BLOCKED and m <= MAX_ROWS and n <= MAX_ROWS, f"sums of up to {MAX_BLOCKED} values and up to {MAX_ROWS} rows and columns, not {(m, n, k)}")
         _need(a.block[ka] == BLOCK and b.block[kb] == BLOCK, "both operands need a scale per 128 values along the contraction")
         _need(a.codes.device == b.codes.device, "a and b are on two devices")
         _need(form in (0, 1, 2), "form is 0, 1 or 2")

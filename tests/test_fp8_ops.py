@@ -310,3 +310,20 @@ def test_a_second_derivative_is_refused():
         dx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             dx.sum().backward()
+
+
+def _too_wide(device="cpu"):
+    """Calls with more columns than the kernels count, of tensors that take no memory."""
+    wide, one = 2 ** 31, lambda dtype: torch.zeros(1, dtype=torch.uint8 if dtype.itemsize == 1 else dtype, device=device).view(dtype)  # noqa: E731
+    x = one(torch.bfloat16).expand(1, wide)
+    scaled = lambda rows, k: F.BlockScaled(one(E4M3).expand(rows, k), one(F.E8M0).expand(rows, -(-k // 128)), (1, 128))  # noqa: E731
+    for call in (lambda: F.quantize(x), lambda: F.quantize(x, (128, 1)), lambda: F.quantize(x, (128, 128)), lambda: F.quantize_both(x),
+                 lambda: F.quantize(one(torch.bfloat16).expand(1, 2 ** 33)), lambda: F.quantize(x[:, :wide - 127]),
+                 lambda: F.quantize(x.t()), lambda: F.matmul(scaled(2, wide - 127), scaled(3, wide - 127)),
+                 lambda: F.matmul(scaled(2, 2 ** 33), scaled(3, 2 ** 33))):
+        with pytest.raises(ValueError, match="up to 2147483"):
+            call()
+
+
+def test_more_columns_than_the_kernels_count_are_refused():
+    _too_wide()

@@ -759,3 +759,8 @@ def test_codes_laid_out_inside_a_graph_and_beside_another_stream(dev):
     x.scales.view(torch.uint8).copy_(other.scales.view(torch.uint8))
     graph.replay()
     assert torch.equal(out, F.matmul(other, qb))
+
+
+def test_more_columns_than_the_kernels_count_are_refused_on_the_gpu(dev):
+    from test_fp8_ops import _too_wide
+    _too_wide(dev)
