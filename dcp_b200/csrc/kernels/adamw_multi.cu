@@ -225,13 +225,45 @@ __device__ __forceinline__ uint2 encode8(float amax, const float (&f)[8], const 
   return make_uint2(four(0), four(4));
 }
 
-// Sum of squares of a CTA's gradients, from the threads' sums on in 64 bits; `parts` are added up in order.  A CTA has a
-// run of chunks, so that it looks for its tensor once and has four loads per thread under way (a chunk at a time from a
-// grid of CTAs: 436 MB in 144 us).
+// Sum of squares of 8 kN values, in fp32 for these few and from there on in 64 bits.  fp32 does not hold a square above 2^128 and
+// rounds one below 2^-126 to a multiple of 2^-149, so where the sum is not finite or below 2^-100 (against which 32 such
+// roundings do not count) it is taken again in 64 bits, from the gradients on: a single gradient of 1e20 would make the norm
+// infinite, and what it clips zero.
+template <typename G, int kN>
+__device__ __forceinline__ double sum_of_squares(const Raw8<G> (&raw)[kN], float scale) {
+  float sq[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < kN; ++u) {
+    float g[8];
+    widen(raw[u], g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = g[j] * scale;
+      sq[j] += x * x;
+    }
+  }
+  const float sum = ((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7]));
+  if (sum >= 0x1p-100f && sum < INFINITY) return double(sum);
+  double wide = 0.0;
+#pragma unroll
+  for (int u = 0; u < kN; ++u) {
+    float g[8];
+    widen(raw[u], g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double x = double(g[j]) * double(scale);
+      wide += x * x;
+    }
+  }
+  return wide;
+}
+
+// Sum of squares of a CTA's gradients; `parts` are added up in order.  A CTA has a run of chunks, so that it looks for its tensor
+// once and has four loads per thread under way (a chunk at a time from a grid of CTAs: 436 MB in 144 us).
 template <typename G>
 __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_constant__ AdamList list, float grad_scale, double* parts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_chunks = list.first_chunk[list.n];
-  float sq[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  double t = 0.0;
   grid_wait();
   int chunk = int(long(n_chunks) * blockIdx.x / gridDim.x);
   const int stop = int(long(n_chunks) * (blockIdx.x + 1) / gridDim.x);
@@ -241,37 +273,22 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
     const G* grad = static_cast<const G*>(list.t[i].grad);
     long e0 = long(chunk - list.first_chunk[i]) * kChunk;
     const long end = min(n, long(last - list.first_chunk[i]) * kChunk);
-    const auto add = [&](const float (&g)[8]) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = g[j] * grad_scale;
-        sq[j] += x * x;
-      }
-    };
     if (list.aligned[i])
       for (; e0 + 4 * kChunk <= end; e0 += 4 * kChunk) {
         Raw8<G> raw[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) load_raw(raw[u], grad + e0 + u * kChunk + threadIdx.x * 8);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float g[8];
-          widen(raw[u], g);
-          add(g);
-        }
+        t += sum_of_squares(raw, grad_scale);
       }
     for (; e0 < end; e0 += kChunk) {
       const long at = e0 + warp * kStateBlock;
-      float g[8];
-      load8(grad, at, lane, n, list.aligned[i] && at + kStateBlock <= n, g);
-      add(g);
+      Raw8<G> raw[1];
+      load8(grad, at, lane, n, list.aligned[i] && at + kStateBlock <= n, raw[0]);
+      t += sum_of_squares(raw, grad_scale);
     }
     chunk = last;
   }
   grid_let_next();
-  double t = 0.0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) t += double(sq[j]);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
   __shared__ double warps[kAdamThreads / 32];

@@ -764,3 +764,62 @@ def test_codes_laid_out_inside_a_graph_and_beside_another_stream(dev):
 def test_more_columns_than_the_kernels_count_are_refused_on_the_gpu(dev):
     from test_fp8_ops import _too_wide
     _too_wide(dev)
+
+
+def _exact_adamw(st, coef, hyper=HYPER):
+    """Weights and moments after a step in 64 bits, of a state before it."""
+    t = int(st["step"]) + 1
+    out = []
+    for i, g in enumerate(st["grads"]):
+        w, g = _weights(st)[i], g.double() * coef
+        m, v = (st["m"][i].double(), st["v"][i].double()) if "m_scales" not in st else \
+            (O.decode_state(st["m"][i], st["m_scales"][i]).double(), O.decode_state(st["v"][i], st["v_scales"][i]).double().square())
+        m, v = hyper["beta1"] * m + (1 - hyper["beta1"]) * g, hyper["beta2"] * v + (1 - hyper["beta2"]) * g * g
+        step = hyper["lr"] * (m / (1 - hyper["beta1"] ** t)) / ((v / (1 - hyper["beta2"] ** t)).sqrt() + hyper["eps"])
+        out.append((w - step - hyper["lr"] * hyper["weight_decay"] * w, m, v, step))
+    return out
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("gtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("at", [5, 9_000, 20_479, 30_001])
+def test_adamw_clips_a_gradient_whose_square_fp32_does_not_hold(dev, bits, gtype, offset, at):
+    st = _adam_state([300, 30_002], bits, torch.bfloat16, gtype, dev, offset)
+    st["grads"][1][at] = -1e20
+    before = _copy(st)
+    length = sum(g.double().square().sum() for g in before["grads"]).sqrt().item()
+    norm = O.adamw_multi(**st, **HYPER, clip=0.5)
+    # Squares in fp32: one rounding each, four added in turn and eight of these by pairs (the first addition is to zero): seven
+    # roundings at most of the sum, half of that of its root, which is rounded once.
+    assert abs(norm.item() / length - 1) <= 4.5 * 2.0 ** -24
+    for i, (w, m, v, step) in enumerate(_exact_adamw(before, 0.5 / (length + 1e-6))):
+        # The coefficient carries the norm's error and three roundings (itself, the scaled one, the gradient's product): 8 * 2^-24
+        # of m's part, 16 of v's; with the roundings of the sums below 2^-19.  m's terms may cancel.
+        terms = 0.9 * (before["m"][i].double() if bits == 32 else O.decode_state(before["m"][i], before["m_scales"][i]).double()).abs() \
+            + 0.1 * before["grads"][i].double().abs() * 0.5 / length
+        near = step.abs() * (terms / m.abs().clamp(min=1e-300)).clamp(min=1.0) * 2.0 ** -18
+        assert ((_weights(st)[i] - w).abs() <= near + w.abs() * 2.0 ** -23).all()
+        if bits == 32:
+            assert ((st["m"][i].double() - m).abs() <= terms * 2.0 ** -19).all() and ((st["v"][i].double() - v).abs() <= v * 2.0 ** -19).all()
+    assert (_weights(st)[1][at] - _weights(before)[1][at]).item() > 0     # by about lr
+
+
+@pytest.mark.parametrize("gtype,size", [(torch.float32, 1e-25), (torch.float32, 1e-41), (torch.bfloat16, 1e-25), (torch.bfloat16, 1e30), (torch.float16, 6e-8),
+                                        (torch.float32, 0.0)])
+def test_adamw_norm_of_tiny_and_huge_gradients(dev, gtype, size):
+    st = _adam_state([77, 50_000], 32, torch.float32, gtype, dev)
+    for g in st["grads"]:
+        g.copy_(torch.randn(g.shape, device=dev) * size)
+    want = sum(g.double().square().sum() for g in st["grads"]).sqrt().item()
+    norm = O.adamw_multi(**st, **HYPER, clip=1.0).item()
+    assert abs(norm - want) <= want * 4.5 * 2.0 ** -24 + 2.0 ** -150     # fp32's smallest values lie 2^-149 apart
+
+
+def test_adamw_norm_of_many_values(dev):
+    n = 100_000_003
+    g = torch.empty(n, dtype=torch.bfloat16, device=dev).normal_(generator=torch.Generator(device=dev).manual_seed(1))
+    w, m, v, step = torch.zeros(n, device=dev), torch.zeros(n, device=dev), torch.zeros(n, device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    norm = O.adamw_multi([w], [g], None, [m], [v], step, **HYPER, clip=1.0).item()
+    want = sum(part.double().square().sum().item() for part in g.split(1 << 24)) ** 0.5
+    assert abs(norm / want - 1) <= 4.5 * 2.0 ** -24
