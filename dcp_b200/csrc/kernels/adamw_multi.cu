@@ -168,7 +168,8 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, long e0, int lane, long
   }
 }
 // Square root by one step of Newton's iteration with the residual of a fused product: to nearest but for one value in a
-// million, without sqrtf's branch for the ends of the range.  Zero for zero; below 2^-126 too small.
+// million, without sqrtf's branch for the ends of the range.  Zero for zero; below 2^-126 too small, NaN for infinity: those
+// take sqrtf.
 __device__ __forceinline__ float root_of(float v) {
   float y;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(v, 1.17549435e-38f)));
@@ -352,6 +353,7 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 5) adamw_multi_kern
   grid_wait();
   if (shared->skip) return;
   const float coef = shared->coef, bc1 = shared->bc1, root_bc2 = shared->root_bc2;
+  const bool small_numbers = kEight && (s.eps < root_bc2 * 0x1p-37f || s.beta2 < 0x1p-10f);   // see update()
   int chunk = blockIdx.x;
   for (int i = find_tensor(list, chunk); chunk < n_chunks; ++i) {
     const AdamTensor& t = list.t[i];
@@ -370,28 +372,29 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 5) adamw_multi_kern
         b.m_byte = t.m_scale[e0 / kStateBlock];
         b.v_byte = t.v_scale[e0 / kStateBlock];
       };
-      const auto update = [&](const Block8<G>& b, long e0, bool vec) {
-        float w[8], m[8], v[8], root[8], g[8];
+      // kWide: for blocks near the ends of fp32's range
+      const auto body = [&](const Block8<G>& b, const float (&g)[8], long e0, bool vec, auto wide) {
+        constexpr bool kWide = decltype(wide)::value;
+        float w[8], m[8], v[8], root[8];
         // the scales are powers of two: they go into the factors the codes are multiplied with anyway
         const float keep_m = s.beta1 * scale_value(b.m_byte), v_scale = scale_value(b.v_byte), keep_v = s.beta2 * v_scale * v_scale;
-        widen(b.grad, g);
         widen_codes(b.m, m);
         widen_codes(b.v, v);
         uint32_t random[8];
         float m_max = 0.f, v_max = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          g[j] *= coef;
           // each rounded by itself: old moments and gradients are short numbers, so blocks whose largest value lies on the
           // very border between two scales are not rare, and a fused product would take them to the other side than the
           // formula
           m[j] = __fadd_rn(__fmul_rn(keep_m, m[j]), __fmul_rn(s.rest1, g[j]));
-          v[j] = __fadd_rn(__fmul_rn(keep_v, v[j] * v[j]), __fmul_rn(__fmul_rn(s.rest2, g[j]), g[j]));
+          const float old = kWide ? v[j] * v_scale : v[j];
+          v[j] = __fadd_rn(__fmul_rn(kWide ? s.beta2 : keep_v, __fmul_rn(old, old)), __fmul_rn(__fmul_rn(s.rest2, g[j]), g[j]));
           if (j & 1) {
             m_max = max3_abs(m_max, m[j - 1], m[j]);
             v_max = max3_abs(v_max, v[j - 1], v[j]);
           }
-          root[j] = root_of(v[j]);
+          root[j] = kWide ? sqrtf(v[j]) : root_of(v[j]);
           w[j] = b.w[j] - s.lr * (m[j] * bc1 * inverse_approx(root[j] * root_bc2 + s.eps) + s.wd * b.w[j]);
           random[j] = mix32_open(uint32_t(e0 + (vec ? lane * 8 + j : j * 32 + lane)) * 0x9e3779b1u + key);
         }
@@ -406,6 +409,22 @@ __global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 5) adamw_multi_kern
           t.m_scale[e0 / kStateBlock] = uint8_t(m_byte);
           t.v_scale[e0 / kStateBlock] = uint8_t(v_byte);
         }
+      };
+      // A v may overflow (its root is infinite and moves nothing), lie below 2^-126 (beside a root above 2^-45 in its block such a
+      // root has the smallest code whatever it is, and beside eps it does not count, unless that is small), or come of a
+      // scale whose square times beta2 leaves fp32's normal range.  The gradients and the old scale tell where none of it can
+      // be: v >= beta2 (224 scale)^2 and (1 - beta2) g^2.
+      const auto update = [&](const Block8<G>& b, long e0, bool vec) {
+        float g[8], g_max = 0.f;
+        widen(b.grad, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          g[j] *= coef;
+          if (j & 1) g_max = max3_abs(g_max, g[j - 1], g[j]);
+        }
+        const bool wide = !(g_max < 0x1p60f) || (b.v_byte == 0 && g_max < 0x1p-30f && g_max > 0.f);
+        if (__any_sync(0xffffffffu, wide) || uint32_t(b.v_byte - 1) < 79u || b.v_byte > 180 || small_numbers) body(b, g, e0, vec, std::true_type());
+        else body(b, g, e0, vec, std::false_type());
       };
       // whole blocks, the next one's loads under way while this one is worked on; then the tensor's end, or all of it where
       // it is not aligned
