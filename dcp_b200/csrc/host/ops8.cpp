@@ -26,6 +26,7 @@ using at::Tensor;
 namespace {
 
 constexpr long kBlock = 128, kStateBlock = 256, kNormWidth = 16384;
+constexpr size_t kStatusWords = 4;
 constexpr long kMaxRows = 0x7fffffff, kMaxBlocked = kMaxRows - (kBlock - 1);   // the kernels count in ints, in whole blocks along a block
 
 void check(int rc, const char* what) {
@@ -215,7 +216,7 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
   const std::tuple<bool, std::optional<Tensor>> no{false, std::nullopt};
   const size_t n = params.size();
   if (n == 0 || n > 0x7fffffff || grads.size() != n || m.size() != n || v.size() != n || (masters && masters->size() != n) ||
-      bool(m_scales) != bool(v_scales) || (m_scales && (m_scales->size() != n || v_scales->size() != n)) || status.size() > 2 || !(clip >= 0) ||
+      bool(m_scales) != bool(v_scales) || (m_scales && (m_scales->size() != n || v_scales->size() != n)) || status.size() > kStatusWords || !(clip >= 0) ||
       (clip > 0 && factor) || !(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1))
     return no;
   const auto device = params[0].device();
@@ -261,11 +262,12 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
   Tensor work = empty_vector(dcpk_adamw_multi_work(int(n)), at::kDouble, step);
   std::optional<Tensor> norm;
   if (clip > 0) norm = empty_vector(1, at::kFloat, step);
-  const int* words[2] = {status.size() > 0 ? status[0].const_data_ptr<int>() : nullptr, status.size() > 1 ? status[1].const_data_ptr<int>() : nullptr};
+  const int* words[kStatusWords] = {};
+  for (size_t i = 0; i < status.size(); ++i) words[i] = status[i].const_data_ptr<int>();
   check(dcpk_adamw_multi(int(n), p.data(), g.data(), masters ? w.data() : nullptr, pm.data(), pv.data(), m_scales ? sm.data() : nullptr,
                          m_scales ? sv.data() : nullptr, sizes.data(), ptype, gtype, step.data_ptr<int64_t>(), float(lr), beta1, beta2,
                          float(eps), float(wd), float(grad_scale), float(clip), factor ? factor->const_data_ptr<float>() : nullptr, seed,
-                         norm ? norm->data_ptr<float>() : nullptr, words[0], words[1], work.data_ptr<double>(), stream()),
+                         norm ? norm->data_ptr<float>() : nullptr, words, int(status.size()), work.data_ptr<double>(), stream()),
         "adamw_multi");
   return {true, norm};
 }

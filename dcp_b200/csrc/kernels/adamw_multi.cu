@@ -50,6 +50,8 @@ struct AdamList {
   int n, base;               // base: tensors in launches before
 };
 struct AdamScalars { float lr, beta1, rest1, beta2, rest2, eps, wd; };   // rest: 1 - beta
+static constexpr int kAdamStatus = 4;
+struct AdamStatus { const int* word[kAdamStatus]; };   // null: none
 // what a step's kernels hand on, in global memory
 struct AdamShared { float coef, bc1, root_bc2; uint32_t key; int skip; };
 
@@ -305,8 +307,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
 // step counter, bias corrections, clipping coefficient: one CTA
 __global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* parts, int n_parts, int64_t* step, double beta1,
                                                             double beta2, float grad_scale, float clip, const float* factor,
-                                                            uint32_t seed, float* norm, const int* status_a,
-                                                            const int* status_b, AdamShared* shared) {
+                                                            uint32_t seed, float* norm, const AdamStatus status, AdamShared* shared) {
   __shared__ double sums[8];
   grid_wait();
   grid_let_next();
@@ -319,7 +320,9 @@ __global__ void __launch_bounds__(256) adamw_prepare_kernel(const double* parts,
   if (threadIdx.x) return;
 #pragma unroll
   for (int w = 1; w < 8; ++w) t += sums[w];
-  const bool skip = (status_a && *status_a != 0) || (status_b && *status_b != 0);
+  bool skip = false;
+#pragma unroll
+  for (int i = 0; i < kAdamStatus; ++i) skip |= status.word[i] && *status.word[i] != 0;
   const int64_t now = *step + 1;
   if (!skip) *step = now;
   shared->skip = skip;
@@ -480,12 +483,15 @@ extern "C" long dcpk_adamw_multi_work(int n_tensors) { return kAdamHead + long((
 // Tensors of one parameter type and one gradient type (0 fp32, 1 fp16, 2 bf16); an entry of `masters` may be null for fp32
 // parameters only.  m_scales null: moments in fp32; otherwise codes with ceil(n / 256) scales.  step: one int64 on the
 // device, counted up.  clip <= 0: none, and norm is not written.  factor: null, or one float on the device that the gradients
-// are multiplied with.  status_a, status_b: null, or words that, when one is not zero, leave everything as it is.
+// are multiplied with.  status: up to four words that, when one is not zero, leave everything as it is.
 extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* const* grads, void* const* masters, void* const* ms,
                                 void* const* vs, void* const* m_scales, void* const* v_scales, const long* sizes, int param_type, int grad_type,
                                 int64_t* step, float lr, double beta1, double beta2, float eps, float wd, float grad_scale, float clip,
-                                const float* factor, unsigned seed, float* norm, const int* status_a, const int* status_b, double* work,
+                                const float* factor, unsigned seed, float* norm, const int* const* status, int n_status, double* work,
                                 void* stream) {
+  if (n_status < 0 || n_status > kAdamStatus) return -3;
+  AdamStatus words;
+  for (int i = 0; i < kAdamStatus; ++i) words.word[i] = i < n_status ? status[i] : nullptr;
   if (n_tensors < 0 || param_type < 0 || param_type > 2 || grad_type < 0 || grad_type > 2) return -3;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   AdamShared* shared = reinterpret_cast<AdamShared*>(work);
@@ -536,7 +542,7 @@ extern "C" int dcpk_adamw_multi(int n_tensors, void* const* params, const void* 
     }
   if (clip > 0.f && n_parts == 0 && cudaMemsetAsync(norm, 0, 4, s) != cudaSuccess) return -5;
   if (launch_overlapped(adamw_prepare_kernel, dim3(1), 256, 0, s, 1, !first, static_cast<const double*>(parts), n_parts, step, beta1, beta2,
-                        grad_scale, clip, factor, uint32_t(seed), norm, status_a, status_b, shared) != cudaSuccess || cudaGetLastError() != cudaSuccess)
+                        grad_scale, clip, factor, uint32_t(seed), norm, words, shared) != cudaSuccess || cudaGetLastError() != cudaSuccess)
     return -5;
   const AdamScalars scalars = {lr, float(beta1), float(1.0 - beta1), float(beta2), float(1.0 - beta2), eps, wd};
   for (int base = 0; base < n_tensors;) {

@@ -39,7 +39,7 @@ long dcpk_adamw_multi_work(int n_tensors);
 int dcpk_adamw_multi(int n_tensors, void* const* params, const void* const* grads, void* const* masters, void* const* ms, void* const* vs,
                      void* const* m_scales, void* const* v_scales, const long* sizes, int param_type, int grad_type, int64_t* step, float lr,
                      double beta1, double beta2, float eps, float wd, float grad_scale, float clip, const float* factor, unsigned seed,
-                     float* norm, const int* status_a, const int* status_b, double* work, void* stream);
+                     float* norm, const int* const* status, int n_status, double* work, void* stream);
 int dcpk_attn_fwd_pair(const void* q_arena, long q_rows, const void* kv_arena, long kv_rows, int hq, int hkv, const void* tiles,
                        int n_tiles, const void* kv_entries, int n_kv_entries, const void* masks, int n_mask_rows,
                        void* const* out_ptrs, float* const* lse_ptrs, int n_dst, int lse_stride_a, int lse_stride_b, int n_dst_a,

@@ -16,7 +16,7 @@
 // written its gradients, so the reduction overlaps the rest of the backward pass.
 //
 // Failure containment: every kernel that changes optimizer state or parameters takes the status
-// words of the arenas whose barriers guard its inputs; if either is nonzero (a barrier wait ran
+// words of what its inputs come from (the arenas whose barriers guard them, the 8-bit products); if one is nonzero (a wait ran
 // out, a table was bad) the kernel returns without touching master weights, moments, main
 // gradients or parameters, so a detected failure never reaches the weights.
 #include <cuda_bf16.h>
@@ -30,11 +30,14 @@ namespace dcpk {
 static constexpr int kMaxRanks = 16;
 struct GradPtrs { const void* p[kMaxRanks]; };
 struct ParamPtrs { void* p[kMaxRanks]; };
-struct StatusPtrs { const int* a; const int* b; };
+static constexpr int kMaxStatus = 4;
+struct StatusPtrs { const int* p[kMaxStatus]; };   // null: none
 
 __device__ __forceinline__ bool failed(const StatusPtrs& st) {
-  return (st.a && *reinterpret_cast<const volatile int*>(st.a) != 0) ||
-         (st.b && *reinterpret_cast<const volatile int*>(st.b) != 0);
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < kMaxStatus; ++i) any |= st.p[i] && *reinterpret_cast<const volatile int*>(st.p[i]) != 0;
+  return any;
 }
 
 // One element of AdamW; bc1 / bc2 are the reciprocals of the bias corrections.  One square root and one division
@@ -241,6 +244,12 @@ __global__ void cast_all_gather_kernel(const float* __restrict__ master, ParamPt
 
 using namespace dcpk;
 
+static bool status_ptrs(StatusPtrs& st, const int* const* words, int n) {
+  if (n < 0 || n > kMaxStatus) return false;
+  for (int i = 0; i < kMaxStatus; ++i) st.p[i] = i < n ? words[i] : nullptr;
+  return true;
+}
+
 extern "C" int dcpk_grad_sqnorm(const void* const* grad_ptrs, int world, long shard_off, long shard_len, float scale,
                                 double* sq_norm, void* stream) {
   if (shard_len <= 0) return 0;
@@ -263,9 +272,10 @@ extern "C" int dcpk_clip_coef(const double* sum, float* sq_norm, float clip, flo
 extern "C" int dcpk_fused_rs_adamw_ag(const void* const* grad_ptrs, void* const* param_ptrs, int world, long shard_off,
                                       long shard_len, float scale, float* master, float* m, float* v, float lr,
                                       float beta1, float beta2, float eps, float wd, int step, const float* clip_coef,
-                                      const int* status_a, const int* status_b, void* stream) {
+                                      const int* const* status, int n_status, void* stream) {
   if (shard_len <= 0) return 0;
-  if (world > kMaxRanks || shard_off % 8 || shard_len % 8) return -3;
+  StatusPtrs st;
+  if (world > kMaxRanks || shard_off % 8 || shard_len % 8 || !status_ptrs(st, status, n_status)) return -3;
   GradPtrs g;
   ParamPtrs p;
   for (int i = 0; i < kMaxRanks; ++i) {
@@ -276,7 +286,7 @@ extern "C" int dcpk_fused_rs_adamw_ag(const void* const* grad_ptrs, void* const*
   // 864 threads per SM: 1024 read and write 5 % slower when nothing else limits them (1.29 against 1.22 ms for 268M)
   fused_rs_adamw_ag_kernel<<<148 * 3, 288, 0, static_cast<cudaStream_t>(stream)>>>(
       g, p, world, size_t(shard_off), size_t(shard_len), scale, master, m, v, lr, beta1, beta2, eps, wd, bc1, bc2,
-      clip_coef, StatusPtrs{status_a, status_b});
+      clip_coef, st);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
@@ -284,28 +294,30 @@ extern "C" int dcpk_fused_rs_adamw_ag(const void* const* grad_ptrs, void* const*
 // grid so it trickles over NVLink next to the GEMMs instead of taking their SMs.
 extern "C" int dcpk_grad_reduce_scatter(const void* const* grad_ptrs, int world, long shard_off, long shard_len,
                                         float scale, float* main_grad, float* sq_norm, int n_ctas,
-                                        const int* status_a, const int* status_b, void* stream) {
+                                        const int* const* status, int n_status, void* stream) {
   if (shard_len <= 0) return 0;
-  if (world > kMaxRanks || shard_off % 8 || shard_len % 8) return -3;
+  StatusPtrs st;
+  if (world > kMaxRanks || shard_off % 8 || shard_len % 8 || !status_ptrs(st, status, n_status)) return -3;
   GradPtrs g;
   for (int i = 0; i < kMaxRanks; ++i) g.p[i] = i < world ? grad_ptrs[i] : nullptr;
   grad_reduce_scatter_kernel<<<n_ctas > 0 ? n_ctas : 148 * 4, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      g, world, size_t(shard_off), size_t(shard_len), scale, main_grad, sq_norm, StatusPtrs{status_a, status_b});
+      g, world, size_t(shard_off), size_t(shard_len), scale, main_grad, sq_norm, st);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
 extern "C" int dcpk_adamw_all_gather(float* master, float* m, float* v, const float* grad, void* const* param_ptrs,
                                      int world, long shard_off, long shard_len, float lr, float beta1, float beta2,
-                                     float eps, float wd, int step, const float* clip_coef, const int* status_a,
-                                     const int* status_b, void* stream) {
+                                     float eps, float wd, int step, const float* clip_coef,
+                                     const int* const* status, int n_status, void* stream) {
   if (shard_len <= 0) return 0;
-  if (world > kMaxRanks || shard_off % 8 || shard_len % 8) return -3;
+  StatusPtrs st;
+  if (world > kMaxRanks || shard_off % 8 || shard_len % 8 || !status_ptrs(st, status, n_status)) return -3;
   ParamPtrs p;
   for (int i = 0; i < kMaxRanks; ++i) p.p[i] = i < world ? param_ptrs[i] : nullptr;
   const float bc1 = 1.f / (1.f - powf(beta1, float(step))), bc2 = 1.f / (1.f - powf(beta2, float(step)));
   adamw_all_gather_kernel<<<148 * 4, 256, 0, static_cast<cudaStream_t>(stream)>>>(
       master, m, v, grad, p, world, size_t(shard_off), size_t(shard_len), lr, beta1, beta2, eps, wd, bc1, bc2,
-      clip_coef, StatusPtrs{status_a, status_b});
+      clip_coef, st);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 

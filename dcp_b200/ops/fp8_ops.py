@@ -98,6 +98,15 @@ def _status(device: torch.device) -> torch.Tensor:
     return _STATUS[device.index]
 
 
+def status_word(device: torch.device) -> torch.Tensor:
+    """The int32 word of a device that the products and the norm's backward pass report a wait that ran out to (0: none).  What
+    they gave is not complete then: an optimizer that reads the word (``status`` of ``optim_ops.adamw_multi``,
+    ``extra_status`` of ``ShardedAdamW``) leaves the weights alone until ``check_status`` has raised and cleared it."""
+    device = torch.device(device)
+    _need(device.type == "cuda", f"status words are those of CUDA devices, not of {device}")
+    return _status(device if device.index is not None else torch.device("cuda", torch.cuda.current_device()))
+
+
 def check_status() -> None:
     """Raise if a bounded wait inside a product ran out since the last call (synchronises)."""
     for index, word in _STATUS.items():

@@ -132,7 +132,8 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
     m, v: fp32 moments; with ``m_scales`` and ``v_scales`` (float8_e8m0fnu, one per 256 values) codes in float8_e4m3fn of m and
     of sqrt(v), rounded stochastically by a hash of ``seed``, step, tensor and element: right on average, and the same bits
     for the same inputs.  ``step``: one int64 on the device, counted up by the call, so a captured step can be replayed; all
-    other numbers are the call's.  A gradient that is not finite makes its own element NaN, and with ``clip`` all."""
+    other numbers are the call's.  ``status``: up to four int32 words, such as ``fp8_ops.status_word``: when one is not zero as
+    the step runs, all stays as it is.  A gradient that is not finite makes its own element NaN, and with ``clip`` all."""
     def call():
         return _native().adamw8(params, grads, masters, m, v, step, lr, beta1, beta2, eps, weight_decay, grad_scale, clip or 0.0, m_scales,
                                    v_scales, seed & 0xFFFFFFFF, factor, status)
@@ -146,7 +147,8 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
         _need(clip is None or factor is None, "either clip, or a factor from elsewhere")
         _need(factor is None or (factor.dtype == torch.float32 and factor.numel() == 1 and factor.device == step.device),
               "factor has to be one float32 on the parameters' device")
-        _need(len(status) <= 2 and all(s.dtype == torch.int32 and s.device == step.device for s in status), "status: up to two int32 words")
+        _need(len(status) <= 4 and all(s.dtype == torch.int32 and s.numel() > 0 and s.device == step.device for s in status),
+              "status: up to four int32 words on the parameters' device")
         _need(not step.is_cuda, "the native call does not take these tensors")
         if any(int(s.reshape(-1)[0]) for s in status):
             return None if clip is None else torch.zeros(1)
@@ -162,14 +164,16 @@ class MultiTensorAdamW:
 
     ``step()`` takes the parameters' ``.grad`` (all of them set, contiguous, of one type).  State of the whole list lies in
     flat tensors: ``master``, ``m``, ``v`` (in 8 bits: codes of m and of sqrt(v), with ``m_scale`` and ``v_scale``); each
-    parameter's part begins at a multiple of 256 values."""
+    parameter's part begins at a multiple of 256 values.  ``status``: words that keep a step from changing anything while one
+    is not zero; gradients that come of 8-bit products need ``fp8_ops.status_word`` among them."""
 
     def __init__(self, params: Sequence[torch.Tensor], lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8, weight_decay: float = 0.1,
-                 clip_grad: Optional[float] = None, state_bits: int = 32, seed: int = 0):
+                 clip_grad: Optional[float] = None, state_bits: int = 32, seed: int = 0, status: Sequence[torch.Tensor] = ()):
         self.params: List[torch.Tensor] = list(params)
         _need(len(self.params) > 0, "no parameters")
         _need(state_bits in (8, 32), "moments are kept in 8 or 32 bits")
         self.lr, self.betas, self.eps, self.wd, self.clip, self.bits, self.seed = lr, betas, eps, weight_decay, clip_grad, state_bits, seed
+        self.status = list(status)
         p0 = self.params[0]
         starts, at = [], 0
         for p in self.params:
@@ -196,7 +200,7 @@ class MultiTensorAdamW:
         _need(all(g is not None for g in grads), "a parameter has no gradient")
         return adamw_multi([p.detach() for p in self.params], grads, self._masters, self._m, self._v, self.step_count, lr=self.lr,
                            beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, weight_decay=self.wd, grad_scale=grad_scale,
-                           clip=self.clip, m_scales=self._m_scales, v_scales=self._v_scales, seed=self.seed)
+                           clip=self.clip, m_scales=self._m_scales, v_scales=self._v_scales, seed=self.seed, status=self.status)
 
     def state_dict(self) -> dict:
         keep = ("master", "m", "v", "m_scale", "v_scale", "step_count")

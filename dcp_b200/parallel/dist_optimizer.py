@@ -28,7 +28,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -115,15 +115,16 @@ class ShardedAdamW:
     def __init__(self, bufs: FlatBuffers, lr: float = 3e-4, betas=(0.9, 0.95), eps: float = 1e-8,
                  weight_decay: float = 0.1, clip_grad: Optional[float] = 1.0, group=None, tp_group=None,
                  n_replicated: int = 0, buckets: Optional[Sequence[Tuple[int, int]]] = None,
-                 extra_status: Optional[torch.Tensor] = None, overlap_ctas: int = 24, state_bits: int = 32, seed: int = 0):
+                 extra_status: Union[None, torch.Tensor, Sequence[torch.Tensor]] = None, overlap_ctas: int = 24, state_bits: int = 32, seed: int = 0):
         """``group`` = the ranks that hold the same parameters (they share the sharded state and
         their gradients are summed).  With tensor parallelism ``tp_group`` links the ranks that hold
         different shards of one model replica and ``n_replicated`` is the length of the leading
         part of the flat buffers that every one of them holds in full: the clipping norm counts
         that part once and the sharded part once per tensor-parallel rank (a bucket lies entirely
         in one of the two parts).  ``buckets``: (offset, length) ranges covering the flat buffer
-        (default: one bucket).  ``extra_status``: status word of another arena (the attention
-        executor's) that, when nonzero, also makes the update kernels leave the weights alone.
+        (default: one bucket).  ``extra_status``: up to three status words of what else the
+        gradients come from (the attention executor's arena, the 8-bit products) that, when nonzero, also make the
+        update kernels leave the weights alone.
         ``state_bits``: 8 keeps m and sqrt(v) as 8-bit codes with a scale per 256 values (2 instead of 8 bytes per
         parameter), rounded stochastically by a hash of ``seed``, step, slice and element (``ops.optim_ops``)."""
         if state_bits not in (8, 32):
@@ -167,6 +168,10 @@ class ShardedAdamW:
         self.clip_coef = torch.ones(1, dtype=torch.float32, device=dev)
         self.grad_scale = 1.0
         self.extra_status = extra_status
+        extra = [] if extra_status is None else [extra_status] if torch.is_tensor(extra_status) else list(extra_status)
+        if len(extra) > 3 or any(t.dtype != torch.int32 or t.numel() < 1 or t.device != dev for t in extra):
+            raise ValueError("extra_status is up to three int32 words on the parameters' device")
+        self._status_words = [bufs.arena.status, *extra]
         self.step_count = 0
         self.kernel_launches = 0
 
@@ -220,13 +225,12 @@ class ShardedAdamW:
             cut(self.v, "state_off"), self.step_tensor, lr=self.lr, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps,
             weight_decay=self.wd, grad_scale=grad_scale, m_scales=[self._scales(self.m_scale, i) for i, _ in parts],
             v_scales=[self._scales(self.v_scale, i) for i, _ in parts], seed=self.seed, factor=self.clip_coef if clipped else None,
-            status=[t for t in (self.bufs.arena.status, self.extra_status) if t is not None])
+            status=self._status_words)
         self.kernel_launches += 2
 
     def _status_ptrs(self):
-        a = _lib.ptr(self.bufs.arena.status)
-        b = _lib.ptr(self.extra_status) if self.extra_status is not None else ctypes.c_void_p(0)
-        return a, b
+        """The kernels' arguments for the status words: their addresses and how many."""
+        return _ptr_array([t.data_ptr() for t in self._status_words]), ctypes.c_int(len(self._status_words))
 
     def _sq_slot(self, shard: BucketShard) -> torch.Tensor:
         """Where a bucket's squared norm is accumulated: replicated / sharded part with tensor
@@ -250,13 +254,13 @@ class ShardedAdamW:
             self._side_used = True
         self.side.wait_stream(main)
         s = self.shards[b]
-        st_a, st_b = self._status_ptrs()
+        status = self._status_ptrs()
         with torch.cuda.stream(self.side):
             a.barrier()                       # every rank's gradients of this bucket are written
             _lib.check(lib.dcpk_grad_reduce_scatter(
                 _ptr_array(a.peer_ptrs("grads")), ctypes.c_int(self.bufs.world), ctypes.c_long(s.flat_off),
                 ctypes.c_long(s.length), ctypes.c_float(self.grad_scale), _lib.ptr(self.main_grad[s.state_off:]),
-                _lib.ptr(self._sq_slot(s)), ctypes.c_int(self.overlap_ctas), st_a, st_b, _lib.stream_handle()),
+                _lib.ptr(self._sq_slot(s)), ctypes.c_int(self.overlap_ctas), *status, _lib.stream_handle()),
                 "grad_reduce_scatter")
         self._reduced[b] = True
         self.kernel_launches += 2
@@ -267,9 +271,9 @@ class ShardedAdamW:
         a = b.arena
         self.step_count += 1
         self.grad_scale = grad_scale
-        st_a, st_b = self._status_ptrs()
+        status = self._status_ptrs()
         if self.overlap:
-            self._step_overlapped(lib, st_a, st_b)
+            self._step_overlapped(lib, status)
             return
         # ---- one rank: (norm pass when clipping) + one fused reduce/AdamW/store kernel per bucket
         grads, params = _ptr_array(a.peer_ptrs("grads")), _ptr_array(a.peer_ptrs("params"))
@@ -296,7 +300,7 @@ class ShardedAdamW:
                 ctypes.c_float(grad_scale), _lib.ptr(self.master[s.state_off:]), _lib.ptr(self.m[s.state_off:]),
                 _lib.ptr(self.v[s.state_off:]), ctypes.c_float(self.lr), ctypes.c_float(self.betas[0]),
                 ctypes.c_float(self.betas[1]), ctypes.c_float(self.eps), ctypes.c_float(self.wd),
-                ctypes.c_int(self.step_count), clip_ptr, st_a, st_b, _lib.stream_handle()), "fused_rs_adamw_ag")
+                ctypes.c_int(self.step_count), clip_ptr, *status, _lib.stream_handle()), "fused_rs_adamw_ag")
         self.kernel_launches += 2 * len(self.shards)
 
     def _finish_norm(self, from_sum: bool = False) -> None:
@@ -314,7 +318,7 @@ class ShardedAdamW:
                                               ctypes.c_float(self.clip), _lib.ptr(self.clip_coef), _lib.stream_handle()),
                    "clip_coef")
 
-    def _step_overlapped(self, lib, st_a, st_b) -> None:
+    def _step_overlapped(self, lib, status) -> None:
         b, a = self.bufs, self.bufs.arena
         main = torch.cuda.current_stream(b.params.device)
         saved = self.overlap_ctas
@@ -340,7 +344,7 @@ class ShardedAdamW:
                 _lib.ptr(self.main_grad[s.state_off:]), params, ctypes.c_int(b.world), ctypes.c_long(s.flat_off),
                 ctypes.c_long(s.length), ctypes.c_float(self.lr), ctypes.c_float(self.betas[0]),
                 ctypes.c_float(self.betas[1]), ctypes.c_float(self.eps), ctypes.c_float(self.wd),
-                ctypes.c_int(self.step_count), clip_ptr, st_a, st_b, _lib.stream_handle()), "adamw_all_gather")
+                ctypes.c_int(self.step_count), clip_ptr, *status, _lib.stream_handle()), "adamw_all_gather")
         self.kernel_launches += len(self.shards)
         a.barrier()   # every rank's parameter buffer holds all updated slices
         self._reduced = [False] * len(self.buckets)

@@ -131,7 +131,8 @@ class TrainEngine:
         self.optimizer = ShardedAdamW(self.bufs, cfg.lr, weight_decay=cfg.weight_decay, clip_grad=cfg.clip_grad,
                                       group=self.opt_group if n_cp > 1 else None, tp_group=self.tp_group,
                                       n_replicated=self.model.n_replicated, buckets=self.model.grad_buckets(),
-                                      extra_status=self.executor.arena.status, state_bits=cfg.optimizer_state_bits, seed=cfg.seed)
+                                      extra_status=[self.executor.arena.status] + ([fp8_ops.status_word(device)] if cfg.fp8 else []),
+                                      state_bits=cfg.optimizer_state_bits, seed=cfg.seed)
         if self.optimizer.overlap and cfg.overlap_grad_reduce:
             self.model.grad_ready_hook = self.optimizer.reduce_bucket
         self.activation_levels = self._plan_activations(group_tokens // dcp)
@@ -278,7 +279,7 @@ class TrainEngine:
         return value
 
     def check_status(self) -> None:
-        """Raise if a device-side wait of this step ran out (attention arenas or optimizer arena).
+        """Raise if a device-side wait of this step ran out (attention arenas, optimizer arena or 8-bit products).
         The update kernels read the same status words and leave the weights alone when one is set."""
         self.executor.check_status()
         self.optimizer.check_status()

@@ -327,3 +327,19 @@ def _too_wide(device="cpu"):
 
 def test_more_columns_than_the_kernels_count_are_refused():
     _too_wide()
+
+
+def test_status_words_are_those_of_devices():
+    with pytest.raises(ValueError, match="CUDA devices"):
+        F.status_word(torch.device("cpu"))
+    word = torch.ones(1, dtype=torch.int32)
+    p = torch.ones(300)
+    p.grad = torch.ones(300)
+    opt = O.MultiTensorAdamW([p], lr=0.1, status=[torch.zeros(1, dtype=torch.int32), word])
+    opt.step()
+    assert (p == 1).all() and int(opt.step_count) == 0
+    word.zero_()
+    opt.step()
+    assert (p != 1).all()
+    with pytest.raises(ValueError, match="up to four"):
+        O.MultiTensorAdamW([p], status=[word] * 5).step()

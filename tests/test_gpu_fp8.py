@@ -852,3 +852,77 @@ def test_adamw_of_second_moments_at_the_ends_of_fp32(dev, gtype, offset, size, e
             assert all(torch.isfinite(w).all() for w in st["masters"])
             assert size < 1e20 or any(torch.isnan(v.float()).any() for v in st["v"])
         ref = _copy(st)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_product_that_gave_up_stops_the_optimizer(dev, bits):
+    """The word is set from the host; whatever the gradients are then, the step changes nothing and the check raises."""
+    eng = _engine(dev, fp8=True, optimizer_state_bits=bits)
+    try:
+        eng.train_step()
+        opt = eng.optimizer
+        state = [eng.bufs.params, opt.master, opt.m, opt.v] + ([opt.m_scale, opt.v_scale, opt.step_tensor] if bits == 8 else [])
+        before = [t.clone() for t in state]
+        F.status_word(dev).fill_(1)
+        inputs = eng.stage_inputs(eng.plans.get(1))
+        eng.run_step(*inputs, 1000)
+        assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(state, before))
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            eng.check_status()
+        eng.check_status()
+        eng.run_step(*inputs, 1000)     # the word is cleared
+        assert not torch.equal(eng.bufs.params, before[0])
+    finally:
+        eng.close()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+def test_every_status_word_stops_the_kernels_of_several_ranks(dev, which):
+    """The kernels that several ranks take, as a world of one."""
+    import ctypes
+    from dcp_b200.ops import _lib
+    from dcp_b200.ops.attention import _ptr_array
+    lib, n = _lib.load(), 4096
+    grads, params = torch.ones(n, device=dev).bfloat16(), torch.ones(n, device=dev).bfloat16()
+    master, m, v, main, sq = (torch.ones(k, device=dev) for k in (n, n, n, n, 1))
+    words = [torch.zeros(1, dtype=torch.int32, device=dev) for _ in range(4)]
+    pointers = _ptr_array([w.data_ptr() for w in words])
+
+    def run():
+        f, p = ctypes.c_float, _lib.ptr
+        _lib.check(lib.dcpk_grad_reduce_scatter(_ptr_array([grads.data_ptr()]), ctypes.c_int(1), ctypes.c_long(0), ctypes.c_long(n), f(2.0), p(main),
+                                                p(sq), ctypes.c_int(0), pointers, ctypes.c_int(4), _lib.stream_handle()), "grad_reduce_scatter")
+        _lib.check(lib.dcpk_adamw_all_gather(p(master), p(m), p(v), p(main), _ptr_array([params.data_ptr()]), ctypes.c_int(1), ctypes.c_long(0),
+                                             ctypes.c_long(n), f(0.1), f(0.9), f(0.95), f(1e-8), f(0.1), ctypes.c_int(1), ctypes.c_void_p(0), pointers,
+                                             ctypes.c_int(4), _lib.stream_handle()), "adamw_all_gather")
+        _lib.check(lib.dcpk_fused_rs_adamw_ag(_ptr_array([grads.data_ptr()]), _ptr_array([params.data_ptr()]), ctypes.c_int(1), ctypes.c_long(0),
+                                              ctypes.c_long(n), f(1.0), p(master), p(m), p(v), f(0.1), f(0.9), f(0.95), f(1e-8), f(0.1), ctypes.c_int(1),
+                                              ctypes.c_void_p(0), pointers, ctypes.c_int(4), _lib.stream_handle()), "fused_rs_adamw_ag")
+
+    words[which].fill_(1)
+    run()
+    assert all((t == 1).all() for t in (params, master, m, v, main, sq))
+    words[which].zero_()
+    run()
+    assert not any((t == 1).any() for t in (params, master, main, sq))
+    assert lib.dcpk_grad_reduce_scatter(_ptr_array([grads.data_ptr()]), ctypes.c_int(1), ctypes.c_long(0), ctypes.c_long(n), ctypes.c_float(1.0),
+                                        _lib.ptr(main), _lib.ptr(sq), ctypes.c_int(0), pointers, ctypes.c_int(5), _lib.stream_handle()) == -3
+
+
+def test_status_words_of_the_optimizers(dev):
+    from dcp_b200.parallel.dist_optimizer import FlatBuffers, ShardedAdamW
+    bufs = FlatBuffers(64, dev)
+    word = torch.zeros(1, dtype=torch.int32, device=dev)
+    for bad in ([word] * 4, torch.zeros(1, device=dev), word.cpu(), [word[:0]]):
+        with pytest.raises(ValueError, match="status"):
+            ShardedAdamW(bufs, extra_status=bad)
+    ShardedAdamW(bufs, extra_status=word), ShardedAdamW(bufs, extra_status=(word, word, word)), ShardedAdamW(bufs)
+    p = torch.ones(300, device=dev).bfloat16()
+    p.grad = torch.ones_like(p)
+    opt = O.MultiTensorAdamW([p], lr=0.1, state_bits=8, status=[F.status_word(dev), word])
+    word.fill_(3)
+    opt.step()
+    assert (p == 1).all() and int(opt.step_count) == 0
+    word.zero_()
+    opt.step()
+    assert (p != 1).all() and int(opt.step_count) == 1
