@@ -53,6 +53,10 @@ struct WithoutGil {
   ~WithoutGil() { PyEval_RestoreThread(state); }
 };
 
+// What is written behind autograd's back: a graph that saved the tensor has to find that it changed.  (Raises for an inference
+// tensor outside inference mode, so before anything is launched.)
+void changes(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
 // A matrix of its own memory, straight from the allocator (a call through the dispatcher takes 0.8 us, and as much again for a
 // view of the result)
 Tensor empty_matrix(long rows, long cols, long pitch, at::ScalarType type, const Tensor& like, bool by_cols = false) {
@@ -177,6 +181,7 @@ std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair
       return std::nullopt;
   if (add && out && !one_or_apart(*add, *out)) return std::nullopt;
   c10::DeviceGuard guard(a.device());
+  if (out) changes(*out);
   Tensor result = out ? *out : empty_matrix(q.rows, p.rows, p.rows, type, a);
   Tensor laid[2];   // operands whose rows do not begin on 16 bytes
   const Tensor* codes[2] = {&a, &b};
@@ -258,6 +263,12 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i)
     if (written[i - 1].second > written[i].first) return no;
+  for (const List* list : {&params, &m, &v})
+    for (const Tensor& t : *list) changes(t);
+  for (const auto* list : {&masters, &m_scales, &v_scales})
+    if (*list)
+      for (const Tensor& t : **list) changes(t);
+  changes(step);
   c10::DeviceGuard guard(device);
   Tensor work = empty_vector(dcpk_adamw_multi_work(int(n)), at::kDouble, step);
   std::optional<Tensor> norm;

@@ -343,3 +343,36 @@ def test_status_words_are_those_of_devices():
     assert (p != 1).all()
     with pytest.raises(ValueError, match="up to four"):
         O.MultiTensorAdamW([p], status=[word] * 5).step()
+
+
+def _check_versions(device):
+    """Autograd sees what the operators write: a graph that saved it raises instead of giving other gradients."""
+    for bits, ptype in ((8, torch.bfloat16), (32, torch.float32)):
+        p = [torch.randn(300, device=device).to(ptype).requires_grad_(), torch.randn(7, 3, device=device).to(ptype).requires_grad_()]
+        opt = O.MultiTensorAdamW(p, state_bits=bits)
+        graphs = [t.square().sum() for t in p]
+        for t in p:
+            t.grad = torch.randn_like(t).detach()
+        opt.step()
+        for g in graphs:
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                g.backward()
+        p[0].square().sum().backward()
+        kept = [opt.m, opt.v, opt.step_count] + [t for t in (opt.master, opt.m_scale, opt.v_scale) if t is not None]
+        before, grads = [t._version for t in kept], [t.grad._version for t in p]
+        opt.step()
+        assert all(t._version > v for t, v in zip(kept, before)) and [t.grad._version for t in p] == grads
+    a, b = F.quantize(torch.randn(5, 130, device=device)), F.quantize(torch.randn(7, 130, device=device), (128, 128))
+    out, scale = torch.zeros(6, 7, device=device), torch.ones(6, 7, device=device, requires_grad=True)
+    graph = (out * scale).sum()
+    F.matmul(a, b, out=out[:5])
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        graph.backward()
+    add = torch.zeros(5, 7, device=device)
+    versions = [t._version for t in (add, a.codes, b.codes)]
+    F.matmul(a, b, add=add, out=out[:5])
+    assert [t._version for t in (add, a.codes, b.codes)] == versions
+
+
+def test_autograd_sees_what_is_written():
+    _check_versions("cpu")

@@ -926,3 +926,14 @@ def test_status_words_of_the_optimizers(dev):
     word.zero_()
     opt.step()
     assert (p != 1).all() and int(opt.step_count) == 1
+
+
+def test_autograd_sees_what_is_written_on_the_gpu(dev):
+    from test_fp8_ops import _check_versions
+    _check_versions(dev)
+    with torch.inference_mode():
+        frozen = torch.zeros(5, 7, device=dev)
+        a, b = F.quantize(torch.ones(5, 130, device=dev)), F.quantize(torch.ones(7, 130, device=dev), (128, 128))
+        assert (F.matmul(a, b, out=frozen) == 130).all()
+    with pytest.raises(RuntimeError, match="inference"):
+        F.matmul(a, b, out=frozen)
