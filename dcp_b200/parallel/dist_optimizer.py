@@ -184,14 +184,23 @@ class ShardedAdamW:
             m, v = self.m, self.v
         else:
             m, v = (torch.empty(self.master.numel(), dtype=torch.float32) for _ in range(2))
-            for s, part in self._state_parts():
-                m[part] = optim_ops.decode_state(self.m[part], self._scales(self.m_scale, s)).cpu()
-                v[part] = optim_ops.decode_state(self.v[part], self._scales(self.v_scale, s)).square_().cpu()
+            for part, scales in self._state_pieces():
+                m[part] = optim_ops.decode_state(self.m[part], self.m_scale[scales]).cpu()
+                v[part] = optim_ops.decode_state(self.v[part], self.v_scale[scales]).square_().cpu()
         return {"master": self.master, "m": m, "v": v, "step": self.step_count,
                 "buckets": list(self.buckets), "world": self.bufs.world, "rank": self.bufs.rank}
 
     def _state_parts(self):
         return [(i, slice(s.state_off, s.state_off + s.length)) for i, s in enumerate(self.shards) if s.length > 0]
+
+    def _state_pieces(self, most: int = 1 << 24):
+        """The slices of values and of scales of 8-bit state in pieces of whole blocks of up to ``most`` values: what is made in
+        32 bits of one stays small."""
+        block = optim_ops.STATE_BLOCK
+        for i, part in self._state_parts():
+            for lo in range(part.start, part.stop, most):
+                hi, at = min(lo + most, part.stop), self.scale_offs[i] + (lo - part.start) // block
+                yield slice(lo, hi), slice(at, at + optim_ops.state_scales(hi - lo))
 
     def _scales(self, t: torch.Tensor, shard: int) -> torch.Tensor:
         return t[self.scale_offs[shard]:self.scale_offs[shard + 1]]
@@ -205,12 +214,12 @@ class ShardedAdamW:
             self.m.copy_(sd["m"]); self.v.copy_(sd["v"])
             return
         self.step_tensor.fill_(self.step_count)
-        for i, part in self._state_parts():
+        for part, where in self._state_pieces():
             for codes, scales, value, root in ((self.m, self.m_scale, sd["m"], False), (self.v, self.v_scale, sd["v"], True)):
                 value = value[part].to(self.master.device, torch.float32)
                 c, sc = optim_ops.encode_state(value.sqrt() if root else value, root=root)
                 codes[part].copy_(c)
-                self._scales(scales, i).view(torch.uint8).copy_(sc.view(torch.uint8))
+                scales[where].view(torch.uint8).copy_(sc.view(torch.uint8))
 
     def _update_8bit(self, grads: torch.Tensor, at: str, grad_scale: float, clipped: bool) -> None:
         """AdamW on this rank's slices, all in one launch: gradients from ``grads`` (the flat buffer or the reduced slices),

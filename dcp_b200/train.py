@@ -325,8 +325,9 @@ class TrainEngine:
         assert meta.get("tp_size", 1) == self.tp_size, "resume needs the tensor-parallel size the checkpoint was written with"
         old_world = int(meta["world"])
         if old_world == self.world:
-            state = torch.load(os.path.join(directory, f"rank{self.rank:03d}.pt"), map_location=self.device,
-                               weights_only=False)
+            # on the host, whatever it was saved from: the optimizer takes it slice by slice, and all of it beside the state that
+            # it replaces does not fit a GPU that the state alone fills by half
+            state = torch.load(os.path.join(directory, f"rank{self.rank:03d}.pt"), map_location="cpu", weights_only=False, mmap=True)
             self.optimizer.load_state_dict(state["optimizer"])
             torch.set_rng_state(state["rng"].cpu())
             torch.cuda.set_rng_state(state["cuda_rng"].cpu(), self.device)

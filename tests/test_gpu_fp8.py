@@ -937,3 +937,52 @@ def test_autograd_sees_what_is_written_on_the_gpu(dev):
         assert (F.matmul(a, b, out=frozen) == 130).all()
     with pytest.raises(RuntimeError, match="inference"):
         F.matmul(a, b, out=frozen)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_resuming_takes_no_room_for_the_file_on_the_gpu(dev, bits, tmp_path, monkeypatch):
+    """What a checkpoint holds comes from the host slice by slice."""
+    eng, other = (_engine(dev, optimizer_state_bits=bits) for _ in range(2))
+    try:
+        eng.train_step()
+        eng.save_checkpoint(str(tmp_path))
+        load, found = torch.load, []
+
+        def tensors(x):
+            return [x] if torch.is_tensor(x) else [t for y in (x.values() if isinstance(x, dict) else x if isinstance(x, (list, tuple)) else ()) for t in tensors(y)]
+
+        monkeypatch.setattr(torch, "load", lambda *a, **kw: found.append(load(*a, **kw)) or found[-1])
+        torch.cuda.synchronize(), torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        if bits == 8:
+            pieces = other.optimizer._state_pieces
+            monkeypatch.setattr(other.optimizer, "_state_pieces", lambda: pieces(1 << 16))
+        other.load_checkpoint(str(tmp_path))
+        assert len(tensors(found)) > 4 and all(t.device.type == "cpu" for t in tensors(found))
+        # pieces of 2^16 values with a few temporaries of up to 8 bytes each; in 32 bits none
+        assert torch.cuda.max_memory_allocated() - held <= (1 << 16) * 8 * 16 + (1 << 20)
+        assert torch.equal(other.bufs.params, eng.bufs.params) and torch.equal(other.optimizer.master, eng.optimizer.master)
+        # value for value, not bit for bit: a block's largest code may be 224 after rounding down, 448 with half its scale
+        monkeypatch.undo()
+        a, b = eng.optimizer.state_dict(), other.optimizer.state_dict()
+        assert torch.equal(a["m"].cpu(), b["m"].cpu()) and torch.equal(a["v"].cpu(), b["v"].cpu())
+        assert abs(eng.train_step() - other.train_step()) < 1e-4
+    finally:
+        eng.close()
+        other.close()
+
+
+@pytest.mark.parametrize("most", [256, 1024, 1 << 24])
+def test_8_bit_state_in_pieces_is_the_whole(dev, most):
+    (_, opt), (_, other) = _sharded(dev, 8), _sharded(dev, 8)
+    for i in range(2):
+        _grads(opt.bufs, i)
+        opt.step()
+    whole = opt.state_dict()
+    pieces = opt._state_pieces
+    opt._state_pieces = lambda: pieces(most)
+    assert all(torch.equal(opt.state_dict()[k], whole[k]) for k in ("m", "v"))
+    pieces2 = other._state_pieces
+    other._state_pieces = lambda: pieces2(most)
+    other.load_state_dict(whole)
+    assert all(torch.equal(other.state_dict()[k], whole[k]) for k in ("m", "v"))
