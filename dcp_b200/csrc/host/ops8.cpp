@@ -249,7 +249,7 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
   }
   // memory given twice would be written by two blocks at once
   std::vector<std::pair<uintptr_t, uintptr_t>> written;
-  written.reserve(6 * n);
+  written.reserve(6 * n + 1);
   const auto writes = [&](const std::vector<void*>& list, size_t i, long bytes) {
     const uintptr_t start = reinterpret_cast<uintptr_t>(list[i]);
     if (start && bytes > 0) written.emplace_back(start, start + uintptr_t(bytes));
@@ -260,9 +260,22 @@ std::tuple<bool, std::optional<Tensor>> adamw8(const List& params, const List& g
     writes(pm, i, sizes[i] * of_state), writes(pv, i, sizes[i] * of_state);
     writes(sm, i, blocks(sizes[i], kStateBlock)), writes(sv, i, blocks(sizes[i], kStateBlock));
   }
+  written.emplace_back(reinterpret_cast<uintptr_t>(step.const_data_ptr()), reinterpret_cast<uintptr_t>(step.const_data_ptr()) + 8);
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i)
     if (written[i - 1].second > written[i].first) return no;
+  // and what is read would change under the readers
+  const auto apart = [&](const void* from, long bytes) {
+    const uintptr_t start = reinterpret_cast<uintptr_t>(from);
+    const auto next = std::lower_bound(written.begin(), written.end(), std::make_pair(start, uintptr_t(0)));
+    return bytes <= 0 || ((next == written.end() || next->first >= start + uintptr_t(bytes)) && (next == written.begin() || next[-1].second <= start));
+  };
+  const long of_grad = long(grads[0].element_size());
+  for (size_t i = 0; i < n; ++i)
+    if (!apart(g[i], sizes[i] * of_grad)) return no;
+  if (factor && !apart(factor->const_data_ptr(), 4)) return no;
+  for (const Tensor& s : status)
+    if (!apart(s.const_data_ptr(), 4)) return no;
   for (const List* list : {&params, &m, &v})
     for (const Tensor& t : *list) changes(t);
   for (const auto* list : {&masters, &m_scales, &v_scales})

@@ -5,6 +5,7 @@
 """
 from __future__ import annotations
 
+import bisect
 from typing import List, Optional, Sequence
 
 import torch
@@ -92,9 +93,15 @@ def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta
     return norm
 
 
-def _check_written(*lists) -> None:
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for ts in lists for t in ts or () if t.numel() > 0)
+def _check_written(written, read) -> None:
+    """What is written shares memory with nothing else that is written or read."""
+    span = lambda t: (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())  # noqa: E731
+    spans = sorted(span(t) for ts in written for t in ts or () if t.numel() > 0)
     _need(all(end <= start for (_, end), (start, _) in zip(spans, spans[1:])), "memory that the step writes is given twice")
+    starts = [start for start, _ in spans]
+    for lo, hi in (span(t) for t in read if t.numel() > 0):
+        i = bisect.bisect_left(starts, lo)
+        _need((i == len(spans) or starts[i] >= hi) and (i == 0 or spans[i - 1][1] <= lo), "gradients, factor or status share memory with what the step writes")
 
 
 def _check_lists(params, grads, masters, m, v, step, m_scales, v_scales):
@@ -126,7 +133,7 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
                 m_scales: Optional[Sequence[torch.Tensor]] = None, v_scales: Optional[Sequence[torch.Tensor]] = None,
                 seed: int = 0, factor: Optional[torch.Tensor] = None, status: Sequence[torch.Tensor] = ()) -> Optional[torch.Tensor]:
     """One AdamW step over lists of contiguous tensors, in place; returns the norm of the scaled gradients (fp32, one element)
-    where ``clip`` limits it, else None.
+    where ``clip`` limits it, else None.  What it writes shares memory with nothing else that it is given.
 
     params: bf16, fp16 or fp32, all of one type; grads: of one type; masters: fp32 (None: fp32 parameters are their own).
     m, v: fp32 moments; with ``m_scales`` and ``v_scales`` (float8_e8m0fnu, one per 256 values) codes in float8_e4m3fn of m and
@@ -141,7 +148,6 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
     taken, norm = call() if step.is_cuda and (clip is None or clip > 0) else (False, None)
     if not taken:
         _check_lists(params, grads, masters, m, v, step, m_scales, v_scales)
-        _check_written(params, masters, m, v, m_scales, v_scales)
         _need(0 <= beta1 < 1 and 0 <= beta2 < 1, f"betas from 0 to below 1, not {beta1} and {beta2}")
         _need(clip is None or clip > 0, "clip has to be positive")
         _need(clip is None or factor is None, "either clip, or a factor from elsewhere")
@@ -149,6 +155,8 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
               "factor has to be one float32 on the parameters' device")
         _need(len(status) <= 4 and all(s.dtype == torch.int32 and s.numel() > 0 and s.device == step.device for s in status),
               "status: up to four int32 words on the parameters' device")
+        _check_written((params, masters, m, v, m_scales, v_scales, [step]),
+                       [*grads, *([] if factor is None else [factor]), *(s.reshape(-1)[:1] for s in status)])
         _need(not step.is_cuda, "the native call does not take these tensors")
         if any(int(s.reshape(-1)[0]) for s in status):
             return None if clip is None else torch.zeros(1)

@@ -376,3 +376,37 @@ def _check_versions(device):
 
 def test_autograd_sees_what_is_written():
     _check_versions("cpu")
+
+
+def _check_read_memory(device):
+    """Gradients, factor and status words that lie in what the step writes, wherever in it."""
+    for bits in (8, 32):
+        st = _state([300, 300], bits, torch.bfloat16, torch.bfloat16, device=device)
+        buf = torch.zeros(4000, dtype=torch.uint8, device=device)
+        f32 = buf.view(torch.float32)
+        word = lambda i: buf[4 * i:4 * i + 4].view(torch.int32)  # noqa: E731
+        masters = [f32[100:400], f32[500:800]]
+        bf16 = buf.view(torch.bfloat16)
+        # in 16-bit values the masters are [200, 800) and [1000, 1600)
+        for lo, ok in ((0, False), (250, False), (799, False), (800, False), (1599, False), (1600, True), (1700, True)):
+            given = {**st, **HYPER, "masters": masters, "grads": [st["grads"][0], bf16[lo:lo + 300]]}
+            if ok:
+                O.adamw_multi(**given)
+            else:
+                with pytest.raises(ValueError, match="share memory"):
+                    O.adamw_multi(**given)
+        for i, ok in ((99, True), (100, False), (399, False), (400, True), (799, False), (800, True)):
+            for extra in (dict(factor=f32[i:i + 1]), dict(status=[word(i)])):
+                given = {**st, **HYPER, "masters": masters, **extra}
+                if ok:
+                    O.adamw_multi(**given)
+                else:
+                    with pytest.raises(ValueError, match="share memory"):
+                        O.adamw_multi(**given)
+        moments = buf[:1200].view(torch.float32) if bits == 32 else buf[:300].view(E4M3)
+        with pytest.raises(ValueError, match="given twice"):
+            O.adamw_multi(**{**st, **HYPER, "m": [st["m"][0], moments], "step": buf[:8].view(torch.int64)})
+
+
+def test_adamw_refuses_to_read_what_it_writes():
+    _check_read_memory("cpu")

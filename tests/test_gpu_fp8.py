@@ -986,3 +986,8 @@ def test_8_bit_state_in_pieces_is_the_whole(dev, most):
     other._state_pieces = lambda: pieces2(most)
     other.load_state_dict(whole)
     assert all(torch.equal(other.state_dict()[k], whole[k]) for k in ("m", "v"))
+
+
+def test_adamw_refuses_to_read_what_it_writes_on_the_gpu(dev):
+    from test_fp8_ops import _check_read_memory
+    _check_read_memory(dev)
