@@ -56,6 +56,14 @@ def decode_state(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return (flat.float() * scales.float().repeat_interleave(STATE_BLOCK)[:flat.numel()]).view(codes.shape)
 
 
+def _norm64(grads, grad_scale, device) -> torch.Tensor:
+    total = torch.zeros(1, dtype=torch.float64, device=device)
+    for g in grads:
+        total += (g.double() * grad_scale).square().sum()
+    return total.sqrt()
+
+
+@torch.no_grad()
 def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta2, eps, weight_decay, grad_scale=1.0, clip=None,
                           m_scales=None, v_scales=None, seed=0):
     step += 1
@@ -63,10 +71,7 @@ def adamw_multi_reference(params, grads, masters, m, v, step, *, lr, beta1, beta
     bc1, root_bc2 = (1 / (1 - beta1 ** t)).float(), (1 / (1 - beta2 ** t)).sqrt().float()
     coef, norm = grad_scale, None
     if clip is not None:
-        total = torch.zeros(1, dtype=torch.float64, device=step.device)
-        for g in grads:
-            total += (g.double() * grad_scale).square().sum()
-        norm = total.sqrt()
+        norm = _norm64(grads, grad_scale, step.device)
         coef = grad_scale * (clip / (norm + 1e-6)).float().clamp(max=1.0)
         norm = norm.float()
     key = _mix32((seed + int(step) * 0x9E3779B1) & 0xFFFFFFFF)
@@ -159,7 +164,7 @@ def adamw_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m
                        [*grads, *([] if factor is None else [factor]), *(s.reshape(-1)[:1] for s in status)])
         _need(not step.is_cuda, "the native call does not take these tensors")
         if any(int(s.reshape(-1)[0]) for s in status):
-            return None if clip is None else torch.zeros(1)
+            return None if clip is None else _norm64(grads, grad_scale, step.device).float().detach()
         return adamw_multi_reference(params, grads, masters, m, v, step, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
                                      weight_decay=weight_decay, grad_scale=grad_scale if factor is None else grad_scale * float(factor),
                                      clip=clip, m_scales=m_scales, v_scales=v_scales, seed=seed)

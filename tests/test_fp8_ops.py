@@ -410,3 +410,25 @@ def _check_read_memory(device):
 
 def test_adamw_refuses_to_read_what_it_writes():
     _check_read_memory("cpu")
+
+
+def _check_leaves_and_norm(device):
+    """Parameters that are leaves of a graph are stepped whatever the grad mode; a step that a status word stops has its norm."""
+    for bits, ptype in ((8, torch.bfloat16), (32, torch.float32)):
+        st = _state([300, 7], bits, ptype, ptype, device=device)
+        plain = {k: [t.clone() for t in x] if isinstance(x, list) else x.clone() if torch.is_tensor(x) else x for k, x in st.items()}
+        for k in ("params", "grads"):
+            for t in st[k]:
+                t.requires_grad_()
+        want = sum(g.double().square().sum() for g in plain["grads"]).sqrt().item() * 0.5
+        stopped = O.adamw_multi(**st, **HYPER, grad_scale=0.5, clip=1.0, status=[torch.ones(1, dtype=torch.int32, device=device)])
+        assert torch.equal(st["params"][0], plain["params"][0]) and abs(stopped.item() / want - 1) < 1e-6
+        norm = O.adamw_multi(**st, **HYPER, grad_scale=0.5, clip=1.0)
+        O.adamw_multi(**plain, **HYPER, grad_scale=0.5, clip=1.0)
+        assert torch.equal(norm, stopped) and not norm.requires_grad
+        assert all(torch.equal(a, b) and a.requires_grad for a, b in zip(st["params"], plain["params"]))
+        assert st["masters"] is None or not any(w.requires_grad for w in st["masters"])
+
+
+def test_adamw_of_leaves_and_its_norm():
+    _check_leaves_and_norm("cpu")

@@ -991,3 +991,8 @@ def test_8_bit_state_in_pieces_is_the_whole(dev, most):
 def test_adamw_refuses_to_read_what_it_writes_on_the_gpu(dev):
     from test_fp8_ops import _check_read_memory
     _check_read_memory(dev)
+
+
+def test_adamw_of_leaves_and_its_norm_on_the_gpu(dev):
+    from test_fp8_ops import _check_leaves_and_norm
+    _check_leaves_and_norm(dev)
