@@ -5,6 +5,7 @@
 // whatever device they are; for anything else it returns nothing before it allocates or launches anything, and the caller
 // says what is wrong or brings the tensors into shape and asks again.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -177,7 +178,8 @@ std::optional<Tensor> matmul8(const Tensor& a, const Tensor& a_scales, std::pair
     return std::nullopt;
   const at::ScalarType type = out_type == 0 ? at::kFloat : out_type == 1 ? at::kHalf : at::kBFloat16;
   for (const auto* t : {&add, &out})
-    if (*t && (!rows_of(**t) || (*t)->size(0) != q.rows || (*t)->size(1) != p.rows || (*t)->scalar_type() != type || (*t)->device() != a.device()))
+    if (*t && (!rows_of(**t) || (*t)->size(0) != q.rows || (*t)->size(1) != p.rows || (*t)->scalar_type() != type || (*t)->device() != a.device() ||
+               ((*t)->requires_grad() && at::GradMode::is_enabled())))
       return std::nullopt;
   if (add && out && !one_or_apart(*add, *out)) return std::nullopt;
   c10::DeviceGuard guard(a.device());

@@ -12,8 +12,8 @@ A product's scales have to run along the contraction in blocks of 128, so
 * ``dx = dy w``     takes dy by rows and the same codes of w:               ``matmul(dy, w, trans_b=False)``
 * ``dw = dy^T x``   takes both by tokens (128 x 1):                         ``matmul(dy, x, trans_a=True, trans_b=False)``
 
-``linear`` and ``norm_linear`` are these three as autograd functions (of a first derivative; a second is refused).  On a
-CUDA tensor the kernels always run (a missing library raises); CPU tensors take the plain forms.  All calls run on the
+``linear`` and ``norm_linear`` are these three as autograd functions (of a first derivative; a second is refused); the pieces
+that they are made of pass no gradient on.  On a CUDA tensor the kernels always run (a missing library raises); CPU tensors take the plain forms.  All calls run on the
 current stream of their tensors' device, allocate their results there and may be captured into a CUDA graph once a call has
 been made on the device.  (As with torch's own functions, a backward pass is captured together with its forward pass, not
 while an eager graph of the same leaves lives.)
@@ -116,7 +116,7 @@ def check_status() -> None:
             raise RuntimeError(f"8-bit product on cuda:{index} gave up waiting (status {code}): its results are not complete")
 
 
-# --------------------------------------------------------------------------- plain forms (fp32)
+# --------------------------------------------------------------------------- plain forms (fp32; like the kernels without autograd)
 def _scale_bytes(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     mantissa, exponent = torch.frexp(amax)
     k = exponent - (9 if dtype == E4M3 else 16) + (mantissa > 0.875).to(exponent.dtype)   # largest code: 0.875 * 2^9 or 2^16
@@ -124,6 +124,7 @@ def _scale_bytes(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.where(torch.isfinite(amax), k, torch.full_like(k, 255)).to(torch.uint8)
 
 
+@torch.no_grad()
 def quantize_reference(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK), dtype: torch.dtype = E4M3) -> BlockScaled:
     rows, cols = x.shape
     br, bc = block
@@ -136,6 +137,7 @@ def quantize_reference(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK), dty
     return BlockScaled(codes.to(dtype), scales, (br, bc))
 
 
+@torch.no_grad()
 def rmsnorm_quant_reference(x, w, eps, residual=None, dtype=E4M3):
     h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
     hf = h.float()
@@ -143,6 +145,7 @@ def rmsnorm_quant_reference(x, w, eps, residual=None, dtype=E4M3):
     return quantize_reference(hf * rstd[:, None] * w.float(), (1, BLOCK), dtype), h, rstd
 
 
+@torch.no_grad()
 def rmsnorm_quant_bwd_reference(h, w, rstd, dy, add=None):
     xh, g = h.float() * rstd[:, None], dy.float() * w.float()
     dx = rstd[:, None] * (g - xh * (g * xh).mean(-1, keepdim=True))
@@ -151,6 +154,7 @@ def rmsnorm_quant_bwd_reference(h, w, rstd, dy, add=None):
     return dx.to(h.dtype), (dy.float() * xh).sum(0)
 
 
+@torch.no_grad()
 def matmul_reference(a, b, trans_a=False, trans_b=True, out_dtype=torch.bfloat16, add=None):
     x, y = a.dequantize(), b.dequantize()
     out = (x.t() if trans_a else x) @ (y.t() if trans_b else y)
@@ -261,7 +265,8 @@ def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
 def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bool = True, out_dtype: torch.dtype = torch.bfloat16,
            add: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, form: int = 0) -> torch.Tensor:
     """op(a) op(b) of the values the codes stand for, summed in fp32 and rounded once; ``add`` (of the output's type and shape,
-    rows contiguous) is added before the rounding; it may be ``out`` itself, and shares nothing with it otherwise.
+    rows contiguous) is added before the rounding; it may be ``out`` itself, and shares nothing with it otherwise.  No autograd: an
+    ``add`` or ``out`` that requires a gradient is refused where one would be recorded.
 
     a: [M, K], or [K, M] with ``trans_a``; b: [N, K], or [K, N] without ``trans_b`` -> [M, N] in bf16, fp16 or fp32.  Along K
     both need a scale per 128 values; along the other dimension one per value or per 128.  Codes whose rows begin on 16 bytes
@@ -294,6 +299,8 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
             if out is not None:
                 rows = _rows(add)   # a copy where its rows are not contiguous
                 _need(_same_place(rows, out) or _apart(rows, out), "add has to be out itself or lie apart from it")
+        _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (add, out))),
+              "products pass no gradient on: add and out may not require one (see linear and norm_linear)")
         if not a.codes.is_cuda:
             got = matmul_reference(a, b, trans_a, trans_b, out_dtype, add)
             return got if out is None else out.copy_(got)

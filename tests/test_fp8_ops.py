@@ -432,3 +432,24 @@ def _check_leaves_and_norm(device):
 
 def test_adamw_of_leaves_and_its_norm():
     _check_leaves_and_norm("cpu")
+
+
+def _check_pieces_pass_no_gradient(device):
+    """No result carries a graph, and a product that would drop a gradient is refused where one would be recorded."""
+    x, w = torch.randn(3, 130, device=device, requires_grad=True), torch.ones(130, device=device, requires_grad=True)
+    y, h, rstd = F.rmsnorm_quant(x, w, residual=x.detach())
+    dx, dw = F.rmsnorm_quant_bwd(h, w, rstd, x)
+    b = F.quantize(torch.randn(5, 130, device=device, requires_grad=True), (128, 128))
+    out = F.matmul(y, b, out_dtype=torch.float32)
+    assert not any(t.requires_grad for t in (y.codes, y.scales, h, rstd, dx, dw, b.codes, b.scales, out, *F.quantize(x)[:2]))
+    leaf = torch.zeros(3, 5, device=device, requires_grad=True)
+    for call in (lambda: F.matmul(y, b, out_dtype=torch.float32, add=leaf), lambda: F.matmul(y, b, out=leaf), lambda: F.matmul(y, b, out=leaf * 1),
+                 lambda: F.matmul(y, b, add=leaf, out=torch.zeros(3, 5, device=device))):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(F.matmul(y, b, out_dtype=torch.float32, add=leaf), out) and torch.equal(F.matmul(y, b, out=leaf), out)
+
+
+def test_pieces_pass_no_gradient():
+    _check_pieces_pass_no_gradient("cpu")

@@ -996,3 +996,8 @@ def test_adamw_refuses_to_read_what_it_writes_on_the_gpu(dev):
 def test_adamw_of_leaves_and_its_norm_on_the_gpu(dev):
     from test_fp8_ops import _check_leaves_and_norm
     _check_leaves_and_norm(dev)
+
+
+def test_pieces_pass_no_gradient_on_the_gpu(dev):
+    from test_fp8_ops import _check_pieces_pass_no_gradient
+    _check_pieces_pass_no_gradient(dev)
