@@ -20,6 +20,7 @@ while an eager graph of the same leaves lives.)
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -312,6 +313,11 @@ def matmul(a: BlockScaled, b: BlockScaled, *, trans_a: bool = False, trans_b: bo
 
 
 # --------------------------------------------------------------------------- autograd
+def _matrix(t: torch.Tensor) -> torch.Tensor:
+    """[..., N] as a matrix, without values too."""
+    return t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
+
 def _grad_products(dy: torch.Tensor, x: torch.Tensor, wq: BlockScaled, need_x: bool, need_w: bool):
     """(dx, dw) of y = x w^T in 8 bits, in the types of dy."""
     if need_x and need_w:
@@ -326,7 +332,7 @@ def _grad_products(dy: torch.Tensor, x: torch.Tensor, wq: BlockScaled, need_x: b
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _matrix(x)
         wq = quantize(weight, (BLOCK, BLOCK))
         ctx.save_for_backward(x2, wq.codes, wq.scales)
         return matmul(quantize(x2), wq, out_dtype=x.dtype).view(*x.shape[:-1], weight.shape[0])
@@ -335,7 +341,7 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x2, codes, scales = ctx.saved_tensors
-        dx, dw = _grad_products(dy.reshape(-1, dy.shape[-1]), x2, BlockScaled(codes, scales, (BLOCK, BLOCK)), *ctx.needs_input_grad)
+        dx, dw = _grad_products(_matrix(dy), x2, BlockScaled(codes, scales, (BLOCK, BLOCK)), *ctx.needs_input_grad)
         return None if dx is None else dx.view(*dy.shape[:-1], x2.shape[1]), dw
 
 
@@ -349,7 +355,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 class _NormLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, norm_weight, weight, eps, residual):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _matrix(x)
         y, h, rstd = rmsnorm_quant(x2, norm_weight, eps, None if residual is None else residual.reshape(x2.shape))
         wq = quantize(weight, (BLOCK, BLOCK))
         ctx.save_for_backward(h, norm_weight, rstd, wq.codes, wq.scales)
@@ -364,7 +370,7 @@ class _NormLinear(torch.autograd.Function):
         if dout is None:   # only h was used
             return dh, None, None, None, dh if ctx.with_residual else None
         h, norm_weight, rstd, codes, scales = ctx.saved_tensors
-        d2 = dout.reshape(-1, dout.shape[-1])
+        d2 = _matrix(dout)
         need_w = ctx.needs_input_grad[2]
         # the weight gradient needs the norm's result by tokens: made again, in h's type
         y = (h.float() * rstd[:, None] * norm_weight.float()).to(h.dtype) if need_w else None

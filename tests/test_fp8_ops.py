@@ -453,3 +453,25 @@ def _check_pieces_pass_no_gradient(device):
 
 def test_pieces_pass_no_gradient():
     _check_pieces_pass_no_gradient("cpu")
+
+
+def _check_linear_of_nothing(device):
+    """No tokens, no outputs, nothing to add up: empty results or zeros, and gradients of zero."""
+    for shape, n in (((0, 256), 8), ((3, 0, 256), 8), ((4, 256), 0), ((2, 3, 256), 0), ((4, 0), 8), ((0, 0), 8), ((256,), 8)):
+        x = torch.zeros(shape, device=device, requires_grad=True)
+        w = torch.zeros(n, shape[-1], device=device, requires_grad=True)
+        out = F.linear(x, w)
+        assert out.shape == (*shape[:-1], n) and not out.any()
+        out.sum().backward()
+        assert x.grad.shape == x.shape and w.grad.shape == w.shape and not x.grad.any() and not w.grad.any()
+        if shape[-1] == 0:
+            continue
+        leaves = [t.detach().clone().requires_grad_() for t in (x, torch.ones(shape[-1], device=device), w, x)]
+        out, h = F.norm_linear(leaves[0], leaves[1], leaves[2], 1e-5, leaves[3])
+        assert out.shape == (*shape[:-1], n) and h.shape == x.shape
+        (out.sum() + 2 * h.sum()).backward()
+        assert not leaves[1].grad.any() and not leaves[2].grad.any() and (leaves[0].grad == 2).all() and torch.equal(leaves[0].grad, leaves[3].grad)
+
+
+def test_linear_of_nothing():
+    _check_linear_of_nothing("cpu")

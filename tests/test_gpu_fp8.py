@@ -1001,3 +1001,8 @@ def test_adamw_of_leaves_and_its_norm_on_the_gpu(dev):
 def test_pieces_pass_no_gradient_on_the_gpu(dev):
     from test_fp8_ops import _check_pieces_pass_no_gradient
     _check_pieces_pass_no_gradient(dev)
+
+
+def test_linear_of_nothing_on_the_gpu(dev):
+    from test_fp8_ops import _check_linear_of_nothing
+    _check_linear_of_nothing(dev)
