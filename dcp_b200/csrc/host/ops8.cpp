@@ -41,9 +41,9 @@ long up(long n, long to) { return (n + to - 1) / to * to; }
 long blocks(long n, long size) { return (n + size - 1) / size; }
 
 bool dense(const Tensor& t) { return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !t.is_conj(); }
-// a matrix whose rows are contiguous, of any pitch that leaves them apart
+// a matrix whose rows are contiguous, of any pitch that leaves them apart; one without values may have any strides
 bool rows_of(const Tensor& t) {
-  return dense(t) && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  return dense(t) && t.dim() == 2 && (t.numel() == 0 || ((t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1))));
 }
 long pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 bool on_16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }

@@ -64,8 +64,8 @@ def _up(n: int, to: int) -> int:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A 2-D tensor whose rows are contiguous and apart, of any pitch."""
-    return t if (t.stride(1) == 1 or t.shape[1] <= 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+    """A 2-D tensor whose rows are contiguous and apart, of any pitch (and any strides without values)."""
+    return t if t.numel() == 0 or (t.stride(1) == 1 or t.shape[1] <= 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
 _NATIVE = None
