@@ -95,7 +95,9 @@ def _status(device: torch.device) -> torch.Tensor:
     if device.index not in _STATUS:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call one of the 8-bit operators on this device before capturing a graph with them")
-        _STATUS.setdefault(device.index, torch.zeros(1, dtype=torch.int32, device=device))
+        word = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()    # other streams read it
+        _STATUS.setdefault(device.index, word)
     return _STATUS[device.index]
 
 
@@ -109,11 +111,13 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 
 def check_status() -> None:
-    """Raise if a bounded wait inside a product ran out since the last call (synchronises)."""
-    for index, word in _STATUS.items():
+    """Raise if a bounded wait inside a product ran out since the last call (waits for all streams of the devices)."""
+    for index, word in list(_STATUS.items()):
+        torch.cuda.synchronize(index)
         code = int(word.item())
         if code:
             word.zero_()
+            torch.cuda.synchronize(index)
             raise RuntimeError(f"8-bit product on cuda:{index} gave up waiting (status {code}): its results are not complete")
 
 

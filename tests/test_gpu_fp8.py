@@ -1006,3 +1006,29 @@ def test_pieces_pass_no_gradient_on_the_gpu(dev):
 def test_linear_of_nothing_on_the_gpu(dev):
     from test_fp8_ops import _check_linear_of_nothing
     _check_linear_of_nothing(dev)
+
+
+def test_status_across_streams(dev, monkeypatch):
+    """A new word is zero for every stream, and the check waits for what runs on another one."""
+    monkeypatch.setattr(F, "_STATUS", {})
+    side, busy = torch.cuda.Stream(), torch.randn(8192, 8192, device=dev)
+    # memory that was not zero, whose next owner is the word
+    used = [torch.full((1,), 7, dtype=torch.int32, device=dev) for _ in range(64)]
+    torch.cuda.synchronize()
+    del used
+    for _ in range(20):
+        busy @ busy
+    word = F.status_word(dev)
+    with torch.cuda.stream(side):
+        seen = word.clone()
+    side.synchronize()
+    assert seen.item() == 0
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy @ busy
+        word.fill_(1)
+    with pytest.raises(RuntimeError, match="gave up"):
+        F.check_status()
+    with torch.cuda.stream(side):
+        assert word.clone().item() == 0
+    F.check_status()
