@@ -1032,3 +1032,190 @@ def test_status_across_streams(dev, monkeypatch):
     with torch.cuda.stream(side):
         assert word.clone().item() == 0
     F.check_status()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("at", [0, 300, 2047, 2500])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_a_bad_gradient_leaves_its_block_alone(dev, bad, at, offset):
+    """Codes and scales of all other elements, with the bad one's old moments at zero, so that it cannot be its block's largest."""
+    st = _adam_state([700, 2600], 8, torch.bfloat16, torch.bfloat16, dev, offset)
+    for k in ("m", "v"):
+        st[k][1].view(torch.uint8)[at] = 0
+    clean = _copy(st)
+    st["grads"][1][at], clean["grads"][1][at] = bad, 0.0
+    O.adamw_multi(**st, **HYPER), O.adamw_multi(**clean, **HYPER)
+    keep = torch.arange(2600, device=dev) != at
+    for k in ("m", "v", "masters", "params"):
+        assert torch.isnan(st[k][1][at].float()), k
+        assert torch.equal(_bits(st[k][0]), _bits(clean[k][0])) and torch.equal(st[k][1].float()[keep], clean[k][1].float()[keep]), k
+    for k in ("m_scales", "v_scales"):
+        assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(st[k], clean[k])), k
+
+
+def test_overlapped_step_with_8_bit_state(dev):
+    """The step of several ranks (slices reduced on a side stream, the update, the new parameters to every rank) as a world of one:
+    gradients times 0.5 are exact, so without a norm, whose sum has no fixed order there, it gives the bits of the other."""
+    (bufs, opt), (bufs2, opt2) = _sharded(dev, 8), _sharded(dev, 8)
+    for o in (opt, opt2):
+        o.clip = None
+    opt2.overlap, opt2.side = True, torch.cuda.Stream()
+    opt2.main_grad = torch.zeros(opt2.master.numel(), device=dev)
+    for i in range(3):
+        _grads(bufs, i), _grads(bufs2, i)
+        for b in (3, 2):
+            opt2.grad_scale = 0.5
+            opt2.reduce_bucket(b)
+        opt.step(0.5), opt2.step(0.5)
+        for k in ("m", "v", "m_scale", "v_scale", "master", "step_tensor"):
+            assert torch.equal(_bits(getattr(opt, k)), _bits(getattr(opt2, k))), k
+        assert torch.equal(bufs.params, bufs2.params)
+    opt2.clip = 0.5
+    _grads(bufs2, 7)
+    before = opt2.master.clone()
+    want = {"params": [bufs2.params[s.flat_off:s.flat_off + s.length].clone() for s in opt2.shards], "step": opt2.step_tensor.clone()}
+    parts = [slice(s.state_off, s.state_off + s.length) for s in opt2.shards]
+    want |= {"masters": [before[p].clone() for p in parts], "m": [opt2.m[p].clone() for p in parts], "v": [opt2.v[p].clone() for p in parts],
+             "m_scales": [opt2._scales(opt2.m_scale, i).clone() for i in range(4)], "v_scales": [opt2._scales(opt2.v_scale, i).clone() for i in range(4)]}
+    opt2.step(0.5)
+    O.adamw_multi(**want, grads=[bufs2.grads[s.flat_off:s.flat_off + s.length] for s in opt2.shards], lr=1e-2, beta1=0.9, beta2=0.95, eps=1e-8,
+                  weight_decay=0.1, grad_scale=0.5, clip=0.5)
+    step = (torch.cat(want["masters"]) - before).abs()
+    # the norm in fp32, its 40000 squares added in any order: 2^-24 times at most some 300 additions of one chain
+    assert ((opt2.master - torch.cat(want["masters"])).abs() <= step * 2.0 ** -14 + before.abs() * 2.0 ** -23).all()
+    assert torch.equal(bufs2.params.float(), opt2.master.bfloat16().float())
+
+
+# --------------------------------------------------------------------------- the layers, compared closely
+# Two runs in 8 bits that differ by d somewhere differ by sqrt(2^-3 d) after the next quantizer, so whole gradients of two forms
+# cannot be compared closely.  Instead every call is compared on the very operands it had, and how the layer is put together is
+# compared with quantizers that round nothing.
+@pytest.mark.parametrize("level", [None, 0, 1, 2])
+def test_every_call_of_the_layers_in_8_bits(dev, level, monkeypatch):
+    calls = {k: getattr(F, k) for k in ("quantize", "quantize_both", "matmul", "rmsnorm_quant", "rmsnorm_quant_bwd")}
+    count = dict.fromkeys(calls, 0)
+
+    def quantize(x, block=(1, 128), dtype=E4M3):
+        count["quantize"] += 1
+        got = calls["quantize"](x, block, dtype)
+        _same(got, F.quantize_reference(x, block, dtype))
+        return got
+
+    def quantize_both(x, dtype=E4M3):
+        count["quantize_both"] += 1
+        got = calls["quantize_both"](x, dtype)
+        for q, block in zip(got, ((1, 128), (128, 1))):
+            _same(q, F.quantize_reference(x, block, dtype))
+        return got
+
+    def matmul(a, b, *, trans_a=False, trans_b=True, out_dtype=torch.bfloat16, add=None, out=None):
+        count["matmul"] += 1
+        was = None if add is None else add.clone()
+        got = calls["matmul"](a, b, trans_a=trans_a, trans_b=trans_b, out_dtype=out_dtype, add=add, out=out)
+        _check_product(got, a, b, dict(trans_a=trans_a, trans_b=trans_b), was)
+        return got
+
+    def rmsnorm_quant(x, w, eps=1e-5, residual=None, dtype=E4M3):
+        count["rmsnorm_quant"] += 1
+        y, h, rstd = calls["rmsnorm_quant"](x, w, eps, residual, dtype)
+        _check_norm(x, w, eps, residual, y, h, rstd, dtype)
+        return y, h, rstd
+
+    def rmsnorm_quant_bwd(h, w, rstd, dy, add=None):
+        count["rmsnorm_quant_bwd"] += 1
+        dx, dw = calls["rmsnorm_quant_bwd"](h, w, rstd, dy, add)
+        r, xh, g = rstd.double()[:, None], h.double() * rstd.double()[:, None], dy.double() * w.double()
+        more = 0 if add is None else add.double()
+        want, size = r * (g - xh * (g * xh).mean(-1, keepdim=True)) + more, r * (g.abs() + xh.abs() * (g * xh).abs().mean(-1, keepdim=True)) + abs(more)
+        assert ((dx.double() - want).abs() <= want.abs() * HALF[h.dtype] + size * 60 * 2.0 ** -24).all()
+        assert ((dw.double() - (dy.double() * xh).sum(0)).abs() <= (dy.double() * xh).abs().sum(0) * (h.shape[0] / 100 + 150) * 2.0 ** -24).all()
+        return dx, dw
+
+    for k, f in dict(quantize=quantize, quantize_both=quantize_both, matmul=matmul, rmsnorm_quant=rmsnorm_quant, rmsnorm_quant_bwd=rmsnorm_quant_bwd).items():
+        monkeypatch.setattr(F, k, f)
+    eng = _engine(dev, fp8=True, activation_budget_gb=-1.0 if level is None else 0.0)
+    try:
+        if level is not None:
+            eng.model.layer_levels = [level, level]
+        _gradients(eng)
+        # of each layer four products forward and eight back; again QKV, output and gate | up, or what of them is not kept
+        assert count["quantize_both"] == count["rmsnorm_quant_bwd"] * 2 == 8 and count["matmul"] >= 2 * (12 + (3, 1, 0)[level or 0]), count
+    finally:
+        eng.close()
+
+
+@pytest.mark.parametrize("level,ranks", [(None, "one"), (0, "one"), (1, "one"), (2, "one"), (0, "as of several"), (1, "as of several"),
+                                         (2, "as of several")])
+def test_how_the_layers_in_8_bits_are_put_together(dev, level, ranks, monkeypatch):
+    """With quantizers that round nothing the layers are those of the model in 16 bits, up to roundings to 16 bits: of a gradient's
+    eleven products two operands and a result each, in two forms, 66 roundings of 2^-8 / sqrt(3) in the mean: 2^-5.8; 2^-5
+    allowed.  ``as of several``: the form that tensor parallelism takes, with sums over one rank."""
+    budget = -1.0 if level is None else 0.0
+    eng, other = _engine(dev, fp8=True, activation_budget_gb=budget), _engine(dev, activation_budget_gb=budget)
+    kept = lambda x, block=(1, 128): F.BlockScaled(x.float(), torch.ones(1, device=dev), block)  # noqa: E731
+
+    def norm(x, w, eps=1e-5, residual=None):
+        h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+        rstd = torch.rsqrt(h.float().square().mean(-1) + eps)
+        return kept(h.float() * rstd[:, None] * w.float()), h, rstd
+
+    def product(a, b, *, trans_a=False, trans_b=True, out_dtype=torch.bfloat16, add=None, out=None):
+        got = (a.codes.t() if trans_a else a.codes) @ (b.codes.t() if trans_b else b.codes) + (0 if add is None else add.float())
+        return got.to(out_dtype) if out is None else out.copy_(got)
+
+    try:
+        if level is not None:
+            for e in (eng, other):
+                e.model.layer_levels = [level, level]
+        loss0, want = _gradients(other)
+        for k, f in dict(quantize=kept, quantize_both=lambda x: (kept(x), kept(x)), matmul=product, rmsnorm_quant=norm).items():
+            monkeypatch.setattr(F, k, f)
+        if ranks != "one":
+            eng.model.tp_group, eng.model.tp_sum = object(), lambda t: t
+        loss, grads = _gradients(eng)
+        assert abs(loss - loss0) <= 2.0 ** -9 * loss0
+        off = {k: ((g - want[k]).norm() / want[k].norm()).item() for k, g in grads.items()}
+        assert max(off.values()) <= 2.0 ** -5, sorted(off.items(), key=lambda t: -t[1])[:4]
+    finally:
+        eng.close()
+        other.close()
+
+
+@pytest.mark.parametrize("level", [0, 2])
+def test_layers_in_8_bits_add_to_gradients(dev, level):
+    """With ``accumulate_grads`` a layer adds to what is there, rounded once: a gradient of its own is rounded when it is written,
+    the sum when it is."""
+    eng = _engine(dev, fp8=True, activation_budget_gb=0.0)
+    try:
+        eng.model.layer_levels = [level, level]
+        plan = eng.plans.get(0)
+        inputs = eng.stage_inputs(plan)
+
+        def run(base):
+            eng.model.grads_flat.copy_(base)
+            eng.model.loss(*inputs, 1.0 / plan.n_global_tokens).backward()
+            torch.cuda.synchronize()
+            return {k: t.grad.double().clone() for k, t in eng.model.p.items()}
+
+        base = torch.zeros_like(eng.model.grads_flat)
+        own = run(base)
+        base.copy_(torch.randn(base.shape, device=dev) * eng.model.grads_flat.float().std())
+        eng.model.accumulate_grads = True
+        got = run(base)
+        eng.model.grads_flat.copy_(base)
+        there = {k: t.grad.double().clone() for k, t in eng.model.p.items()}
+        for k in own:
+            if not k.startswith("l"):
+                continue
+            near = 2.0 ** -8 * (own[k].abs() + (own[k] + there[k]).abs() * (1 + 2.0 ** -7))
+            off = (got[k] - own[k] - there[k]).abs()
+            if k in ("l1.wd", "l1.wgu", "l1.norm2"):
+                assert (off <= near).all(), k    # nothing before them adds in an order that may differ
+            # attention's dQ does
+            assert off.norm() <= near.norm() + 2.0 ** -8 * own[k].norm(), k
+        # and a second time over the same codes
+        again = run(base)
+        for k in ("l1.wd", "l1.wgu", "l1.norm2"):
+            assert torch.equal(again[k], got[k]), k
+    finally:
+        eng.close()
