@@ -672,10 +672,14 @@ static GemmPlan plan_gemm(long p_rows, long q_rows, bool q_rows_inner, int k, in
   g.tiles_p = (p_rows + 255) / 256;
   g.tiles_q = (q_rows + 255) / 256;
   const long pair_tiles = g.tiles_p * g.tiles_q;
-  // Pairs where their tiles give two thirds of them work, or fewer tiles long sums, which are cut; us with pairs / split:
+  // Pairs where their tiles give two thirds of them work, or fewer tiles long sums, which are cut, or where the other kernel,
+  // which is not persistent, has more CTAs than processors and so a second round; us with pairs / split:
   // 2048 x 1536 x 1024 (48 tiles) 9.5 / 12.4, 200 x 28672 x 4096 (112) 32 / 49, 1024 x 2048 x 4096 (32) 18.4 / 13.5, 512 x 4096 x
-  // 14336 (32) 32.5 / 34.8, 1536 x 1024 x 16384 (24) 28 / 37, 512 x 1024 x 4096 (8) 14.3 / 10.5.
-  g.pairs = form == 1 || (form == 0 && q_rows > 128 && (pair_tiles >= 48 || pair_tiles * ((k + 127) / 128) >= 2304));
+  // 14336 (32) 32.5 / 34.8, 1536 x 1024 x 16384 (24) 28 / 37, 512 x 1024 x 4096 (8) 14.3 / 10.5; a second round, from cold: 256 x
+  // 9728 x 4096 (38 tiles, 152 CTAs) 23.6 / 31.7, 512 x 5120 x 5120 (40, 160) 25.6 / 33.8, 768 x 3328 x 512 (39, 156) 13.3 / 15.4, 256 x
+  // 12032 x 2048 (47, 188) 19.5 / 23.6; none: 1536 x 1536 x 2048 (36, 144) 21.5 / 13.3, 300 x 5120 x 4096 (40, 120) 22.8 / 18.5.
+  const long split_ctas = ((p_rows + 127) / 128) * ((q_rows + 127) / 128);
+  g.pairs = form == 1 || (form == 0 && q_rows > 128 && (pair_tiles >= 48 || pair_tiles * ((k + 127) / 128) >= 2304 || split_ctas > 2 * kGemmPairs));
   if (g.pairs) {
     g.n = 256;
     const int rest = int(pair_tiles % kGemmPairs);

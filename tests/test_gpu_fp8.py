@@ -1219,3 +1219,11 @@ def test_layers_in_8_bits_add_to_gradients(dev, level):
             assert torch.equal(again[k], got[k]), k
     finally:
         eng.close()
+
+
+@pytest.mark.parametrize("how", ["forward", "dgrad", "wgrad"])
+@pytest.mark.parametrize("m,n,k", [(512, 5120, 300), (256, 9729, 130), (300, 5120, 513), (768, 3328, 1000), (1535, 1537, 257)])
+def test_matmul_around_a_round_of_small_tiles(dev, how, m, n, k):
+    """Outputs of about as many tiles of 128 x 128 as there are processors, where the rule goes from one kernel to the other."""
+    a, b, kw = _operands(m, n, k, how, dev)
+    _check_product(F.matmul(a, b, **kw), a, b, kw)
