@@ -156,6 +156,20 @@ __global__ void __launch_bounds__(256) grad_sqnorm_kernel(GradPtrs grads, int wo
     unpack_f32x2(sq_2[j], lo, hi);
     t += double(lo) + double(hi);
   }
+  // Squares that fp32 does not hold: again in 64 bits.  One gradient of 1e20 would make the norm infinite, and all that it clips
+  // zero.  (Of one rank: sums over ranks are kept in 32 bits.)
+  if (kOne && !(t < double(INFINITY))) {
+    t = 0.0;
+    for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n_vec; i += stride) {
+      const uint4 raw = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(grads.p[0]) + shard_off)[i];
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double lo = double(__uint_as_float(w[j] << 16)) * double(scale), hi = double(__uint_as_float(w[j] & 0xffff0000u)) * double(scale);
+        t += lo * lo + hi * hi;
+      }
+    }
+  }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
   __shared__ double part[8];

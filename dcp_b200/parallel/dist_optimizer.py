@@ -376,4 +376,6 @@ class ShardedAdamW:
         self.bufs.arena.check_status()
 
     def grad_norm(self) -> float:
-        return float(self.sq_norm.sqrt().item())
+        """Norm of the gradients of the last step that clipped (of one rank without tensor parallelism: summed in 64 bits)."""
+        one = not self.overlap and self.tp_group is None
+        return float((self.sq_sum[0] if one else self.sq_norm).sqrt().item())

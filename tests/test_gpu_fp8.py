@@ -1227,3 +1227,20 @@ def test_matmul_around_a_round_of_small_tiles(dev, how, m, n, k):
     """Outputs of about as many tiles of 128 x 128 as there are processors, where the rule goes from one kernel to the other."""
     a, b, kw = _operands(m, n, k, how, dev)
     _check_product(F.matmul(a, b, **kw), a, b, kw)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("at", [0, 4103, 12_110, 30_003])
+def test_sharded_optimizer_clips_a_gradient_whose_square_fp32_does_not_hold(dev, bits, at):
+    bufs, opt = _sharded(dev, bits)
+    _grads(bufs, 0)
+    bufs.grads[at] = 1e20
+    length = bufs.grads.double().norm().item()
+    w = opt.master.double()
+    opt.step()
+    assert abs(opt.grad_norm() / length - 1) <= 2.0 ** -20
+    # the first step is g / (|g| + eps) of the clipped gradient, whatever its length: the one moves by lr, the others, 1e-20 of it, not
+    g = bufs.grads.double() * (0.5 / length)
+    want = w - 1e-2 * (g / (g.abs() + 1e-8) + 0.1 * w)
+    # m / (sqrt(v) + eps) of a dozen roundings, and moments that are not rounded yet
+    assert ((opt.master.double() - want).abs() <= 1e-2 * 2.0 ** -18 + w.abs() * 2.0 ** -23).all()
