@@ -28,7 +28,7 @@ namespace {
 
 constexpr long kBlock = 128, kStateBlock = 256, kNormWidth = 16384;
 constexpr size_t kStatusWords = 4;
-constexpr long kMaxRows = 0x7fffffff, kMaxBlocked = kMaxRows - (kBlock - 1);   // the kernels count in ints, in whole blocks along a block
+constexpr long kMaxRows = 0x7fffffff, kMaxBlocked = kMaxRows - (kBlock - 1);   // the kernels count in ints, along a row in whole blocks
 
 void check(int rc, const char* what) {
   if (rc != 0) throw std::runtime_error(std::string(what) + " failed with code " + std::to_string(rc));

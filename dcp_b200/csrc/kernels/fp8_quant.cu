@@ -1,7 +1,8 @@
 // Makers of 8-bit codes (see fp8_common.cuh), all bound by HBM in bf16 and fp32 rows on 16 bytes: 16384 x 4096 bf16 with a
 // residual 72 us (6.6 TB/s; copying runs at 6.55), its backward with an addition 81 (6.7), by rows 31 (6.4), by blocks 30
 // (6.7); both ways at once 48 (5.6: 80 registers leave three CTAs to an SM, 36 % of its warps, which do not cover two barriers
-// and a walk through shared memory; 61 % of the issue slots are used).  Rows that do not begin on 16 bytes run at 2.7 to 3.6 TB/s, in fp32 at 2.8 to 4.8.
+// and a walk through shared memory; 61 % of the issue slots are used).  Rows that do not begin on 16 bytes run at 2.7 to 3.6 TB/s,
+// in fp32 at 2.8 to 4.8.
 //
 //  fp8_norm        h = x + residual, rounded to x's type; y = h * rsqrt(mean(h^2) + eps) * w as codes with a scale per 128
 //                  channels.  One CTA per row, the row in registers: x and the residual are read once, h and the codes written

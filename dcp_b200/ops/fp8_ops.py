@@ -13,10 +13,10 @@ A product's scales have to run along the contraction in blocks of 128, so
 * ``dw = dy^T x``   takes both by tokens (128 x 1):                         ``matmul(dy, x, trans_a=True, trans_b=False)``
 
 ``linear`` and ``norm_linear`` are these three as autograd functions (of a first derivative; a second is refused); the pieces
-that they are made of pass no gradient on.  On a CUDA tensor the kernels always run (a missing library raises); CPU tensors take the plain forms.  All calls run on the
-current stream of their tensors' device, allocate their results there and may be captured into a CUDA graph once a call has
-been made on the device.  (As with torch's own functions, a backward pass is captured together with its forward pass, not
-while an eager graph of the same leaves lives.)
+that they are made of pass no gradient on.  On a CUDA tensor the kernels always run (a missing library raises); CPU tensors
+take the plain forms.  All calls run on the current stream of their tensors' device, allocate their results there and may be
+captured into a CUDA graph once a call has been made on the device.  (As with torch's own functions, a backward pass is
+captured together with its forward pass, not while an eager graph of the same leaves lives.)
 """
 from __future__ import annotations
 
